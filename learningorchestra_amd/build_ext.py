@@ -28,6 +28,7 @@ SOURCES = [
     os.path.join(CSRC, "tree_hist.hip"),
     os.path.join(CSRC, "embedding.hip"),
     os.path.join(CSRC, "batchnorm.hip"),
+    os.path.join(CSRC, "layernorm.hip"),
 ]
 
 

@@ -131,6 +131,18 @@ void launch_embedding_fwd(const void* ids, const void* table, void* out,
                           long n, int dim, hipStream_t s);
 void launch_embedding_bwd(const void* ids, const void* dy, void* gtable,
                           long n, int dim, hipStream_t s);
+void launch_layernorm_fwd(int dtype, const void* x, long ldx, const void* res,
+                          long ldr, const float* gamma, const float* beta,
+                          void* y, long ldy, void* sum, long lds, float* mean,
+                          float* invstd, long rows, int cols, float eps,
+                          hipStream_t s);
+int layernorm_bwd_parts(int dtype, long rows, int cols);
+void launch_layernorm_bwd(int dtype, const void* dy, long ldy, const void* x,
+                          long ldx, const void* skip, long ldk,
+                          const float* mean, const float* invstd,
+                          const float* gamma, void* dx, long ldd, float* part,
+                          float* dgamma, float* dbeta, long rows, int cols,
+                          hipStream_t s);
 }  // namespace lo
 
 namespace {
@@ -671,6 +683,127 @@ void embedding_bwd(at::Tensor ids, at::Tensor dy, at::Tensor gtable) {
                            ids.numel(), dim, stream());
 }
 
+// ----------------------------------------------------------- layernorm ----
+int float_code(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be on GPU");
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return 0;
+    case at::kHalf: return 1;
+    case at::kFloat: return 2;
+    default: TORCH_CHECK(false, name, " must be bf16, fp16 or fp32");
+  }
+}
+
+void check_launch(const char* name) {
+  const hipError_t e = hipGetLastError();
+  TORCH_CHECK(e == hipSuccess, name, ": ", hipGetErrorString(e));
+}
+
+// rows of like's shape, type and device; the row stride is free. out: written
+// to, so its rows may not overlap
+void check_rows(const at::Tensor& t, const at::Tensor& like, const char* name,
+                bool out) {
+  TORCH_CHECK(t.dim() == 2 && t.sizes() == like.sizes(), name,
+              " must have the input's shape");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name,
+              " must have the input's type");
+  TORCH_CHECK(t.device() == like.device(), name,
+              " must be on the input's device");
+  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name,
+              " must be contiguous along its columns");
+  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= (out ? t.size(1) : 0), name,
+              out ? " must not overlap itself" : " has a negative row stride");
+}
+
+void check_vec(const at::Tensor& t, const at::Tensor& like, int64_t n,
+               const char* name) {
+  check_f32(t, name);
+  TORCH_CHECK(t.device() == like.device(), name,
+              " must be on the input's device");
+  TORCH_CHECK(t.numel() == n, name, " must hold ", n, " values");
+}
+
+constexpr int64_t kLayerNormCols = 32768;  // a row fits one block's registers
+
+void check_layernorm(const at::Tensor& x) {
+  TORCH_CHECK(x.dim() == 2, "x must be [rows, cols]");
+  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= kLayerNormCols,
+              "layer norm takes 1 to ", kLayerNormCols, " columns");
+}
+
+void layernorm_fwd(at::Tensor x, at::Tensor gamma, at::Tensor beta, double eps,
+                   at::Tensor out, c10::optional<at::Tensor> mean,
+                   c10::optional<at::Tensor> invstd,
+                   c10::optional<at::Tensor> residual,
+                   c10::optional<at::Tensor> sum_out) {
+  const int code = float_code(x, "x");
+  check_layernorm(x);
+  const int64_t rows = x.size(0), cols = x.size(1);
+  check_rows(x, x, "x", false);
+  check_rows(out, x, "out", true);
+  check_vec(gamma, x, cols, "gamma");
+  check_vec(beta, x, cols, "beta");
+  TORCH_CHECK(mean.has_value() == invstd.has_value(),
+              "mean and invstd come together");
+  if (mean) {
+    check_vec(*mean, x, rows, "mean");
+    check_vec(*invstd, x, rows, "invstd");
+  }
+  TORCH_CHECK(!sum_out || residual, "sum_out needs a residual");
+  if (residual) check_rows(*residual, x, "residual", false);
+  if (sum_out) {
+    check_rows(*sum_out, x, "sum_out", true);
+    TORCH_CHECK(rows == 0 || sum_out->data_ptr() != out.data_ptr(),
+                "out and sum_out must be two tensors");
+  }
+  if (rows == 0) return;
+  const c10::DeviceGuard guard(x.device());
+  lo::launch_layernorm_fwd(
+      code, x.data_ptr(), x.stride(0), residual ? residual->data_ptr() : nullptr,
+      residual ? residual->stride(0) : 0, gamma.data_ptr<float>(),
+      beta.data_ptr<float>(), out.data_ptr(), out.stride(0),
+      sum_out ? sum_out->data_ptr() : nullptr, sum_out ? sum_out->stride(0) : 0,
+      mean ? mean->data_ptr<float>() : nullptr,
+      invstd ? invstd->data_ptr<float>() : nullptr, rows, (int)cols,
+      (float)eps, stream());
+  check_launch("layernorm_fwd");
+}
+
+void layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor mean,
+                   at::Tensor invstd, at::Tensor gamma, at::Tensor dgamma,
+                   at::Tensor dbeta, at::Tensor dx,
+                   c10::optional<at::Tensor> dskip) {
+  const int code = float_code(x, "x");
+  check_layernorm(x);
+  const int64_t rows = x.size(0), cols = x.size(1);
+  check_rows(x, x, "x", false);
+  check_rows(dy, x, "dy", false);
+  check_rows(dx, x, "dx", true);
+  if (dskip) check_rows(*dskip, x, "dskip", false);
+  check_vec(mean, x, rows, "mean");
+  check_vec(invstd, x, rows, "invstd");
+  check_vec(gamma, x, cols, "gamma");
+  check_vec(dgamma, x, cols, "dgamma");
+  check_vec(dbeta, x, cols, "dbeta");
+  const c10::DeviceGuard guard(x.device());
+  if (rows == 0) {
+    dgamma.zero_();
+    dbeta.zero_();
+    return;
+  }
+  at::Tensor part;
+  const int n = lo::layernorm_bwd_parts(code, rows, (int)cols);
+  if (n) part = at::empty({n, 2, cols}, gamma.options());
+  lo::launch_layernorm_bwd(
+      code, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
+      dskip ? dskip->data_ptr() : nullptr, dskip ? dskip->stride(0) : 0,
+      mean.data_ptr<float>(), invstd.data_ptr<float>(),
+      gamma.data_ptr<float>(), dx.data_ptr(), dx.stride(0),
+      n ? part.data_ptr<float>() : nullptr, dgamma.data_ptr<float>(),
+      dbeta.data_ptr<float>(), rows, (int)cols, stream());
+  check_launch("layernorm_bwd");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -717,6 +850,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("mean"), py::arg("invstd"), py::arg("M"),
         py::arg("rmean") = py::none(), py::arg("rvar") = py::none(),
         py::arg("momentum") = 0.0, py::arg("eps") = 1e-5);
+  m.def("layernorm_fwd", &layernorm_fwd, py::arg("x"), py::arg("gamma"),
+        py::arg("beta"), py::arg("eps"), py::arg("out"),
+        py::arg("mean") = py::none(), py::arg("invstd") = py::none(),
+        py::arg("residual") = py::none(), py::arg("sum_out") = py::none());
+  m.def("layernorm_bwd", &layernorm_bwd, py::arg("dy"), py::arg("x"),
+        py::arg("mean"), py::arg("invstd"), py::arg("gamma"),
+        py::arg("dgamma"), py::arg("dbeta"), py::arg("dx"),
+        py::arg("dskip") = py::none());
   m.def("add_relu", &add_relu);
   m.def("avgpool_global", &avgpool_global);
   m.def("avgpool_global_bwd", &avgpool_global_bwd);

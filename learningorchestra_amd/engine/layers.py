@@ -634,6 +634,77 @@ class BatchNormReLU(Layer):
                 self.running_var.device))
 
 
+class LayerNorm(Layer):
+    '''Layer norm over the last axis (layernorm.hip), the norm that does not
+    depend on the batch: same result for one text as inside a batch, no
+    running state. gamma/beta in the arena.'''
+
+    def __init__(self, name: str, channels: int, eps: float = 1e-5):
+        assert 1 <= channels <= 32768
+        self.name = name
+        self.c = channels
+        self.eps = eps
+        self.arena: Optional[ParamArena] = None
+        self._bufs = {}
+
+    def build(self, arena: ParamArena) -> None:
+        self.arena = arena
+        arena.add(self.name + ".g", (self.c,), torch.ones(self.c))
+        arena.add(self.name + ".b", (self.c,), torch.zeros(self.c))
+
+    def param_names(self):
+        return [self.name + ".g", self.name + ".b"]
+
+    def _alloc(self, x):
+        key = (tuple(x.shape), x.dtype)
+        if self._bufs.get("key") != key:
+            M = x.numel() // self.c
+            dev = x.device
+            self._bufs = {
+                "key": key, "M": M,
+                "y": torch.empty((M, self.c), device=dev, dtype=x.dtype),
+                "dx": torch.empty((M, self.c), device=dev, dtype=x.dtype),
+                "mean": torch.empty(M, device=dev),
+                "invstd": torch.empty(M, device=dev),
+            }
+        return self._bufs
+
+    def forward(self, x: torch.Tensor,
+                residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``residual``: normalise x + residual; the sum stays in
+        ``self.sum`` (x's shape) for the skip path."""
+        assert x.shape[-1] == self.c
+        bufs = self._alloc(x)
+        x2 = x.reshape(bufs["M"], self.c)
+        self._x2 = x2
+        if residual is not None:
+            if "sum" not in bufs:
+                bufs["sum"] = torch.empty_like(bufs["y"])
+            self._x2 = bufs["sum"]
+            residual = residual.reshape(bufs["M"], self.c)
+        F.layernorm_fwd(x2, self.arena.pf(self.name + ".g"),
+                        self.arena.pf(self.name + ".b"), self.eps, bufs["y"],
+                        mean=bufs["mean"], invstd=bufs["invstd"],
+                        residual=residual,
+                        sum_out=bufs["sum"] if residual is not None else None)
+        self.sum = self._x2.view(x.shape) if residual is not None else None
+        return bufs["y"].view(x.shape)
+
+    def backward(self, dy: torch.Tensor,
+                 dskip: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``dskip``: gradient that reached ``self.sum`` past the norm. The
+        result is the gradient of x and of the residual alike."""
+        bufs = self._bufs
+        if dskip is not None:
+            dskip = dskip.reshape(bufs["M"], self.c)
+        F.layernorm_bwd(dy.reshape(bufs["M"], self.c), self._x2, bufs["mean"],
+                        bufs["invstd"], self.arena.pf(self.name + ".g"),
+                        self.arena.g(self.name + ".g"),
+                        self.arena.g(self.name + ".b"), bufs["dx"],
+                        dskip=dskip)
+        return bufs["dx"].view(dy.shape)
+
+
 class AvgPoolGlobal(Layer):
     '''Global average pool [B,H,W,C] -> [B,C] (batchnorm.hip kernels).'''
 

@@ -503,6 +503,90 @@ def bn_bwd(dy2d: torch.Tensor, y2d: torch.Tensor, x2d: torch.Tensor,
     dx.copy_(d.to(dx.dtype))
 
 
+# --------------------------------------------------------------- layernorm
+def layernorm_fwd(x2d: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor,
+                  eps: float, out: torch.Tensor,
+                  mean: Optional[torch.Tensor] = None,
+                  invstd: Optional[torch.Tensor] = None,
+                  residual: Optional[torch.Tensor] = None,
+                  sum_out: Optional[torch.Tensor] = None) -> None:
+    """Layer norm over the rows of x2d [M, C] (bf16, fp16 or fp32, any row
+    stride, 1 <= C <= 32768) with fp32 gamma/beta [C]. Writes out (x2d's type)
+    and, for training, mean and invstd (fp32 [M]). ``residual`` [M, C] is
+    added first; the sum, rounded to x2d's type, is what gets normalised and
+    goes to ``sum_out`` (the backward pass's x2d). ``out`` and ``sum_out`` may
+    be one of the inputs."""
+    if _is_gpu(x2d):
+        require_ext().layernorm_fwd(x2d, gamma, beta, eps, out, mean, invstd,
+                                    residual, sum_out)
+        return
+    _check_layernorm(x2d, (out, residual, sum_out), (gamma, beta),
+                     (mean, invstd))
+    if (mean is None) != (invstd is None):
+        raise RuntimeError("mean and invstd come together")
+    if sum_out is not None and residual is None:
+        raise RuntimeError("sum_out needs a residual")
+    s = x2d
+    if residual is not None:
+        s = (x2d.float() + residual.float()).to(x2d.dtype)
+    xf = s.float()
+    mu = xf.mean(1, keepdim=True)
+    rstd = ((xf - mu).square().mean(1, keepdim=True) + eps).rsqrt()
+    y = ((xf - mu) * rstd * gamma + beta).to(out.dtype)
+    if sum_out is not None:
+        sum_out.copy_(s)
+    out.copy_(y)
+    if mean is not None:
+        mean.copy_(mu.view(-1))
+        invstd.copy_(rstd.view(-1))
+
+
+def layernorm_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, mean: torch.Tensor,
+                  invstd: torch.Tensor, gamma: torch.Tensor,
+                  dgamma: torch.Tensor, dbeta: torch.Tensor, dx: torch.Tensor,
+                  dskip: Optional[torch.Tensor] = None) -> None:
+    """Layer norm backward from what ``layernorm_fwd`` normalised (x2d, or its
+    ``sum_out``) and its mean/invstd. Writes dgamma, dbeta (fp32 [C],
+    overwritten; the same sums on every run) and dx. ``dskip`` [M, C], the
+    gradient that reaches the sum past the norm, is added to dx, which then is
+    the gradient of x and of the residual alike."""
+    if _is_gpu(x2d):
+        require_ext().layernorm_bwd(dy2d, x2d, mean, invstd, gamma, dgamma,
+                                    dbeta, dx, dskip)
+        return
+    _check_layernorm(x2d, (dy2d, dx, dskip), (gamma, dgamma, dbeta),
+                     (mean, invstd))
+    g = dy2d.float()
+    xhat = (x2d.float() - mean.view(-1, 1)) * invstd.view(-1, 1)
+    h = g * gamma
+    d = invstd.view(-1, 1) * (h - h.mean(1, keepdim=True)
+                              - xhat * (h * xhat).mean(1, keepdim=True))
+    if dskip is not None:
+        d = d + dskip.float()
+    dgamma.copy_((g * xhat).sum(0))
+    dbeta.copy_(g.sum(0))
+    dx.copy_(d.to(dx.dtype))
+
+
+def _check_layernorm(x, rows, vecs, stats) -> None:
+    # the CPU path refuses what the kernels' bindings refuse
+    if x.dim() != 2 or not 1 <= x.shape[1] <= 32768:
+        raise RuntimeError("layer norm takes [rows, 1 to 32768 columns]")
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise RuntimeError("x must be bf16, fp16 or fp32")
+    for t in rows:
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype
+                              or t.device != x.device):
+            raise RuntimeError("activations must have the input's shape, "
+                               "type and device")
+    for group, n in ((vecs, x.shape[1]), (stats, x.shape[0])):
+        for t in group:
+            if t is not None and (t.numel() != n or t.dtype != torch.float32
+                                  or t.device != x.device):
+                raise RuntimeError(f"statistics and parameters must be fp32 "
+                                   f"with {n} values")
+
+
 # ------------------------------------------------------------ residual add
 def add_relu(a: torch.Tensor, b: torch.Tensor, out: Optional[torch.Tensor] = None,
              relu: bool = True) -> torch.Tensor:

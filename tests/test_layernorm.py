@@ -1,0 +1,415 @@
+"""Layer norm, forward and backward, against the definition in 64 bits.
+
+Tolerances. u = 2^-24 is fp32's largest relative rounding error, half(T) the
+output type's. A row's sums take at most 64 roundings on any path (32 elements
+in a thread, 6 shuffle levels, 16 waves, a few more), so mean is off by at most
+64 u avg|x|, the variance by 64 u relative (its own sum) plus the square of the
+former, invstd by 32 u and four more operations. That makes
+    xhat:  ex = u (64 invstd avg|x| + 40 |xhat|)
+    y:     half |y| + |gamma| ex + 4 u (|gamma xhat| + |beta|)
+    dx:    half |dx| + invstd (4 u |h| + dc1 + |xhat| dc2 + |c2| ex)
+           + 40 u |dx|,  dc1 = 66 u avg|h|, dc2 = 66 u avg|h xhat| + avg(|h| ex)
+    dgamma: (rows/512 + 100) u sum|dy xhat| + sum(|dy| ex)
+    dbeta:  (rows/512 + 100) u sum|dy|
+where a thread adds at most rows/512 + 1 rows in turn and 100 covers the joins.
+"""
+import pytest
+import torch
+
+from learningorchestra_amd.engine.arena import ParamArena
+from learningorchestra_amd.engine.layers import LayerNorm
+from learningorchestra_amd.ops import functional as F
+
+U = 2.0 ** -24
+EPS = 1e-5
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+SIZES = [(1, 1), (3, 2), (5, 7), (1, 8), (9, 9), (130, 16), (17, 63), (64, 128),
+         (33, 129), (70, 250), (2, 384), (11, 515), (2, 1000), (7, 1537),
+         (1031, 24), (5, 2050), (3, 4100), (2, 8192), (2, 9001), (1, 20000),
+         (2, 32768)]
+
+
+def _data(rows, cols, dtype, device, seed=0, shift=0.5):
+    g = torch.Generator().manual_seed(seed)
+    d = {"x": (torch.randn(rows, cols, generator=g)
+               + shift * torch.randn(cols, generator=g)).to(dtype),
+         "residual": torch.randn(rows, cols, generator=g).to(dtype),
+         "dy": torch.randn(rows, cols, generator=g).to(dtype),
+         "dskip": torch.randn(rows, cols, generator=g).to(dtype),
+         "gamma": 1 + 0.2 * torch.randn(cols, generator=g),
+         "beta": 0.2 * torch.randn(cols, generator=g)}
+    return {k: v.to(device) for k, v in d.items()}
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _reference(s, d, dtype, dskip=None):
+    """64-bit results and their tolerances from the normalised input s."""
+    x, dy = s.double().cpu(), d["dy"].double().cpu()
+    gamma, beta = d["gamma"].double().cpu(), d["beta"].double().cpu()
+    mean = x.mean(1, keepdim=True)
+    invstd = ((x - mean).square().mean(1, keepdim=True) + EPS).rsqrt()
+    xhat = (x - mean) * invstd
+    ex = U * (64 * invstd * x.abs().mean(1, keepdim=True) + 40 * xhat.abs())
+    y = xhat * gamma + beta
+    h = dy * gamma
+    c1, c2 = h.mean(1, keepdim=True), (h * xhat).mean(1, keepdim=True)
+    dn = invstd * (h - c1 - xhat * c2)
+    dx = dn if dskip is None else dn + dskip.double().cpu()
+    dc1 = 66 * U * h.abs().mean(1, keepdim=True)
+    dc2 = (66 * U * (h * xhat).abs().mean(1, keepdim=True)
+           + (h.abs() * ex).mean(1, keepdim=True))
+    depth = (x.shape[0] / 512 + 100) * U
+    half = _half(dtype)
+    ref = {"y": y, "mean": mean.view(-1), "invstd": invstd.view(-1), "dx": dx,
+           "dgamma": (dy * xhat).sum(0), "dbeta": dy.sum(0)}
+    # an fp16 result below the normal range is off by half its smallest step
+    tiny = torch.finfo(dtype).smallest_normal * half
+    tol = {"y": half * y.abs() + gamma.abs() * ex
+           + 4 * U * ((gamma * xhat).abs() + beta.abs()) + tiny,
+           "mean": 64 * U * x.abs().mean(1) + 1e-30,
+           "invstd": 40 * U * invstd.view(-1),
+           "dx": half * dx.abs() + 40 * U * (dn.abs() + dx.abs()) + tiny
+           + invstd * (4 * U * h.abs() + dc1 + xhat.abs() * dc2
+                       + c2.abs() * ex),
+           "dgamma": depth * (dy * xhat).abs().sum(0)
+           + (dy.abs() * ex).sum(0) + 1e-30,
+           "dbeta": depth * dy.abs().sum(0) + 1e-30}
+    # the square of mean's own error, where it shows beside var + eps
+    tol["invstd"] = tol["invstd"] + 0.5 * invstd.view(-1) ** 3 \
+        * tol["mean"] ** 2
+    return ref, tol
+
+
+def _close(got, ref, tol, name):
+    err = (got.double().cpu() - ref).abs()
+    assert bool((err <= tol).all()), \
+        f"{name}: off by {(err / tol).max().item():.2f} tolerances"
+
+
+def _forward(d, residual, out=None):
+    x = d["x"]
+    o = {"y": torch.empty_like(x) if out is None else out,
+         "mean": torch.empty(x.shape[0], device=x.device),
+         "invstd": torch.empty(x.shape[0], device=x.device)}
+    s = x
+    if residual:
+        s = o["sum"] = torch.empty_like(x)
+    F.layernorm_fwd(x, d["gamma"], d["beta"], EPS, o["y"], mean=o["mean"],
+                    invstd=o["invstd"], residual=d["residual"] if residual
+                    else None, sum_out=o.get("sum"))
+    return s, o
+
+
+def _backward(s, o, d, dskip):
+    g = {"dx": torch.empty_like(s),
+         "dgamma": torch.full_like(d["gamma"], 7.0),
+         "dbeta": torch.full_like(d["beta"], 7.0)}
+    F.layernorm_bwd(d["dy"], s, o["mean"], o["invstd"], d["gamma"],
+                    g["dgamma"], g["dbeta"], g["dx"],
+                    dskip=d["dskip"] if dskip else None)
+    return g
+
+
+@pytest.mark.parametrize("skip", [False, True])
+@pytest.mark.parametrize("rows,cols", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_and_backward(device, dtype, rows, cols, skip):
+    d = _data(rows, cols, dtype, device)
+    s, o = _forward(d, skip)
+    if skip:
+        want = (d["x"].float() + d["residual"].float()).to(dtype)
+        assert torch.equal(o["sum"], want)
+    g = _backward(s, o, d, skip)
+    ref, tol = _reference(s, d, dtype, d["dskip"] if skip else None)
+    for k in ("y", "mean", "invstd"):
+        _close(o[k], ref[k], tol[k], k)
+    for k in ("dx", "dgamma", "dbeta"):
+        _close(g[k], ref[k], tol[k], k)
+    # without statistics: the same output
+    y = torch.empty_like(d["x"])
+    F.layernorm_fwd(d["x"], d["gamma"], d["beta"], EPS, y,
+                    residual=d["residual"] if skip else None)
+    assert torch.equal(y, o["y"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(70000, 8), (20011, 40), (9000, 1000),
+                                       (3000, 4096), (1500, 9000)])
+def test_many_rows(rows, cols):
+    d = _data(rows, cols, torch.bfloat16, "cuda")
+    s, o = _forward(d, False)
+    g = _backward(s, o, d, False)
+    ref, tol = _reference(s, d, torch.bfloat16)
+    _close(o["y"], ref["y"], tol["y"], "y")
+    for k in g:
+        _close(g[k], ref[k], tol[k], k)
+    again = _backward(s, o, d, False)
+    for k in g:
+        assert torch.equal(g[k], again[k]), k
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_row_strides_and_neighbours(device, dtype):
+    """Row strides and starts that no vector load is aligned to, and nothing
+    written outside the rows."""
+    rows, cols = 37, 203
+    d = _data(rows, cols, dtype, device)
+
+    def strided(t, lead, pad):
+        wide = torch.full((rows, cols + lead + pad), 5.0, dtype=dtype,
+                          device=device)
+        wide[:, lead:lead + cols] = t
+        return wide, wide[:, lead:lead + cols]
+
+    e = dict(d)
+    for i, k in enumerate(("x", "residual", "dy", "dskip")):
+        e[k] = strided(d[k], i + 1, 3)[1]
+    wide_y, y = strided(torch.zeros_like(d["x"]), 1, 4)
+    wide_s, sm = strided(torch.zeros_like(d["x"]), 3, 2)
+    wide_d, dx = strided(torch.zeros_like(d["x"]), 5, 1)
+    mean = torch.empty(rows, device=device)
+    invstd = torch.empty(rows, device=device)
+    F.layernorm_fwd(e["x"], e["gamma"], e["beta"], EPS, y, mean=mean,
+                    invstd=invstd, residual=e["residual"], sum_out=sm)
+    dg, db = torch.empty_like(d["gamma"]), torch.empty_like(d["beta"])
+    F.layernorm_bwd(e["dy"], sm, mean, invstd, e["gamma"], dg, db, dx,
+                    dskip=e["dskip"])
+    s, o = _forward(d, True)
+    g = _backward(s, o, d, True)
+    assert torch.equal(y, o["y"]) and torch.equal(sm, o["sum"])
+    assert torch.equal(dx, g["dx"])
+    assert torch.equal(dg, g["dgamma"]) and torch.equal(db, g["dbeta"])
+    for wide, lead in ((wide_y, 1), (wide_s, 3), (wide_d, 5)):
+        assert bool((wide[:, :lead] == 5).all())
+        assert bool((wide[:, lead + cols:] == 5).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_broadcast_rows(device):
+    """One row shown many times (stride 0) as x, residual and dy."""
+    d = _data(6, 100, torch.float32, device)
+    e = dict(d)
+    for k in ("x", "residual", "dy", "dskip"):
+        e[k] = d[k][:1].expand(6, 100)
+        d[k] = e[k].contiguous()
+    e_s, e_o = _forward({**e, "x": e["x"]}, True,
+                        out=torch.empty_like(d["x"]))
+    s, o = _forward(d, True)
+    assert torch.equal(e_o["y"], o["y"])
+    a = {"dx": torch.empty_like(d["x"]),
+         "dgamma": torch.empty_like(d["gamma"]),
+         "dbeta": torch.empty_like(d["beta"])}
+    F.layernorm_bwd(e["dy"], s, o["mean"], o["invstd"], d["gamma"],
+                    a["dgamma"], a["dbeta"], a["dx"], dskip=e["dskip"])
+    g = _backward(s, o, d, True)
+    for k in g:
+        assert torch.equal(a[k], g[k]), k
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("cols", [5, 96, 1001, 3000])
+def test_in_place(device, cols):
+    d = _data(21, cols, torch.bfloat16, device)
+    s, o = _forward(d, True)
+    g = _backward(s, o, d, True)
+    e = {k: v.clone() for k, v in d.items()}
+    F.layernorm_fwd(e["x"], e["gamma"], e["beta"], EPS, e["x"],
+                    residual=e["residual"], sum_out=e["residual"])
+    assert torch.equal(e["x"], o["y"]) and torch.equal(e["residual"], o["sum"])
+    dg, db = torch.empty_like(e["gamma"]), torch.empty_like(e["beta"])
+    F.layernorm_bwd(e["dy"], s, o["mean"], o["invstd"], e["gamma"], dg, db,
+                    e["dy"], dskip=e["dskip"])
+    assert torch.equal(e["dy"], g["dx"])
+    assert torch.equal(dg, g["dgamma"]) and torch.equal(db, g["dbeta"])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("cols", [12, 130, 1030])
+def test_far_mean_and_constant_rows(device, cols):
+    """A mean a thousand times the spread keeps its digits (the second sum is
+    over differences), and a constant row gives beta."""
+    d = _data(9, cols, torch.float32, device)
+    d["x"] += 1000.0
+    d["x"][4] = 3.0
+    s, o = _forward(d, False)
+    ref, tol = _reference(s, d, torch.float32)
+    _close(o["y"], ref["y"], tol["y"], "y")
+    assert (o["y"][4].double().cpu() - d["beta"].double().cpu()).abs().max() \
+        <= tol["y"][4].max()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("cols", [6, 77, 2000])
+def test_bad_rows_stay_alone(device, bad, cols):
+    d = _data(10, cols, torch.bfloat16, device)
+    s0, o0 = _forward(d, False)
+    g0 = _backward(s0, o0, d, False)
+    e = {k: v.clone() for k, v in d.items()}
+    e["x"][3, cols // 2] = bad
+    s, o = _forward(e, False)
+    g = _backward(s, o, e, False)
+    keep = [r for r in range(10) if r != 3]
+    assert bool(o["y"][3].isnan().all())
+    assert torch.equal(o["y"][keep], o0["y"][keep])
+    assert torch.equal(g["dx"][keep], g0["dx"][keep])
+    # a bad dy column reaches that column's sums and its own row only
+    e = {k: v.clone() for k, v in d.items()}
+    e["dy"][5, 1] = bad
+    g = _backward(s0, o0, e, False)
+    keep = [r for r in range(10) if r != 5]
+    others = [c for c in range(cols) if c != 1]
+    assert torch.equal(g["dx"][keep], g0["dx"][keep])
+    assert torch.equal(g["dbeta"][others], g0["dbeta"][others])
+    assert torch.equal(g["dgamma"][others], g0["dgamma"][others])
+    assert not bool(g["dbeta"][1].isfinite())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_rows(device):
+    d = _data(0, 40, torch.bfloat16, device)
+    s, o = _forward(d, True)
+    g = _backward(s, o, d, True)
+    assert float(g["dgamma"].abs().sum()) == 0
+    assert float(g["dbeta"].abs().sum()) == 0
+
+
+def test_gradients_against_differences():
+    """The formula's gradients agree with central differences of the forward
+    pass in 64 bits (step 1e-6: error about 1e-9)."""
+    d = _data(4, 11, torch.float32, "cpu")
+    x, gamma, beta, dy = (d[k].double() for k in ("x", "gamma", "beta", "dy"))
+
+    def loss(x_, ga, be):
+        mu = x_.mean(1, keepdim=True)
+        rs = ((x_ - mu).square().mean(1, keepdim=True) + EPS).rsqrt()
+        return ((((x_ - mu) * rs) * ga + be) * dy).sum()
+
+    ref, _ = _reference(d["x"], d, torch.float32)
+    for name, idx in (("dx", 0), ("dgamma", 1), ("dbeta", 2)):
+        args = [x, gamma, beta]
+        num = torch.zeros_like(args[idx])
+        flat = num.view(-1)
+        for i in range(flat.numel()):
+            side = []
+            for step in (1e-6, -1e-6):
+                moved = args[idx].clone()
+                moved.view(-1)[i] += step
+                side.append(loss(*args[:idx], moved, *args[idx + 1:]))
+            flat[i] = (side[0] - side[1]) / 2e-6
+        assert (num - ref[name]).abs().max() < 1e-7
+
+
+@pytest.mark.gpu
+def test_other_stream_and_graph():
+    d = _data(300, 384, torch.bfloat16, "cuda")
+    s, o = _forward(d, True)
+    g = _backward(s, o, d, True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        s2, o2 = _forward(d, True)
+        g2 = _backward(s2, o2, d, True)
+    side.synchronize()
+    for a, b in ((o, o2), (g, g2)):
+        for k in a:
+            assert torch.equal(a[k], b[k]), k
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s3, o3 = _forward(d, True)
+        g3 = _backward(s3, o3, d, True)
+    for seed in range(4):
+        for k, v in _data(300, 384, torch.bfloat16, "cuda", seed=seed).items():
+            d[k].copy_(v)
+        s, o = _forward(d, True)
+        g = _backward(s, o, d, True)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in ((o, o3), (g, g3)):
+            for k in a:
+                assert torch.equal(a[k], b[k]), (seed, k)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    d = _data(4, 16, torch.bfloat16, device)
+    s, o = _forward(d, False)
+    ga, be, x = d["gamma"], d["beta"], d["x"]
+
+    def fwd(x=x, ga=ga, be=be, out=None, **kw):
+        F.layernorm_fwd(x, ga, be, EPS,
+                        torch.empty_like(x) if out is None else out, **kw)
+
+    def bwd(dy=d["dy"], x=x, mean=o["mean"], invstd=o["invstd"], ga=ga,
+            dg=None, dx=None, dskip=None):
+        F.layernorm_bwd(dy, x, mean, invstd, ga,
+                        torch.empty_like(ga) if dg is None else dg,
+                        torch.empty_like(ga),
+                        torch.empty_like(x) if dx is None else dx, dskip=dskip)
+
+    wide = torch.zeros(2, 32769, device=device)
+    calls = [
+        lambda: fwd(x=x.view(2, 2, 16)),
+        lambda: fwd(x=x.long()),
+        lambda: fwd(x=x.double()),
+        lambda: fwd(out=torch.empty_like(x[:3])),
+        lambda: fwd(out=torch.empty_like(x, dtype=torch.float32)),
+        lambda: fwd(ga=ga[:8]),
+        lambda: fwd(be=be.to(torch.bfloat16)),
+        lambda: fwd(mean=o["mean"]),
+        lambda: fwd(mean=o["mean"][:2], invstd=o["invstd"][:2]),
+        lambda: fwd(residual=x.float()),
+        lambda: fwd(sum_out=torch.empty_like(x)),
+        lambda: fwd(x=wide, ga=wide[0], be=wide[1]),
+        lambda: fwd(x=wide[:, :0], ga=ga[:0], be=be[:0]),
+        lambda: bwd(dy=d["dy"][:2]),
+        lambda: bwd(dy=d["dy"].float()),
+        lambda: bwd(mean=o["mean"][:2]),
+        lambda: bwd(dg=torch.empty(3, device=device)),
+        lambda: bwd(dx=torch.empty_like(x, dtype=torch.float16)),
+        lambda: bwd(dskip=x[:, :8]),
+    ]
+    if device == "cuda":
+        calls += [
+            lambda: fwd(ga=ga.cpu()),
+            lambda: fwd(out=torch.empty_like(x).cpu()),
+            lambda: fwd(x=x.t(), ga=ga[:4].clone(), be=be[:4].clone()),
+            lambda: fwd(out=x[:1].expand(4, 16)),
+            lambda: fwd(residual=x, sum_out=x, out=x),
+            lambda: bwd(ga=ga[::2]),
+        ]
+    for i, call in enumerate(calls):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} was taken")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layer(device):
+    arena = ParamArena(device)
+    layer = LayerNorm("ln", 48)
+    layer.build(arena)
+    arena.finalize()
+    assert layer.param_names() == ["ln.g", "ln.b"]
+    d = _data(30, 48, torch.bfloat16, device)
+    arena.pf("ln.g").copy_(d["gamma"])
+    arena.pf("ln.b").copy_(d["beta"])
+    x3, r3 = d["x"].view(5, 6, 48), d["residual"].view(5, 6, 48)
+    y = layer.forward(x3, residual=r3)
+    assert y.shape == x3.shape and layer.sum.shape == x3.shape
+    dx = layer.backward(d["dy"].view(5, 6, 48), dskip=d["dskip"].view(5, 6, 48))
+    ref, tol = _reference(layer.sum.view(30, 48), d, torch.bfloat16,
+                          d["dskip"])
+    _close(y.view(30, 48), ref["y"], tol["y"], "y")
+    _close(dx.view(30, 48), ref["dx"], tol["dx"], "dx")
+    _close(arena.g("ln.g"), ref["dgamma"], tol["dgamma"], "dgamma")
+    _close(arena.g("ln.b"), ref["dbeta"], tol["dbeta"], "dbeta")
+    # another batch without the skip path
+    y = layer.forward(x3[:2].contiguous())
+    assert layer.sum is None and y.shape == (2, 6, 48)
