@@ -29,6 +29,7 @@ SOURCES = [
     os.path.join(CSRC, "embedding.hip"),
     os.path.join(CSRC, "batchnorm.hip"),
     os.path.join(CSRC, "layernorm.hip"),
+    os.path.join(CSRC, "newton_schulz.hip"),
 ]
 
 

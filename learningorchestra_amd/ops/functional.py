@@ -12,6 +12,7 @@ Activation layout is NHWC everywhere (SURVEY §2.9 + conv_pool.hip header).
 """
 from __future__ import annotations
 
+import math
 import os
 from typing import Optional, Tuple
 
@@ -327,6 +328,145 @@ def adam_step(master: torch.Tensor, grad: torch.Tensor, m1: torch.Tensor,
     m2.mul_(b2).addcmul_(g, g, value=1 - b2)
     master.addcdiv_(m1 * c1, (m2 * c2).sqrt() + eps, value=-lr)
     mirror.copy_(master.to(mirror.dtype))
+
+
+# ------------------------------------------------- Newton-Schulz and Muon
+# quintic whose five steps bring singular values from about 0.005 up to
+# between 0.7 and 1.2: the steepest start, at the price of not settling at 1
+NS_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def _ns_coeffs(steps: int, coeffs) -> list:
+    """[a, b, c] per step, flat, from one triple or one triple per step."""
+    if int(steps) != steps or not 1 <= steps <= 100:
+        raise ValueError("Newton-Schulz takes 1 to 100 steps")
+    rows = [coeffs] * int(steps) if len(coeffs) == 3 and not hasattr(
+        coeffs[0], "__len__") else list(coeffs)
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError("coeffs: one (a, b, c), or one for each step")
+    flat = [float(v) for r in rows for v in r]
+    top = 1.0           # the largest singular value, before and after a step
+    for a, b, c in zip(*[iter(flat)] * 3):
+        if not all(math.isfinite(v) for v in (a, b, c)):
+            raise ValueError("coeffs must be finite")
+        # |p| is largest at the end or where p' = a + 3 b q + 5 c q^2 = 0
+        q, disc = [top * top], 9 * b * b - 20 * a * c
+        if c and disc >= 0:
+            q += [(-3 * b + r * math.sqrt(disc)) / (10 * c) for r in (1, -1)]
+        elif not c and b:
+            q.append(-a / (3 * b))
+        top = max(math.sqrt(v) * abs(a + b * v + c * v * v)
+                  for v in q if 0 <= v <= top * top)
+        if top >= 2 ** 20:
+            raise ValueError("these coefficients let the singular values "
+                             "grow past 2^20")
+    return flat
+
+
+def _newton_schulz_ref(x: torch.Tensor, flat: list, eps: float) -> torch.Tensor:
+    tall = x.shape[-2] > x.shape[-1]
+    if tall:
+        x = x.transpose(-2, -1)
+    x = x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps)
+    for i in range(0, len(flat), 3):
+        a, b, c = flat[i:i + 3]
+        gram = x @ x.transpose(-2, -1)
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.transpose(-2, -1) if tall else x
+
+
+def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS,
+                  eps: float = 1e-7,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The nearest matrix to G with orthonormal rows (or columns, if tall), by
+    Newton-Schulz steps X <- a X + (b A + c A^2) X, A = X X^T, from
+    X = G / (|G|_F + eps). g [m, n] or a batch [..., m, n] in bf16, fp16 or
+    fp32; computed to fp32's accuracy and rounded once to ``out``, of g's shape
+    and type (it may be g). ``coeffs``: (a, b, c), or a triple for each step;
+    such that grow singular values past 2^20 are refused. A zero matrix stays
+    zero. A view that is not contiguous is copied first."""
+    flat = _ns_coeffs(steps, coeffs)
+    if g.dim() < 2:
+        raise ValueError("g must be a matrix or a batch of them")
+    if g.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError("g must be bf16, fp16 or fp32")
+    if out is None:
+        out = torch.empty_like(g, memory_format=torch.contiguous_format)
+    if out.shape != g.shape or out.dtype != g.dtype or out.device != g.device \
+            or not out.is_contiguous():
+        raise ValueError("out must be contiguous and of g's shape, type and "
+                         "device")
+    if _is_gpu(g):
+        three = (-1 if g.numel() else 0, g.shape[-2], g.shape[-1])
+        require_ext().orthogonalize(g.contiguous().view(three),
+                                    out.view(three), flat, eps)
+        return out
+    if g.numel():
+        out.copy_(_newton_schulz_ref(g.contiguous().float(), flat, eps))
+    return out
+
+
+class MuonPlan:
+    """What ``muon_step`` keeps between steps for the weight matrices of one
+    flat arena of ``numel`` elements: ``views`` lists them as (offset, rows,
+    cols), offsets being multiples of 8 as ParamArena's are. On a GPU it owns
+    the kernels' tables and their workspace (about 16 bytes an element for wide
+    matrices), so steps that share a plan have to be ordered, like steps that
+    share a momentum."""
+
+    def __init__(self, views, numel: int, device) -> None:
+        self.views = [tuple(int(v) for v in t) for t in views]
+        self.numel = int(numel)
+        self.device = torch.device(device)
+        if any(len(t) != 3 for t in self.views) or not self.views:
+            raise ValueError("views: (offset, rows, cols) for each matrix")
+        end = 0
+        for off, m, n in sorted(self.views):
+            if off < end or off % 8 or m < 1 or n < 1:
+                raise ValueError("matrices must start on a multiple of 8 "
+                                 "elements and not overlap")
+            end = off + m * n
+        if end > self.numel:
+            raise ValueError("a matrix ends outside the arena")
+        self._native = None
+        if self.device.type == "cuda":
+            dev = self.device if self.device.index is not None else \
+                torch.device("cuda", torch.cuda.current_device())
+            self._native = require_ext().MuonPlan(
+                [list(t) for t in self.views], self.numel, str(dev))
+
+
+def muon_step(plan: MuonPlan, master: torch.Tensor, grad: torch.Tensor,
+              mom: torch.Tensor, mirror: torch.Tensor, lr: float,
+              mu: float = 0.95, wd: float = 0.0, gscale: float = 1.0,
+              nesterov: bool = True, steps: int = 5, coeffs=NS_COEFFS,
+              eps: float = 1e-7) -> None:
+    """One Muon step of the plan's matrices, in place on flat fp32 master,
+    grad and momentum and the bf16 mirror:
+
+        mom <- mu mom + gscale g;  U = gscale g + mu mom (nesterov) or mom
+        w <- (1 - lr wd) w - lr sqrt(max(1, rows / cols)) orthogonalize(U)
+
+    Elements outside the matrices stay as they are. Every rank that starts
+    from the same values ends with the same values."""
+    flat = _ns_coeffs(steps, coeffs)
+    if plan._native is not None:
+        plan._native.step(master, grad, mom, mirror, lr, mu, wd, gscale,
+                          nesterov, flat, eps)
+        return
+    for t in (master, grad, mom, mirror):
+        if t.numel() != plan.numel or t.is_cuda:
+            raise RuntimeError(f"the plan is for {plan.numel} elements on "
+                               f"{plan.device}")
+    for off, m, n in plan.views:
+        sl = slice(off, off + m * n)
+        g = grad[sl] * gscale
+        mom[sl].mul_(mu).add_(g)
+        u = g + mu * mom[sl] if nesterov else mom[sl]
+        o = _newton_schulz_ref(u.view(m, n), flat, eps).reshape(-1)
+        gain = max(1.0, m / n) ** 0.5
+        master[sl].mul_(1.0 - lr * wd).add_(o, alpha=-lr * gain)
+        mirror[sl] = master[sl].to(mirror.dtype)
 
 
 # --------------------------------------------------------------- reductions
