@@ -121,7 +121,8 @@ void launch_relu_bwd(const void* dy, const void* y, void* dx, long n, hipStream_
 void launch_sgd(void* master, const void* grad, void* mom, void* mirror, long n,
                 float lr, float mu, float wd, float gscale, hipStream_t s);
 void launch_adam(void* master, const void* grad, void* m1, void* m2, void* mirror,
-                 const void* step_dev, long n, float lr, float b1, float b2,
+                 const void* step_dev, const void* ranges, int n_ranges,
+                 long longest, long n, float lr, float b1, float b2,
                  float eps, float wd, float gscale, hipStream_t s);
 void launch_colsum(const void* dy, void* out, long M, int N, long ldy, hipStream_t s);
 void launch_colsum_masked(const void* dy, const void* mask, void* out, long M,
@@ -590,9 +591,41 @@ void adam_step(at::Tensor master, at::Tensor grad, at::Tensor m1, at::Tensor m2,
               "step_dev must be int32 on GPU");
   TORCH_CHECK(master.numel() % 4 == 0, "arena must be 4-aligned");
   lo::launch_adam(master.data_ptr(), grad.data_ptr(), m1.data_ptr(), m2.data_ptr(),
-                  mirror.data_ptr(), step_dev.data_ptr(), master.numel(),
-                  (float)lr, (float)b1, (float)b2, (float)eps, (float)wd,
-                  (float)gscale, stream());
+                  mirror.data_ptr(), step_dev.data_ptr(), nullptr, 0, 0,
+                  master.numel(), (float)lr, (float)b1, (float)b2, (float)eps,
+                  (float)wd, (float)gscale, stream());
+}
+
+// the same step on parts of the arena only: ranges [k, 2] (start, end), int64
+// on the GPU, the longest of them long
+void adam_ranges(at::Tensor master, at::Tensor grad, at::Tensor m1,
+                 at::Tensor m2, at::Tensor mirror, at::Tensor step_dev,
+                 at::Tensor ranges, int64_t longest, double lr, double b1,
+                 double b2, double eps, double wd, double gscale) {
+  check_f32(master, "master");
+  check_f32(grad, "grad");
+  check_f32(m1, "m1");
+  check_f32(m2, "m2");
+  check_bf16(mirror, "mirror");
+  for (const auto& t : {grad, m1, m2, mirror})
+    TORCH_CHECK(t.numel() == master.numel() && t.device() == master.device(),
+                "the arena's tensors must match");
+  TORCH_CHECK(master.numel() % 4 == 0, "arena must be 4-aligned");
+  TORCH_CHECK(step_dev.scalar_type() == at::kInt &&
+                  step_dev.device() == master.device(),
+              "step_dev must be int32 on the arena's GPU");
+  TORCH_CHECK(ranges.scalar_type() == at::kLong && ranges.is_contiguous() &&
+                  ranges.dim() == 2 && ranges.size(1) == 2 &&
+                  ranges.device() == master.device() &&
+                  ranges.size(0) <= 65535,
+              "ranges must be int64 [k, 2] on the arena's GPU");
+  if (ranges.size(0) == 0 || longest <= 0) return;
+  const c10::DeviceGuard guard(master.device());
+  lo::launch_adam(master.data_ptr(), grad.data_ptr(), m1.data_ptr(), m2.data_ptr(),
+                  mirror.data_ptr(), step_dev.data_ptr(), ranges.data_ptr(),
+                  (int)ranges.size(0), longest, master.numel(), (float)lr,
+                  (float)b1, (float)b2, (float)eps, (float)wd, (float)gscale,
+                  stream());
 }
 
 at::Tensor colsum(at::Tensor dy, at::Tensor out,
@@ -1075,6 +1108,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("relu_bwd", &relu_bwd);
   m.def("sgd_step", &sgd_step);
   m.def("adam_step", &adam_step);
+  m.def("adam_ranges", &adam_ranges);
   m.def("colsum", &colsum, py::arg("dy"), py::arg("out"),
         py::arg("mask") = py::none());
   m.def("argmax_rows", &argmax_rows);

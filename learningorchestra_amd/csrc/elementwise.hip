@@ -77,16 +77,24 @@ void launch_sgd(void* master, const void* grad, void* mom, void* mirror, long n,
 // ---------------------------------------------------------- adam_step ------
 // step_dev: device step counter (graph-capture-safe bias correction — the
 // count is read on DEVICE, so replaying a captured step keeps correcting)
+// ranges: null, or gridDim.y (start, end) pairs, multiples of 4 elements, that
+// the step keeps to (one launch for parameters that lie apart)
 __global__ void adam_kernel(float* __restrict__ master, const float* __restrict__ grad,
                             float* __restrict__ m1, float* __restrict__ m2,
                             bf16* __restrict__ mirror,
-                            const int* __restrict__ step_dev, long n4, float lr,
+                            const int* __restrict__ step_dev,
+                            const long* __restrict__ ranges, long n4, float lr,
                             float b1, float b2, float eps, float wd,
                             float gscale) {
   const float t = (float)*step_dev;
   const float c1 = 1.f / (1.f - __powf(b1, t));
   const float c2 = 1.f / (1.f - __powf(b2, t));
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n4;
+  long i0 = 0;
+  if (ranges) {
+    i0 = max(ranges[2 * blockIdx.y] / 4, 0L);
+    n4 = min(ranges[2 * blockIdx.y + 1] / 4, n4);
+  }
+  for (long i = i0 + (long)blockIdx.x * blockDim.x + threadIdx.x; i < n4;
        i += (long)gridDim.x * blockDim.x) {
     f32x4 p = *(const f32x4*)(master + i * 4);
     f32x4 g = *(const f32x4*)(grad + i * 4);
@@ -111,15 +119,18 @@ __global__ void adam_kernel(float* __restrict__ master, const float* __restrict_
 }
 
 void launch_adam(void* master, const void* grad, void* m1, void* m2, void* mirror,
-                 const void* step_dev, long n, float lr, float b1, float b2,
+                 const void* step_dev, const void* ranges, int n_ranges,
+                 long longest, long n, float lr, float b1, float b2,
                  float eps, float wd, float gscale, hipStream_t s) {
   const long n4 = n / 4;
   const int block = 256;
-  const int grid = (int)min((n4 + block - 1) / block, (long)2048);
-  hipLaunchKernelGGL(adam_kernel, dim3(grid), dim3(block), 0, s,
-                     (float*)master, (const float*)grad, (float*)m1, (float*)m2,
-                     (bf16*)mirror, (const int*)step_dev, n4, lr, b1, b2, eps,
-                     wd, gscale);
+  const long most = ranges ? longest / 4 : n4;
+  const int grid = (int)min((most + block - 1) / block, (long)2048);
+  hipLaunchKernelGGL(adam_kernel, dim3(grid, ranges ? n_ranges : 1),
+                     dim3(block), 0, s, (float*)master, (const float*)grad,
+                     (float*)m1, (float*)m2, (bf16*)mirror,
+                     (const int*)step_dev, (const long*)ranges, n4, lr, b1, b2,
+                     eps, wd, gscale);
 }
 
 // ------------------------------------------------------------- colsum ------

@@ -1,2 +1,2 @@
-from .arena import ParamArena, SGD, Adam  # noqa: F401
+from .arena import ParamArena, SGD, Adam, Muon  # noqa: F401
 from . import layers  # noqa: F401

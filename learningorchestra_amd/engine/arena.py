@@ -18,7 +18,7 @@ vectorized kernels.
 from __future__ import annotations
 
 import math
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -156,3 +156,77 @@ class Adam:
         F.adam_step(a.master, a.grad, self.m1, self.m2, a.mirror, self.lr,
                     self.betas[0], self.betas[1], self.eps, self.weight_decay,
                     self.t, gscale)
+
+
+class Muon:
+    """Muon over the arena's weight matrices, Adam over the rest.
+
+    A matrix (every 2-D parameter with both sides above 1, convolutions as
+    [out channels, taps * in channels]) moves along its momentum's
+    orthogonalised form, one grouped call for all of them (newton_schulz.hip);
+    biases, norms and the matrices named in ``exclude`` - embeddings and the
+    classifier's head, by custom - move by the fused Adam kernel, kept to their
+    ranges of the flat arena. ``weight_decay`` is decoupled on the
+    matrices (w <- (1 - lr wd) w) and Adam's own on the rest."""
+
+    def __init__(self, arena: ParamArena, lr: float = 0.02,
+                 momentum: float = 0.95, nesterov: bool = True,
+                 steps: int = 5, weight_decay: float = 0.0,
+                 exclude: Sequence[str] = (), adam_lr: float = 1e-3,
+                 betas=(0.9, 0.999), eps: float = 1e-8):
+        self.arena = arena
+        self.lr, self.momentum, self.nesterov = lr, momentum, nesterov
+        self.steps, self.weight_decay = int(steps), weight_decay
+        self.adam_lr, self.betas, self.eps = adam_lr, tuple(betas), eps
+        names = {name for name, _, _ in arena._specs}
+        unknown = set(exclude) - names
+        if unknown:
+            raise ValueError(f"exclude: no parameters {sorted(unknown)}")
+        self.matrices, views, rest = [], [], []
+        for name, shape, _ in arena._specs:
+            off, n = arena._offsets[name]
+            if len(shape) == 2 and min(shape) > 1 and name not in exclude:
+                self.matrices.append(name)
+                views.append((off, *shape))
+            elif rest and rest[-1][1] == off:
+                rest[-1][1] = off + _pad8(n)
+            else:
+                rest.append([off, off + _pad8(n)])
+        if not views:
+            raise ValueError("no weight matrix left for Muon")
+        self.plan = F.MuonPlan(views, arena.numel, arena.master.device)
+        self._rest = F.AdamRanges(rest, arena.numel, arena.master.device)
+        self.mom = torch.zeros_like(arena.master)   # also Adam's m1
+        self.m2 = torch.zeros_like(arena.master)
+        self.t = (torch.zeros(1, dtype=torch.int32, device=arena.master.device)
+                  if arena.master.is_cuda else 0)
+
+    def step(self, gscale: float = 1.0) -> None:
+        a = self.arena
+        self.t += 1
+        F.muon_step(self.plan, a.master, a.grad, self.mom, a.mirror, self.lr,
+                    self.momentum, self.weight_decay, gscale, self.nesterov,
+                    self.steps)
+        F.adam_ranges(self._rest, a.master, a.grad, self.mom, self.m2,
+                      a.mirror, self.adam_lr, self.betas[0], self.betas[1],
+                      self.eps, self.weight_decay, self.t, gscale)
+
+    def state_dict(self):
+        return {"mom": self.mom.cpu().clone(), "m2": self.m2.cpu().clone(),
+                "t": int(self.t),
+                "lr": self.lr, "momentum": self.momentum,
+                "nesterov": self.nesterov, "steps": self.steps,
+                "weight_decay": self.weight_decay, "adam_lr": self.adam_lr,
+                "betas": list(self.betas), "eps": self.eps}
+
+    def load_state_dict(self, sd):
+        self.mom.copy_(sd["mom"].to(self.mom.device))
+        self.m2.copy_(sd["m2"].to(self.m2.device))
+        if torch.is_tensor(self.t):
+            self.t.fill_(sd["t"])
+        else:
+            self.t = sd["t"]
+        for k in ("lr", "momentum", "nesterov", "steps", "weight_decay",
+                  "adam_lr", "eps"):
+            setattr(self, k, sd[k])
+        self.betas = tuple(sd["betas"])

@@ -13,7 +13,7 @@ import torch
 from ..parallel import (all_reduce_grads, get_world_size, is_distributed,
                         oversubscribed)
 from ..parallel.ddp import device_step_lock
-from .arena import SGD, Adam
+from .arena import SGD, Adam, Muon
 from .layers import SequentialClassifier
 
 
@@ -249,3 +249,8 @@ def make_sgd(model: SequentialClassifier, lr=0.05, momentum=0.9, wd=0.0) -> SGD:
 
 def make_adam(model: SequentialClassifier, lr=1e-3) -> Adam:
     return Adam(model.arena, lr=lr)
+
+
+def make_muon(model, lr=0.02, momentum=0.95, wd=0.0, exclude=()) -> Muon:
+    return Muon(model.arena, lr=lr, momentum=momentum, weight_decay=wd,
+                exclude=exclude)

@@ -7,6 +7,8 @@ NHWC convs with W=1 over the sequence axis, im2col + MFMA GEMM with fused
 bias+ReLU) -> max-over-time pooling (maxpool kernel, KH = T-k+1) -> concat ->
 padded-head linear + fused softmax-CE. Every hot op is a gfx950 HIP kernel;
 branch concat/split and the branch-grad sum are device memcpy/add glue.
+``layer_norm`` puts a layer norm (layernorm.hip) behind the embedding and one
+before the classifier.
 """
 from __future__ import annotations
 
@@ -17,14 +19,16 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from ..engine.arena import ParamArena
-from ..engine.layers import Conv2dNHWC, Embedding, Linear, MaxPool2dNHWC
+from ..engine.layers import (Conv2dNHWC, Embedding, LayerNorm, Linear,
+                             MaxPool2dNHWC)
 from ..ops import functional as F
 
 
 class TextCNN:
     def __init__(self, vocab: int = 20000, emb_dim: int = 128,
                  filters: int = 128, kernel_sizes: Sequence[int] = (3, 4, 5),
-                 num_classes: int = 2, device="cpu", seed: int = 0):
+                 num_classes: int = 2, device="cpu", seed: int = 0,
+                 layer_norm: bool = False):
         self.vocab, self.emb_dim, self.filters = vocab, emb_dim, filters
         self.kernel_sizes = tuple(kernel_sizes)
         self.num_classes = num_classes
@@ -46,8 +50,13 @@ class TextCNN:
             pool.fuse_relu = True
             conv.relu_bwd_upstream = True
         self.fc = Linear("fc", filters * len(self.kernel_sizes), self.cpad)
-        for lay in [self.emb, *self.convs, self.fc]:
-            lay.build(self.arena)
+        self.ln_emb = self.ln_cat = None
+        if layer_norm:
+            self.ln_emb = LayerNorm("ln_emb", emb_dim)
+            self.ln_cat = LayerNorm("ln_cat", filters * len(self.kernel_sizes))
+        for lay in [self.emb, self.ln_emb, *self.convs, self.ln_cat, self.fc]:
+            if lay is not None:
+                lay.build(self.arena)
         self.arena.finalize(seed)
 
         self.loss_sum = torch.zeros(1, dtype=torch.float32, device=self.device)
@@ -73,6 +82,8 @@ class TextCNN:
         B, S = ids.shape
         bufs = self._alloc(B, S)
         e = self.emb.forward(ids).view(B, S, 1, self.emb_dim)
+        if self.ln_emb is not None:
+            e = self.ln_emb.forward(e)
         Fn = self.filters
         for i, (k, conv, pool) in enumerate(zip(self.kernel_sizes, self.convs,
                                                 self.pools)):
@@ -80,7 +91,10 @@ class TextCNN:
             pool.set_window(y.shape[1], 1)            # max-over-time
             p = pool.forward(y)                       # [B, 1, 1, F]
             bufs["cat"][:, i * Fn:(i + 1) * Fn] = p.view(B, Fn)
-        return self.fc.forward(bufs["cat"])
+        cat = bufs["cat"]
+        if self.ln_cat is not None:
+            cat = self.ln_cat.forward(cat)
+        return self.fc.forward(cat)
 
     def train_step(self, ids: torch.Tensor, y: torch.Tensor,
                    gscale: Optional[float] = None,
@@ -97,6 +111,10 @@ class TextCNN:
         dcat = self.fc.backward(bufs["dlogits"])      # [B, 3F]
         if grad_hook:
             grad_hook(self.fc.param_names())
+        if self.ln_cat is not None:
+            dcat = self.ln_cat.backward(dcat)
+            if grad_hook:
+                grad_hook(self.ln_cat.param_names())
         Fn = self.filters
         dxe = bufs["dxe"]
         for i, (k, conv, pool) in enumerate(zip(self.kernel_sizes, self.convs,
@@ -122,6 +140,10 @@ class TextCNN:
                     dxe.copy_(dbranch)
                 else:
                     dxe.add_(dbranch)
+        if self.ln_emb is not None:
+            dxe = self.ln_emb.backward(dxe)
+            if grad_hook:
+                grad_hook(self.ln_emb.param_names())
         self.emb.backward(dxe.view(B, S, self.emb_dim))
         if grad_hook:
             grad_hook(self.emb.param_names())

@@ -14,7 +14,7 @@ from typing import Optional, Sequence
 import numpy as np
 import torch
 
-from ..engine.trainer import Trainer, make_sgd
+from ..engine.trainer import Trainer, make_muon, make_sgd
 from .mnist_cnn import build_mnist_cnn
 from .tabular import (GaussianNBClassifier, LogisticRegressionClassifier,  # noqa: F401 - re-export
                       MLPClassifier)
@@ -115,25 +115,34 @@ class MnistCNN:
 
 
 class TextCNNClassifier:
-    """Keras-surface wrapper over the TextCNN engine model (IMDb config)."""
+    """Keras-surface wrapper over the TextCNN engine model (IMDb config).
+    ``layer_norm`` normalises the embeddings and the pooled features;
+    ``optimizer`` is "sgd", or "muon": orthogonalised updates of the
+    convolutions, Adam for the rest."""
 
     def __init__(self, vocab: int = 20000, emb_dim: int = 128,
                  filters: int = 128, kernel_sizes=(3, 4, 5),
                  num_classes: int = 2, seed: int = 0, lr: float = 0.05,
-                 batch_size: int = 512, device: Optional[str] = None):
+                 batch_size: int = 512, device: Optional[str] = None,
+                 layer_norm: bool = False, optimizer: str = "sgd"):
         from .textcnn import build_textcnn
+        if optimizer not in ("sgd", "muon"):
+            raise ValueError(f"optimizer must be sgd or muon, not {optimizer!r}")
         self.device = _default_device(device)
         self.lo_spec = {"vocab": vocab, "emb_dim": emb_dim,
                         "filters": filters,
                         "kernel_sizes": list(kernel_sizes),
                         "num_classes": num_classes, "seed": seed, "lr": lr,
-                        "batch_size": batch_size}
+                        "batch_size": batch_size, "layer_norm": layer_norm,
+                        "optimizer": optimizer}
         self.model = build_textcnn(self.device, seed=seed, vocab=vocab,
                                    emb_dim=emb_dim, filters=filters,
                                    kernel_sizes=tuple(kernel_sizes),
-                                   num_classes=num_classes)
-        self.trainer = Trainer(self.model, make_sgd(self.model, lr=lr),
-                               device=self.device)
+                                   num_classes=num_classes,
+                                   layer_norm=layer_norm)
+        opt = (make_muon(self.model, lr=lr, exclude=("emb.w", "fc.w"))
+               if optimizer == "muon" else make_sgd(self.model, lr=lr))
+        self.trainer = Trainer(self.model, opt, device=self.device)
         self.batch_size = batch_size
 
     def _to_ids(self, x) -> torch.Tensor:

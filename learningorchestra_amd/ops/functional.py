@@ -330,6 +330,42 @@ def adam_step(master: torch.Tensor, grad: torch.Tensor, m1: torch.Tensor,
     mirror.copy_(master.to(mirror.dtype))
 
 
+class AdamRanges:
+    """Parts of a flat arena, (start, end) pairs of multiples of 8 elements,
+    for ``adam_ranges``."""
+
+    def __init__(self, ranges, numel: int, device) -> None:
+        self.ranges = [(int(a), int(b)) for a, b in ranges]
+        for a, b in self.ranges:
+            if not 0 <= a < b <= numel or a % 8 or b % 8:
+                raise ValueError("ranges must be multiples of 8 within the "
+                                 "arena")
+        self.numel = int(numel)
+        self.longest = max((b - a for a, b in self.ranges), default=0)
+        self._table = torch.tensor(self.ranges, dtype=torch.int64,
+                                   device=device).view(-1, 2)
+
+
+def adam_ranges(ranges: AdamRanges, master: torch.Tensor, grad: torch.Tensor,
+                m1: torch.Tensor, m2: torch.Tensor, mirror: torch.Tensor,
+                lr: float, b1: float, b2: float, eps: float, wd: float, step,
+                gscale: float = 1.0) -> None:
+    """``adam_step`` on some ranges of the arena, in one launch."""
+    if ranges.numel != master.numel():
+        raise RuntimeError(f"the ranges are for {ranges.numel} elements")
+    if _is_gpu(master):
+        if not torch.is_tensor(step):
+            step = torch.tensor([int(step)], dtype=torch.int32,
+                                device=master.device)
+        require_ext().adam_ranges(master, grad, m1, m2, mirror, step,
+                                  ranges._table, ranges.longest, lr, b1, b2,
+                                  eps, wd, gscale)
+        return
+    for a, b in ranges.ranges:
+        adam_step(master[a:b], grad[a:b], m1[a:b], m2[a:b], mirror[a:b], lr,
+                  b1, b2, eps, wd, step, gscale)
+
+
 # ------------------------------------------------- Newton-Schulz and Muon
 # quintic whose five steps bring singular values from about 0.005 up to
 # between 0.7 and 1.2: the steepest start, at the price of not settling at 1

@@ -1,0 +1,262 @@
+"""The Muon optimizer and layer norm inside the engine: parameter split, steps
+against the operators they are made of, checkpoints, captured steps, and a
+small network's gradients."""
+import io
+import os
+
+import pytest
+import torch
+import torch.multiprocessing as mp
+
+from learningorchestra_amd.data.synthetic import imdb_batch
+from learningorchestra_amd.engine.arena import Muon, ParamArena
+from learningorchestra_amd.engine.layers import (LayerNorm, Linear,
+                                                 SequentialClassifier)
+from learningorchestra_amd.engine.trainer import Trainer, make_muon
+from learningorchestra_amd.models.textcnn import build_textcnn
+from learningorchestra_amd.models.zoo import TextCNNClassifier
+from learningorchestra_amd.ops import functional as F
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _arena(device):
+    a = ParamArena(device)
+    a.add("emb.w", (30, 8), 0.1)
+    a.add("conv.w", (16, 40), 0.1)
+    a.add("conv.b", (16,), 0.1)
+    a.add("ln.g", (24,), 0.1)
+    a.add("row.w", (1, 24), 0.1)
+    a.add("tall.w", (70, 9), 0.1)
+    a.add("head.w", (8, 70), 0.1)
+    a.finalize(seed=3)
+    return a
+
+
+def _grads(arena, seed):
+    g = torch.randn(arena.numel, generator=torch.Generator().manual_seed(seed))
+    arena.grad.copy_(g * 1e-2)
+    for name, _, _ in arena._specs:   # the padding holds no gradient
+        off, n = arena._offsets[name]
+        arena.grad[off + n:off + (n + 7) // 8 * 8] = 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_matrices_and_the_rest(device):
+    a = _arena(device)
+    opt = Muon(a, exclude=("emb.w", "head.w"))
+    assert opt.matrices == ["conv.w", "tall.w"]
+    assert Muon(_arena(device)).matrices == ["emb.w", "conv.w", "tall.w",
+                                             "head.w"]
+    with pytest.raises(ValueError):
+        Muon(a, exclude=("nothing",))
+    with pytest.raises(ValueError):
+        Muon(a, exclude=("emb.w", "conv.w", "tall.w", "head.w"))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_step_is_its_operators(device):
+    a, b = _arena(device), _arena(device)
+    opt = Muon(a, lr=0.03, momentum=0.9, weight_decay=0.1, exclude=("emb.w",),
+               adam_lr=0.01)
+    views = [(b._offsets[n][0], *b.p(n).shape) for n in opt.matrices]
+    plan = F.MuonPlan(views, b.numel, device)
+    mom, m2 = torch.zeros_like(b.master), torch.zeros_like(b.master)
+    t = torch.zeros(1, dtype=torch.int32, device=device)
+    for seed in range(3):
+        for arena in (a, b):
+            _grads(arena, seed)
+        opt.step(gscale=0.5)
+        t += 1
+        F.muon_step(plan, b.master, b.grad, mom, b.mirror, 0.03, 0.9, 0.1, 0.5)
+        for name, shape, _ in b._specs:
+            if name in opt.matrices:
+                continue
+            off, n = b._offsets[name]
+            sl = slice(off, off + (n + 7) // 8 * 8)
+            F.adam_step(b.master[sl], b.grad[sl], mom[sl], m2[sl],
+                        b.mirror[sl], 0.01, 0.9, 0.999, 1e-8, 0.1, t, 0.5)
+        for x, y in ((a.master, b.master), (a.mirror, b.mirror),
+                     (opt.mom, mom), (opt.m2, m2)):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_checkpoint(device):
+    a = _arena(device)
+    opt = Muon(a, lr=0.03, exclude=("emb.w",))
+    for seed in range(2):
+        _grads(a, seed)
+        opt.step()
+    buf = io.BytesIO()
+    torch.save({"model": a.state_dict(), "optimizer": opt.state_dict()}, buf)
+    buf.seek(0)
+    b = _arena(device)
+    again = Muon(b, exclude=("emb.w",))
+    saved = torch.load(buf, map_location="cpu", weights_only=True)
+    b.load_state_dict(saved["model"])
+    again.load_state_dict(saved["optimizer"])
+    for seed in range(2, 4):
+        for arena, o in ((a, opt), (b, again)):
+            _grads(arena, seed)
+            o.step()
+    assert torch.equal(a.master, b.master)
+
+
+@pytest.mark.gpu
+def test_captured_steps():
+    """A captured step goes on as eager ones do, Adam's count included."""
+    a, b = _arena("cuda"), _arena("cuda")
+    eager, captured = (Muon(x, exclude=("emb.w",)) for x in (a, b))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.step()
+    for seed in range(4):
+        _grads(a, seed)
+        _grads(b, seed)
+        eager.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a.master, b.master)
+        assert torch.equal(a.mirror, b.mirror)
+    assert int(captured.t) == 4
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_ranges_refusals(device):
+    for bad in ([(0, 12)], [(4, 16)], [(16, 8)], [(0, 72)], [(-8, 8)]):
+        with pytest.raises(ValueError):
+            F.AdamRanges(bad, 64, device)
+    r = F.AdamRanges([(8, 16)], 64, device)
+    z = torch.zeros(72, device=device)
+    with pytest.raises(RuntimeError):
+        F.adam_ranges(r, z, z, z, z, z.bfloat16(), 0.1, 0.9, 0.99, 1e-8, 0.0, 1)
+    # no ranges: nothing moves
+    w = torch.ones(64, device=device)
+    F.adam_ranges(F.AdamRanges([], 64, device), w, w.clone(), w.clone(),
+                  w.clone(), w.bfloat16(), 0.1, 0.9, 0.99, 1e-8, 0.0, 1)
+    assert bool((w == 1).all())
+
+
+def _network(device):
+    return SequentialClassifier(
+        [LayerNorm("ln0", 48), Linear("fc1", 48, 64, relu=True),
+         LayerNorm("ln1", 64), Linear("fc2", 64, 16)], num_classes=10,
+        device=device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_network_gradients_and_steps(device):
+    """Layer norms between linear layers, stepped by Muon. Gradients agree with
+    autograd in fp32: about 16 roundings to bf16 of values and gradients lie
+    between a parameter and the loss, each off by 2^-8 at most."""
+    m = _network(device)
+    gen = torch.Generator().manual_seed(5)
+    x = (torch.randn(96, 48, generator=gen) * 2 + 1).bfloat16().to(device)
+    y = torch.randint(0, 10, (96,), generator=gen).to(device)
+    for name in ("ln0", "ln1"):
+        m.arena.pf(name + ".g").mul_(1.25)
+        m.arena.pf(name + ".b").add_(0.25)
+    m.arena.mirror.copy_(m.arena.master)
+    m.post_opt_step()
+    m.train_step(x, y)
+    p = {n: m.arena.pf(n).detach().cpu().clone().requires_grad_()
+         for n, _, _ in m.arena._specs}
+
+    def norm(t, name):
+        mu = t.mean(1, keepdim=True)
+        z = (t - mu) / ((t - mu).square().mean(1, keepdim=True) + 1e-5).sqrt()
+        return z * p[name + ".g"] + p[name + ".b"]
+
+    h = norm(x.cpu().float(), "ln0") @ p["fc1.w"].T + p["fc1.b"]
+    h = norm(torch.relu(h), "ln1") @ p["fc2.w"].T + p["fc2.b"]
+    torch.nn.functional.cross_entropy(h[:, :10], y.cpu()).backward()
+    for n, t in p.items():
+        got = m.arena.g(n).cpu()
+        assert (got - t.grad).norm() <= 16 * 2 ** -8 * t.grad.norm() + 1e-6, n
+    trainer = Trainer(m, make_muon(m, exclude=("fc2.w",)), device=device)
+    before = m.arena.state_dict()
+    for _ in range(3):
+        trainer.step_async(x, y)
+    after = m.arena.state_dict()
+    assert all(bool(torch.isfinite(v).all()) for v in after.values())
+    assert all(not torch.equal(before[n], after[n]) for n in p)
+    assert torch.equal(m.arena.mirror, m.arena.master.bfloat16())
+    assert m.predict(x).shape == (96,)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_textcnn_with_both(device):
+    m = build_textcnn(device, vocab=500, emb_dim=32, filters=64,
+                      layer_norm=True)
+    opt = make_muon(m, exclude=("emb.w", "fc.w"))
+    assert opt.matrices == ["conv3.w", "conv4.w", "conv5.w"]
+    hooked = []
+    ids, y = (t.to(device) for t in imdb_batch(16, seq_len=24, vocab=500,
+                                               seed=0))
+    m.train_step(ids, y, grad_hook=hooked.extend)
+    assert sorted(hooked) == sorted(n for n, _, _ in m.arena._specs)
+    assert all(float(m.arena.g(n).abs().sum()) > 0 for n in
+               ("ln_emb.g", "ln_emb.b", "ln_cat.g", "ln_cat.b", "emb.w"))
+    trainer = Trainer(m, opt, device=device)
+    for _ in range(2):
+        trainer.step_async(ids, y)
+    assert bool(torch.isfinite(m.arena.master).all())
+    assert m.predict(ids).shape == (16,)
+    # one text's norm is the same alone and in its batch
+    feats = torch.randn(16, 192).bfloat16().to(device)
+    whole = m.ln_cat.forward(feats).clone()
+    assert torch.equal(m.ln_cat.forward(feats[5:6].contiguous()), whole[5:6])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_classifier_options(device):
+    with pytest.raises(ValueError):
+        TextCNNClassifier(vocab=50, optimizer="other", device=device)
+    ids, y = imdb_batch(32, seq_len=16, vocab=50, seed=1)
+    c = TextCNNClassifier(vocab=50, emb_dim=32, filters=64, batch_size=16,
+                          device=device, layer_norm=True, optimizer="muon",
+                          lr=0.02)
+    hist = c.fit(ids.numpy(), y.numpy(), epochs=2)
+    assert all(v == v for v in hist["loss"])
+    assert c.predict(ids.numpy()).shape == (32,)
+    d = TextCNNClassifier(device=device, **c.lo_spec)   # as stored and loaded
+    d.load_state_dict(c.state_dict())
+    assert (d.predict(ids.numpy()) == c.predict(ids.numpy())).all()
+
+
+def _worker(rank, world, port, q):
+    os.environ.update({"RANK": str(rank), "WORLD_SIZE": str(world),
+                       "LOCAL_RANK": str(rank),
+                       "MASTER_ADDR": "127.0.0.1", "MASTER_PORT": str(port)})
+    import torch.distributed as dist
+    from learningorchestra_amd.parallel import init_distributed
+    try:
+        torch.set_num_threads(1)
+        init_distributed(backend="gloo")
+        m = _network("cpu")
+        trainer = Trainer(m, make_muon(m, exclude=("fc2.w",)), device="cpu")
+        gen = torch.Generator().manual_seed(50 + rank)
+        x = torch.randn(32, 48, generator=gen).bfloat16()
+        y = torch.randint(0, 10, (32,), generator=gen)
+        for _ in range(3):
+            trainer.step_async(x, y)
+        q.put((rank, m.arena.master.tolist()))
+        dist.destroy_process_group()
+    except Exception as exc:  # pragma: no cover
+        q.put((rank, f"ERROR: {exc!r}"))
+
+
+@pytest.mark.timeout(240)
+def test_two_ranks_stay_identical():
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_worker, args=(r, 2, 29547, q))
+             for r in range(2)]
+    for p in procs:
+        p.start()
+    results = [q.get(timeout=220)[1] for _ in range(2)]
+    for p in procs:
+        p.join(timeout=30)
+    assert not isinstance(results[0], str), results[0]
+    assert results[0] == results[1]
