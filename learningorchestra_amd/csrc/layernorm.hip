@@ -282,8 +282,19 @@ __global__ __launch_bounds__(1024) void layernorm_join_kernel(
   const int width = 2 * cols;
   const int c = blockIdx.x * 32 + tx;
   float a = 0.f;
-  if (c < width)
-    for (int r = ty; r < n; r += 32) a += part[(long)r * width + c];
+  if (c < width) {
+    // eight loads on their way at a time
+    for (int r0 = ty; r0 < n; r0 += 256) {
+      float v[8];
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = r0 + 32 * i;
+        v[i] = r < n ? part[(long)r * width + c] : 0.f;
+      }
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) a += v[i];
+    }
+  }
   s[ty][tx] = a;
   __syncthreads();
   if (ty == 0 && c < width) {

@@ -179,14 +179,15 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup g, NsInput in,
 // out = alpha * sum + beta * source, all of them carrying their scales.
 enum { GRAM, POLY, APPLY };
 
-template <int T, int KIND>
+template <int T, int KIND, int S>
 __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup g, int from,
                                                          float alpha,
                                                          float beta) {
   constexpr int W = T / 2;      // a wave's square
   constexpr int F = W / 16;     // its 16 x 16 fragments a side
   constexpr int IMG = T * 128;  // bytes of one operand's tile: T rows, 32 k
-  __shared__ __attribute__((aligned(1024))) char lds[4 * IMG];
+  constexpr int LOADS = T / 32; // a wave's loads of one operand's tile
+  extern __shared__ __attribute__((aligned(1024))) char lds[];  // [S][2][IMG]
   long t = xcd_swizzle(blockIdx.x, gridDim.x);
   const NsMat m = find(g, KIND == APPLY ? g.rect_starts : g.tri_starts,
                        KIND == APPLY ? g.rects : g.tris, t);
@@ -215,10 +216,10 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup g, int from,
   // at place p of a row is piece p ^ (row & 7), which spreads a column of
   // pieces over the banks
   auto stage = [&](int kt) {
-    char* buf = lds + (kt & 1) * 2 * IMG;
+    char* buf = lds + (kt % S) * 2 * IMG;
     #pragma unroll
-    for (int i = 0; i < T / 32; ++i) {
-      const int seg = wave * (T / 32) + i;
+    for (int i = 0; i < LOADS; ++i) {
+      const int seg = wave * LOADS + i;
       const int row = seg * 8 + lane / 8;
       const long off = (long)row * 2 * ld + kt * 64 + ((lane % 8) ^ (row & 7)) * 8;
       __builtin_amdgcn_global_load_lds(
@@ -239,33 +240,44 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup g, int from,
 
   f32x4 acc[F][F] = {};
   const int nk = ld / 32;
-  stage(0);
+  for (int kt = 0; kt < S - 1; ++kt)
+    if (kt < nk) stage(kt);
   for (int kt = 0; kt < nk; ++kt) {
-    // tile kt has landed, and every wave is done with the buffer that the
-    // next one goes to
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const char* img = lds + (kt & 1) * 2 * IMG;
+    // tile kt has landed (the S - 2 after it may be on their way), and every
+    // wave is done with the buffer that the next one goes to
+    if (kt + S - 2 < nk)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(
+                       (S - 2) * 2 * LOADS)
+                   : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const char* img = lds + (kt % S) * 2 * IMG;
     f16x8 ph[F], pw[F], qh[F], ql[F];
     #pragma unroll
     for (int i = 0; i < F; ++i) {
       const int row = i * 16 + (lane & 15);
       ph[i] = frag(img, wr * W + row, 0);
       qh[i] = frag(img + IMG, wc * W + row, 0);
+    }
+    #pragma unroll
+    for (int i = 0; i < F; ++i) {
+      const int row = i * 16 + (lane & 15);
       pw[i] = frag(img, wr * W + row, 1);
       ql[i] = frag(img + IMG, wc * W + row, 1);
     }
-    if (kt + 1 < nk) stage(kt + 1);
-    #pragma unroll
-    for (int i = 0; i < F; ++i)
+    if (kt + S - 1 < nk) stage(kt + S - 1);
+    // kind by kind: an accumulator's next use is F * F instructions away
+    auto products = [&](const f16x8 (&p)[F], const f16x8 (&q)[F]) {
       #pragma unroll
-      for (int j = 0; j < F; ++j) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], qh[j],
-                                                           acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], ql[j],
-                                                           acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pw[i], qh[j],
-                                                           acc[i][j], 0, 0, 0);
-      }
+      for (int i = 0; i < F; ++i)
+        #pragma unroll
+        for (int j = 0; j < F; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[i], q[j],
+                                                             acc[i][j], 0, 0, 0);
+    };
+    products(ph, qh);
+    products(ph, ql);
+    products(pw, qh);
   }
 
   // a lane holds rows r..r+3 of column c
@@ -340,8 +352,9 @@ template <int T, int KIND>
 void product(const NsGroup& g, int from, float alpha, float beta,
              hipStream_t s) {
   const long blocks = KIND == APPLY ? g.all_rects : g.all_tris;
-  hipLaunchKernelGGL((ns_product_kernel<T, KIND>), dim3(blocks), dim3(256), 0,
-                     s, g, from, alpha, beta);
+  constexpr int S = T == 64 ? 4 : 2;
+  hipLaunchKernelGGL((ns_product_kernel<T, KIND, S>), dim3(blocks), dim3(256),
+                     S * 2 * T * 128, s, g, from, alpha, beta);
 }
 
 template <int T>
