@@ -13,7 +13,7 @@
 #include <cmath>
 #include <cstring>
 
-#include "newton_schulz.h"
+#include "newton_schulz_plan.h"
 
 namespace lo {
 struct ConvGeom {
@@ -847,86 +847,6 @@ void layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor mean,
 }
 
 // -------------------------------------------- Newton-Schulz and Muon ----
-constexpr int64_t kNsSide = 1 << 20;
-
-// coefficients (a, b, c per step) and the scales that keep every stored value
-// below 2^15: with singular values in [0, s] before a step, X's entries stay
-// below s, A's below s^2, B's below max |b t + c t^2| over t in [0, s^2], the
-// next X's below max |a t + b t^3 + c t^5| over [0, s]
-std::vector<lo::NsStep> ns_steps(const std::vector<double>& coeffs) {
-  TORCH_CHECK(!coeffs.empty() && coeffs.size() % 3 == 0,
-              "coefficients come in threes, for one step at least");
-  auto scale = [](double bound) {
-    TORCH_CHECK(std::isfinite(bound) && bound < 1048576.0,
-                "these coefficients let the singular values grow past 2^20");
-    int e;
-    std::frexp(std::max(bound, 1e-3), &e);  // bound < 2^e
-    return (float)std::ldexp(1.0, 15 - e);
-  };
-  std::vector<lo::NsStep> st(coeffs.size() / 3);
-  double s = 1.001;
-  float sx = scale(s);
-  for (size_t i = 0; i < st.size(); ++i) {
-    const double a = coeffs[3 * i], b = coeffs[3 * i + 1], c = coeffs[3 * i + 2];
-    TORCH_CHECK(std::isfinite(a) && std::isfinite(b) && std::isfinite(c),
-                "coefficients must be finite");
-    // both are largest at the end or where their derivative in q = t^2 is 0
-    const double end = s * s;
-    double mb = 0, ms = 0;
-    auto poly = [&](double q) {
-      if (q >= 0 && q <= end) mb = std::max(mb, std::abs(b * q + c * q * q));
-    };
-    auto value = [&](double q) {
-      if (q >= 0 && q <= end)
-        ms = std::max(ms, std::sqrt(q) * std::abs(a + b * q + c * q * q));
-    };
-    poly(end);
-    value(end);
-    if (c != 0) {
-      poly(-b / (2 * c));
-      const double d = 9 * b * b - 20 * a * c;
-      if (d >= 0) {
-        value((-3 * b + std::sqrt(d)) / (10 * c));
-        value((-3 * b - std::sqrt(d)) / (10 * c));
-      }
-    } else if (b != 0) {
-      value(-a / (3 * b));
-    }
-    const double next = ms * 1.001;
-    st[i] = {(float)a, (float)b, (float)c, sx, scale(s * s * 1.001),
-             scale(mb * 1.001), scale(next)};
-    sx = st[i].sn;
-    s = next;
-  }
-  return st;
-}
-
-int ns_tile(int64_t tiles128) { return tiles128 >= 256 ? 128 : 64; }
-
-int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-
-// fills what depends on the shape; ws and parts are set by the caller
-lo::NsMat ns_mat(int64_t rows, int64_t cols, int tile) {
-  lo::NsMat m{};
-  m.rows = (int)rows;
-  m.cols = (int)cols;
-  m.mp = (int)up(std::min(rows, cols), tile);
-  m.np = (int)up(std::max(rows, cols), tile);
-  m.chunks = (int)(up(rows * cols, lo::kNsChunk) / lo::kNsChunk);
-  m.gain = (float)std::sqrt(std::max(1.0, (double)rows / (double)cols));
-  return m;
-}
-
-struct NsCounts {
-  int64_t chunks, splits, tris, rects, halfs;
-};
-
-NsCounts ns_counts(const lo::NsMat& m, int tile) {
-  const int64_t tm = m.mp / tile, tn = m.np / tile;
-  return {m.chunks, (int64_t)(m.mp / 64) * (m.np / 64), tm * (tm + 1) / 2,
-          tm * tn, 8l * m.mp * m.np + 4l * m.mp * m.mp};
-}
-
 // G [batch, rows, cols] -> out
 void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
                    double eps) {
@@ -938,39 +858,44 @@ void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
                   out.device() == g.device(),
               "out must be contiguous and of g's shape, type and device");
   const int64_t rows = g.size(1), cols = g.size(2);
-  TORCH_CHECK(rows <= kNsSide && cols <= kNsSide, "sides end at ", kNsSide);
-  const auto st = ns_steps(coeffs);
+  TORCH_CHECK(rows <= lo::kNsSide && cols <= lo::kNsSide, "sides end at ", lo::kNsSide);
+  const auto st = lo::ns_steps(coeffs);
   if (g.numel() == 0) return;
   const c10::DeviceGuard guard(g.device());
-  const int64_t big = up(rows, 128) / 128 * (up(cols, 128) / 128);
-  const int tile = ns_tile(big * g.size(0));
-  const lo::NsMat m = ns_mat(rows, cols, tile);
-  const NsCounts n = ns_counts(m, tile);
+  auto mats = lo::ns_plan({{rows, cols}}, g.size(0));
+  lo::NsNeeds n;
+  lo::ns_place(mats, n);
   // at most 4 GiB of workspace beyond one matrix's own
   const int64_t most = std::max<int64_t>(1, (int64_t(1) << 31) / n.halfs);
   const int64_t group = std::min(g.size(0), most);
   auto bytes = g.options().dtype(at::kByte);
   auto ws = at::empty({group * n.halfs * 2}, bytes);
-  auto parts = at::empty({group * n.chunks * 8}, bytes);
+  auto sums = at::empty({group * n.chunks * 8}, bytes);
+  auto parts = at::empty({group * n.parts * 4}, bytes);
+  auto slots = at::empty({group * n.slots * 4}, bytes);
+  lo::NsGroup ng{};
+  ng.one = mats[0];
+  ng.src_step = rows * cols;
+  ng.ws_step = n.halfs;
+  ng.sum_step = (int)n.chunks;
+  ng.chunks = (int)n.chunks;
+  ng.splits = (int)n.splits;
+  ng.ws = ws.data_ptr();
+  ng.sums = (double*)sums.data_ptr();
+  ng.parts = (float*)parts.data_ptr();
+  ng.slots = (unsigned*)slots.data_ptr();
+  for (int k = 0; k < lo::NS_KINDS; ++k) {
+    ng.kinds[k] = (int)n.kinds[k];
+    ng.slot_step[k] = (int)n.slots;
+    ng.part_step[k] = n.parts;
+  }
   for (int64_t b0 = 0; b0 < g.size(0); b0 += group) {
     const int64_t count = std::min(group, g.size(0) - b0);
-    lo::NsGroup ng{};
     ng.count = (int)count;
-    ng.tile = tile;
-    ng.one = m;
-    ng.src_step = rows * cols;
-    ng.ws_step = n.halfs;
-    ng.part_step = n.chunks;
-    ng.chunks = n.chunks;
-    ng.splits = n.splits;
-    ng.tris = n.tris;
-    ng.rects = n.rects;
     ng.all_chunks = n.chunks * count;
     ng.all_splits = n.splits * count;
-    ng.all_tris = n.tris * count;
-    ng.all_rects = n.rects * count;
-    ng.ws = ws.data_ptr();
-    ng.parts = (double*)parts.data_ptr();
+    ng.all_slots = (int)(n.slots * count);
+    for (int k = 0; k < lo::NS_KINDS; ++k) ng.all_kinds[k] = n.kinds[k] * count;
     ng.one.src = b0 * rows * cols;
     const lo::NsInput in{g.data_ptr(), nullptr, 1.f, 0.f, 0};
     const lo::NsOutput o{out.data_ptr(), nullptr, nullptr, 0.f, 0.f};
@@ -982,7 +907,7 @@ void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
 
 // tables and workspace of the Muon steps over one arena's matrices
 struct MuonPlan {
-  at::Tensor table, ws, parts;
+  at::Tensor table, ws, sums, parts, slots;
   lo::NsGroup g{};
   int64_t numel;
 
@@ -992,62 +917,76 @@ struct MuonPlan {
     TORCH_CHECK(device.is_cuda(), "the plan's device must be a GPU");
     TORCH_CHECK(!views.empty(), "a Muon plan needs a matrix");
     std::sort(views.begin(), views.end());
-    int64_t end = 0, tiles = 0;
+    int64_t end = 0;
+    std::vector<std::pair<int64_t, int64_t>> sides;
     for (const auto& v : views) {
       TORCH_CHECK(v[0] >= end && v[0] % 8 == 0, "matrices must start on a "
                   "multiple of 8 elements and not overlap");
-      TORCH_CHECK(v[1] >= 1 && v[2] >= 1 && v[1] <= kNsSide && v[2] <= kNsSide,
-                  "matrix sides must be 1 to ", kNsSide);
+      TORCH_CHECK(v[1] >= 1 && v[2] >= 1 && v[1] <= lo::kNsSide &&
+                      v[2] <= lo::kNsSide,
+                  "matrix sides must be 1 to ", lo::kNsSide);
       end = v[0] + v[1] * v[2];
-      tiles += up(v[1], 128) / 128 * (up(v[2], 128) / 128);
+      sides.emplace_back(v[1], v[2]);
     }
     TORCH_CHECK(end <= numel, "a matrix ends outside the arena");
     const c10::DeviceGuard guard(device);
-    // the longest sums first, so that no block starts one last
-    std::stable_sort(views.begin(), views.end(), [](auto& a, auto& b) {
-      return std::max(a[1], a[2]) > std::max(b[1], b[2]);
-    });
-    g.tile = ns_tile(tiles);
-    g.count = (int)views.size();
-    std::vector<lo::NsMat> mats;
-    std::vector<int> starts[4];
-    NsCounts sum{};
-    for (const auto& v : views) {
-      lo::NsMat m = ns_mat(v[1], v[2], g.tile);
-      const NsCounts n = ns_counts(m, g.tile);
-      m.src = v[0];
-      m.ws = sum.halfs;
-      m.part = (int)sum.chunks;
-      const int64_t at[4] = {sum.chunks, sum.splits, sum.tris, sum.rects};
-      for (int i = 0; i < 4; ++i) starts[i].push_back((int)at[i]);
-      mats.push_back(m);
-      sum = {sum.chunks + n.chunks, sum.splits + n.splits, sum.tris + n.tris,
-             sum.rects + n.rects, sum.halfs + n.halfs};
-      TORCH_CHECK(sum.splits < INT_MAX && sum.chunks < INT_MAX,
-                  "too many elements for one plan");
+    auto mats = lo::ns_plan(sides, 1);
+    lo::NsNeeds n;
+    lo::ns_place(mats, n);
+    for (size_t i = 0; i < mats.size(); ++i) mats[i].src = views[i][0];
+    // a block list for each pass; the products' longest sums first, so that
+    // none of those starts last
+    std::vector<lo::NsBlock> lists[2 + lo::NS_KINDS];
+    for (int i = 0; i < (int)mats.size(); ++i) {
+      const lo::NsMat& m = mats[i];
+      for (int at = 0; at < m.chunks; ++at) lists[0].push_back({i, at});
+      for (int at = 0; at < m.mp / 64 * (m.np / 64); ++at)
+        lists[1].push_back({i, at});
     }
-    const int64_t all[4] = {sum.chunks, sum.splits, sum.tris, sum.rects};
-    for (int i = 0; i < 4; ++i) starts[i].push_back((int)all[i]);
-    const int64_t mb = mats.size() * sizeof(lo::NsMat);
-    const int64_t sb = starts[0].size() * sizeof(int);
-    auto host = at::empty({mb + 4 * sb}, at::kByte);
-    auto* p = host.data_ptr<uint8_t>();
-    std::memcpy(p, mats.data(), mb);
-    for (int i = 0; i < 4; ++i) std::memcpy(p + mb + i * sb, starts[i].data(), sb);
-    table = host.to(device);
-    ws = at::empty({sum.halfs * 2}, table.options());
-    parts = at::empty({sum.chunks * 8}, table.options());
-    auto* d = table.data_ptr<uint8_t>();
+    for (int k = 0; k < lo::NS_KINDS; ++k) {
+      std::vector<int> order(mats.size());
+      for (int i = 0; i < (int)mats.size(); ++i) order[i] = i;
+      auto work = [&](int i) {
+        const lo::NsMat& m = mats[i];
+        return lo::ns_depth(m, k) * m.tile * m.tile / m.kind[k].splits;
+      };
+      std::stable_sort(order.begin(), order.end(),
+                       [&](int a, int b) { return work(a) > work(b); });
+      for (int i : order)
+        for (int at = 0; at < (int)lo::ns_blocks(mats[i], k); ++at)
+          lists[2 + k].push_back({i, at});
+    }
+    size_t bytes = mats.size() * sizeof(lo::NsMat);
+    for (const auto& l : lists) bytes += l.size() * sizeof(lo::NsBlock);
+    auto host = at::empty({(int64_t)bytes}, at::kByte);
+    table = at::empty({(int64_t)bytes}, at::TensorOptions(at::kByte).device(device));
+    auto *h = host.data_ptr<uint8_t>(), *d = table.data_ptr<uint8_t>();
+    size_t pos = mats.size() * sizeof(lo::NsMat);
+    std::memcpy(h, mats.data(), pos);
     g.mats = (const lo::NsMat*)d;
-    const int** to[4] = {&g.chunk_starts, &g.split_starts, &g.tri_starts,
-                         &g.rect_starts};
-    for (int i = 0; i < 4; ++i) *to[i] = (const int*)(d + mb + i * sb);
-    g.all_chunks = sum.chunks;
-    g.all_splits = sum.splits;
-    g.all_tris = sum.tris;
-    g.all_rects = sum.rects;
+    const lo::NsBlock** to[] = {&g.chunk_blocks, &g.split_blocks,
+                                &g.kind_blocks[0], &g.kind_blocks[1],
+                                &g.kind_blocks[2]};
+    for (int i = 0; i < 2 + lo::NS_KINDS; ++i) {
+      const size_t b = lists[i].size() * sizeof(lo::NsBlock);
+      std::memcpy(h + pos, lists[i].data(), b);
+      *to[i] = (const lo::NsBlock*)(d + pos);
+      pos += b;
+    }
+    table.copy_(host);
+    ws = at::empty({n.halfs * 2}, table.options());
+    sums = at::empty({n.chunks * 8}, table.options());
+    parts = at::empty({n.parts * 4}, table.options());
+    slots = at::empty({n.slots * 4}, table.options());
+    g.count = (int)mats.size();
+    g.all_chunks = n.chunks;
+    g.all_splits = n.splits;
+    g.all_slots = (int)n.slots;
+    for (int k = 0; k < lo::NS_KINDS; ++k) g.all_kinds[k] = n.kinds[k];
     g.ws = ws.data_ptr();
-    g.parts = (double*)parts.data_ptr();
+    g.sums = (double*)sums.data_ptr();
+    g.parts = (float*)parts.data_ptr();
+    g.slots = (unsigned*)slots.data_ptr();
   }
 
   void step(at::Tensor master, at::Tensor grad, at::Tensor mom,
@@ -1062,14 +1001,13 @@ struct MuonPlan {
       TORCH_CHECK(t.device() == table.device(), "the plan is on ",
                   table.device());
     }
-    const auto st = ns_steps(coeffs);
+    const auto st = lo::ns_steps(coeffs);
     const c10::DeviceGuard guard(table.device());
     // the step may run on another stream than the plan was made on
     const c10::impl::VirtualGuardImpl impl(table.device().type());
     const c10::Stream now = impl.getStream(table.device());
-    table.record_stream(now);
-    ws.record_stream(now);
-    parts.record_stream(now);
+    for (const at::Tensor& t : {table, ws, sums, parts, slots})
+      if (t.numel()) t.record_stream(now);
     const lo::NsInput in{grad.data_ptr(), mom.data_ptr<float>(), (float)gscale,
                          (float)mu, nesterov ? 1 : 0};
     const lo::NsOutput out{nullptr, master.data_ptr<float>(),

@@ -5,30 +5,53 @@
 
 namespace lo {
 
-constexpr int kNsChunk = 8192;  // elements a block of the elementwise passes
+constexpr int kNsChunk = 8192;  // elements a block of the momentum pass
+
+// the products of a step: A = X X^T, C = a + b A + c A A^T, X' = C X
+enum { NS_GRAM, NS_POLY, NS_APPLY, NS_KINDS };
+
+// how a product's tiles are shared out: the first `whole` take one block each,
+// the others `splits` blocks, each a part of the sum
+struct NsTiles {
+  int whole, splits;
+  int slot;  // first split tile's counter
+  long part; // first split tile's partial sums (floats)
+};
 
 struct NsMat {
   long src;        // first element in the input
   long ws;         // first half of its workspace
   int rows, cols;  // as stored
+  int tile;        // 64 or 128
   int mp, np;      // short and long side, padded to whole tiles
-  int part;        // first of its partial sums
+  int sum;         // first of its partial norms
   int chunks;      // how many
   float gain;      // factor on the learning rate
+  NsTiles kind[NS_KINDS];
 };
 
-// A group of matrices, by a table (mats, *_starts with count + 1 prefix sums)
-// or, without one, count equal matrices spaced by the steps.
+// a block's matrix and its place in it
+struct NsBlock {
+  int mat, at;
+};
+
+// A group of matrices, by tables (mats; blocks of the momentum pass, of the
+// split and of the products) or, without them, count equal matrices spaced by
+// the steps.
 struct NsGroup {
   const NsMat* mats;
-  const int *chunk_starts, *split_starts, *tri_starts, *rect_starts;
-  int count, tile;
+  const NsBlock *chunk_blocks, *split_blocks, *kind_blocks[NS_KINDS];
+  int count;
   NsMat one;
-  long src_step, ws_step, part_step;
-  long chunks, splits, tris, rects;                   // of one of them
-  long all_chunks, all_splits, all_tris, all_rects;  // of the group
+  long src_step, ws_step, part_step[NS_KINDS];
+  int sum_step, slot_step[NS_KINDS];
+  int chunks, splits, kinds[NS_KINDS];             // blocks of one of them
+  long all_chunks, all_splits, all_kinds[NS_KINDS];  // of the group
   void* ws;
-  double* parts;
+  double* sums;
+  float* parts;
+  unsigned* slots;  // arrivals at a split tile, zero between calls
+  int all_slots;
 };
 
 // grad of the input's type; mom (fp32) or null
@@ -47,11 +70,11 @@ struct NsOutput {
   float lr, keep;
 };
 
-// one step's coefficients and the powers of two that X, A, B and the next X
+// one step's coefficients and the powers of two that X, A, C and the next X
 // are stored with
 struct NsStep {
   float a, b, c;
-  float sx, sa, sb, sn;
+  float sx, sa, sc, sn;
 };
 
 void launch_newton_schulz(const NsGroup& g, int dtype, const NsInput& in,

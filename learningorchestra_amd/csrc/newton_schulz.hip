@@ -1,7 +1,7 @@
 // Orthogonalisation by Newton-Schulz steps, and the Muon update around it.
 //
 //   X = G / (|G|_F + eps)
-//   A = X X^T;  B = b A + c A A^T;  X <- a X + B X        (each step)
+//   A = X X^T;  C = a + b A + c A A^T;  X <- C X          (each step)
 //
 // drives the singular values of G towards one and keeps its singular vectors.
 // X has the short side m as rows (G is taken transposed where it is tall).
@@ -17,12 +17,16 @@
 // Layout. A row holds 32 hi, then 32 lo values in turn, so that one 128-byte
 // line of a row feeds one 16x16x32 instruction of each kind. X is kept by rows
 // and, as Y, by columns: then every product is rows times rows,
-//   A = X X^T,  A A^T (A is symmetric),  X' = a X + B Y^T,
-// and A and B, being symmetric, are computed on one triangle of tiles and
+//   A = X X^T,  A A^T (A is symmetric),  X' = C Y^T,
+// and A and C, being symmetric, are computed on one triangle of tiles and
 // written to both. Sides are padded with zeros to whole tiles.
 //
-// A call works on a group of matrices at once; a block finds its matrix in a
-// table of tile counts (a batch of equal matrices needs no table).
+// Sharing out. A call works on a group of matrices at once: a block finds its
+// matrix and tile in a table made with the plan, or by arithmetic for a batch
+// of equal ones. Where tiles are few, or few are left over after full rounds
+// of the chip, several blocks sum a part of a tile each; the last to arrive
+// adds the parts, in their order, so that results do not depend on timing. No
+// block waits for another.
 
 #include "lo_common.h"
 #include "newton_schulz.h"
@@ -32,8 +36,15 @@ namespace lo {
 namespace {
 
 typedef _Float16 f16;
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// four elements at any element-aligned address
+template <typename T>
+struct Quad {
+  typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+};
 
 // element (row, k) of a split matrix with ld values a row; its lo half is 32
 // further
@@ -46,74 +57,133 @@ LO_DEVICE void split(float v, f16& hi, f16& lo) {
   lo = (f16)(v - (float)hi);
 }
 
-// the block's matrix, and its place within it in t
-LO_DEVICE NsMat find(const NsGroup& g, const int* __restrict__ starts, long per,
-                     long& t) {
-  if (!g.mats) {
-    const long i = t / per;
-    t -= i * per;
-    NsMat m = g.one;
-    m.src += i * g.src_step;
-    m.ws += i * g.ws_step;
-    m.part += (int)(i * g.part_step);
-    return m;
+LO_DEVICE unsigned pack(float v) {
+  f16 hi, lo;
+  split(v, hi, lo);
+  return (unsigned)__builtin_bit_cast(unsigned short, hi) |
+         (unsigned)__builtin_bit_cast(unsigned short, lo) << 16;
+}
+
+LO_DEVICE void unpack8(const u32x4& a, const u32x4& b, f16x8& hi, f16x8& lo) {
+  #pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const unsigned v = j < 4 ? a[j] : b[j - 4];
+    hi[j] = __builtin_bit_cast(f16, (unsigned short)v);
+    lo[j] = __builtin_bit_cast(f16, (unsigned short)(v >> 16));
   }
-  int lo = 0, hi = g.count;  // starts[lo] <= t < starts[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (starts[mid] <= t) lo = mid;
-    else hi = mid;
+}
+
+// the block's matrix, and its place within it
+LO_DEVICE NsMat find(const NsGroup& g, const NsBlock* __restrict__ table,
+                     int per, int id, int& at) {
+  if (g.mats) {
+    const NsBlock b = table[id];
+    at = b.at;
+    return g.mats[b.mat];
   }
-  t -= starts[lo];
-  return g.mats[lo];
+  const int i = id / per;
+  at = id - i * per;
+  NsMat m = g.one;
+  m.src += i * g.src_step;
+  m.ws += i * g.ws_step;
+  m.sum += i * g.sum_step;
+  #pragma unroll
+  for (int k = 0; k < NS_KINDS; ++k) {
+    m.kind[k].slot += i * g.slot_step[k];
+    m.kind[k].part += i * g.part_step[k];
+  }
+  return m;
 }
 
 // a matrix's workspace: X and Y, twice (a step reads one pair and writes the
-// other), A, B
+// other), A, C
 struct Planes {
   f16* w;
   long n, a_;
   LO_DEVICE f16* x(int i) const { return w + 2 * i * n; }
   LO_DEVICE f16* y(int i) const { return w + (2 * i + 1) * n; }
   LO_DEVICE f16* a() const { return w + 4 * n; }
-  LO_DEVICE f16* b() const { return w + 4 * n + a_; }
+  LO_DEVICE f16* c() const { return w + 4 * n + a_; }
 };
 
 LO_DEVICE Planes planes(const NsMat& m, void* ws) {
   return {(f16*)ws + m.ws, 2l * m.mp * m.np, 2l * m.mp * m.mp};
 }
 
+// n (at most 4) elements from i on; the rest are zero
 template <typename T>
-LO_DEVICE float grad_at(const NsInput& in, long i) {
-  const float g = (float)((const T*)in.grad)[i] * in.gscale;
-  return in.mom && in.nesterov ? g + in.mu * in.mom[i]
-                               : (in.mom ? in.mom[i] : g);
+LO_DEVICE f32x4 load4(const T* p, long i, int n) {
+  f32x4 v = {};
+  if (n >= 4) {
+    const typename Quad<T>::type q = *(const typename Quad<T>::type*)(p + i);
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (float)q[j];
+  } else {
+    #pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) v[j] = (float)p[i + j];
+  }
+  return v;
+}
+
+template <typename T>
+LO_DEVICE void store4(T* p, long i, int n, const f32x4& v) {
+  if (n >= 4) {
+    typename Quad<T>::type q;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = (T)v[j];
+    *(typename Quad<T>::type*)(p + i) = q;
+  } else {
+    #pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) p[i + j] = (T)v[j];
+  }
+}
+
+// the update's elements, from the momentum that the step has brought forward
+template <typename T>
+LO_DEVICE f32x4 update4(const NsInput& in, long i, int n) {
+  if (!in.mom) return load4((const T*)in.grad, i, n) * in.gscale;
+  const f32x4 m = load4(in.mom, i, n);
+  if (!in.nesterov) return m;
+  return load4((const T*)in.grad, i, n) * in.gscale + in.mu * m;
 }
 
 // momentum (where there is one) and the squares' sums of the update's
-// elements, one per kNsChunk of them
+// elements, one per kNsChunk of them, in 64 bits: no norm overflows
 template <typename T>
 __global__ __launch_bounds__(256) void ns_momentum_kernel(NsGroup g,
                                                           NsInput in) {
-  long t = blockIdx.x;
-  const NsMat m = find(g, g.chunk_starts, g.chunks, t);
+  int at;
+  const NsMat m = find(g, g.chunk_blocks, g.chunks, blockIdx.x, at);
   const long size = (long)m.rows * m.cols;
-  const long e0 = t * kNsChunk;
-  const long e1 = min(size, e0 + kNsChunk);
+  const long e0 = (long)at * kNsChunk;
   double acc = 0.0;
-  for (long e = e0 + threadIdx.x; e < e1; e += 256) {
+  #pragma unroll
+  for (int k = 0; k < kNsChunk / 1024; ++k) {
+    const long e = e0 + k * 1024 + threadIdx.x * 4;
+    const int n = (int)min(size - e, 4l);
+    if (n <= 0) continue;
     const long i = m.src + e;
-    if (in.mom)
-      in.mom[i] = in.mu * in.mom[i] + (float)((const T*)in.grad)[i] * in.gscale;
-    const float u = grad_at<T>(in, i);
-    acc += (double)u * (double)u;
+    f32x4 u = load4((const T*)in.grad, i, n) * in.gscale;
+    if (in.mom) {
+      const f32x4 v = in.mu * load4(in.mom, i, n) + u;
+      store4(in.mom, i, n, v);
+      u = in.nesterov ? u + in.mu * v : v;
+    }
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) acc += (double)u[j] * (double)u[j];
   }
   for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off);
   __shared__ double red[4];
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
   __syncthreads();
   if (threadIdx.x == 0)
-    g.parts[m.part + t] = red[0] + red[1] + red[2] + red[3];
+    g.sums[m.sum + at] = red[0] + red[1] + red[2] + red[3];
+  // the products' counters start a call at zero
+  const int stride = gridDim.x * 256;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < g.all_slots; i += stride)
+    g.slots[i] = 0;
 }
 
 // X and Y from the update: 64 x 64 elements a block
@@ -122,31 +192,40 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup g, NsInput in,
                                                        float scale, float eps) {
   __shared__ float tile[64][65];
   __shared__ double red[4];
-  long t = blockIdx.x;
-  const NsMat m = find(g, g.split_starts, g.splits, t);
+  int at;
+  const NsMat m = find(g, g.split_blocks, g.splits, blockIdx.x, at);
   const Planes p = planes(m, g.ws);
   const int tn = m.np / 64;
-  const int r0 = (int)(t / tn) * 64, c0 = (int)(t % tn) * 64;
+  const int r0 = at / tn * 64, c0 = at % tn * 64;
+  const bool tall = m.rows > m.cols;
 
+  // four elements along the input's rows a load
+  f32x4 v[4];
+  const int b = threadIdx.x % 16 * 4;
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int a = i * 16 + threadIdx.x / 16;
+    const int row = (tall ? c0 : r0) + a, col = (tall ? r0 : c0) + b;
+    v[i] = f32x4{};
+    if (row < m.rows && col < m.cols)
+      v[i] = update4<T>(in, m.src + (long)row * m.cols + col, m.cols - col);
+  }
   double acc = 0.0;
-  for (int i = threadIdx.x; i < m.chunks; i += 256) acc += g.parts[m.part + i];
+  for (int i = threadIdx.x; i < m.chunks; i += 256) acc += g.sums[m.sum + i];
   for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
   __syncthreads();
   const float norm = (float)sqrt(red[0] + red[1] + red[2] + red[3]);
-  const float f = scale / (norm + eps);
-
-  const bool tall = m.rows > m.cols;
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    // consecutive threads along the input's rows
-    const int a = i >> 6, b = i & 63;
-    const int row = tall ? c0 + a : r0 + a;
-    const int col = tall ? r0 + b : c0 + b;
-    float v = 0.f;
-    if (row < m.rows && col < m.cols)
-      v = grad_at<T>(in, m.src + (long)row * m.cols + col) * f;
-    if (tall) tile[b][a] = v;
-    else tile[a][b] = v;
+  const float f = 1.f / (norm + eps);
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int a = i * 16 + threadIdx.x / 16;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = v[i][j] * f * scale;
+      if (tall) tile[b + j][a] = x;
+      else tile[a][b + j] = x;
+    }
   }
   __syncthreads();
   const int r = threadIdx.x >> 2, k = (threadIdx.x & 3) * 16;
@@ -172,40 +251,73 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup g, NsInput in,
   }
 }
 
-// One product of a step on T x T tiles, four waves:
-//   GRAM   A  = X X^T             one triangle, written to both
-//   POLY   B  = b A + c A A^T     one triangle, written to both
-//   APPLY  X' = a X + B Y^T       written as X' and Y'
-// out = alpha * sum + beta * source, all of them carrying their scales.
-enum { GRAM, POLY, APPLY };
+// Tile l of a product, in bands of eight tile rows, down a band's columns
+// first: 64 tiles in turn read 8 + 8 panels. KIND APPLY covers tm x tn tiles,
+// the symmetric ones the lower triangle of tm x tm.
+template <int KIND>
+LO_DEVICE void tile_at(int l, int tm, int tn, int& ti, int& tj) {
+  if (KIND == NS_APPLY) {
+    const int band = l / (8 * tn);
+    const int h = min(8, tm - 8 * band);
+    l -= band * 8 * tn;
+    tj = l / h;
+    ti = 8 * band + l - tj * h;
+    return;
+  }
+  // band b starts at tile 32 b (b - 1) + 36 b
+  int b = (int)sqrtf((float)l * (1.f / 32.f));
+  while (32 * b * (b - 1) + 36 * b > l) --b;
+  while (32 * b * (b + 1) + 36 * (b + 1) <= l) ++b;
+  l -= 32 * b * (b - 1) + 36 * b;
+  const int h = min(8, tm - 8 * b);
+  if (l < h * 8 * b) {
+    tj = l / h;
+    ti = 8 * b + l - tj * h;
+    return;
+  }
+  l -= h * 8 * b;
+  int r = 0;
+  while ((r + 1) * (r + 2) / 2 <= l) ++r;
+  ti = 8 * b + r;
+  tj = 8 * b + l - r * (r + 1) / 2;
+}
 
-template <int T, int KIND, int S>
-__global__ __launch_bounds__(256) void ns_product_kernel(NsGroup g, int from,
-                                                         float alpha,
-                                                         float beta) {
+struct NsProduct {
+  int from;                // the X and Y that the step reads
+  float alpha, beta, diag; // out = alpha * sum + beta * A (+ diag where i = j)
+};
+
+// One product on T x T tiles, four waves, S staged tiles of both operands (32
+// values of the sum each) in LDS. FINAL: the last step's X' goes to the output
+// in place of the workspace.
+template <int T, int KIND, int S, typename O, bool FINAL>
+LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
+                            const NsProduct& pr, const NsOutput& out,
+                            char* lds) {
   constexpr int W = T / 2;      // a wave's square
   constexpr int F = W / 16;     // its 16 x 16 fragments a side
   constexpr int IMG = T * 128;  // bytes of one operand's tile: T rows, 32 k
   constexpr int LOADS = T / 32; // a wave's loads of one operand's tile
-  extern __shared__ __attribute__((aligned(1024))) char lds[];  // [S][2][IMG]
-  long t = xcd_swizzle(blockIdx.x, gridDim.x);
-  const NsMat m = find(g, KIND == APPLY ? g.rect_starts : g.tri_starts,
-                       KIND == APPLY ? g.rects : g.tris, t);
   const Planes pl = planes(m, g.ws);
-  int ti, tj;
-  if (KIND == APPLY) {
-    const int tm = m.mp / T;
-    ti = (int)(t % tm);
-    tj = (int)(t / tm);
-  } else {
-    ti = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while ((long)ti * (ti + 1) / 2 > t) --ti;
-    while ((long)(ti + 1) * (ti + 2) / 2 <= t) ++ti;
-    tj = (int)(t - (long)ti * (ti + 1) / 2);
+  const NsTiles& kd = m.kind[KIND];
+  int slice = 0, splits = 1, l = at, cut = -1;
+  if (at >= kd.whole) {
+    splits = kd.splits;
+    cut = (at - kd.whole) / splits;
+    slice = at - kd.whole - cut * splits;
+    l = kd.whole + cut;
   }
-  const int ld = KIND == GRAM ? m.np : m.mp;  // values a row of both operands
-  const f16* P = KIND == GRAM ? pl.x(from) : KIND == POLY ? pl.a() : pl.b();
-  const f16* Q = KIND == GRAM ? pl.x(from) : KIND == POLY ? pl.a() : pl.y(from);
+  int ti, tj;
+  tile_at<KIND>(l, m.mp / T, m.np / T, ti, tj);
+  const int ld = KIND == NS_GRAM ? m.np : m.mp;  // values a row of operands
+  const int nk = ld / 32;
+  const int k0 = nk * slice / splits, k1 = nk * (slice + 1) / splits;
+  const f16* P = KIND == NS_GRAM   ? pl.x(pr.from)
+                 : KIND == NS_POLY ? pl.a()
+                                   : pl.c();
+  const f16* Q = KIND == NS_GRAM   ? pl.x(pr.from)
+                 : KIND == NS_POLY ? pl.a()
+                                   : pl.y(pr.from);
   P += (long)ti * T * 2 * ld;
   Q += (long)tj * T * 2 * ld;
 
@@ -216,7 +328,7 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup g, int from,
   // at place p of a row is piece p ^ (row & 7), which spreads a column of
   // pieces over the banks
   auto stage = [&](int kt) {
-    char* buf = lds + (kt % S) * 2 * IMG;
+    char* buf = lds + (kt - k0) % S * 2 * IMG;
     #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int seg = wave * LOADS + i;
@@ -239,19 +351,18 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup g, int from,
   };
 
   f32x4 acc[F][F] = {};
-  const int nk = ld / 32;
-  for (int kt = 0; kt < S - 1; ++kt)
-    if (kt < nk) stage(kt);
-  for (int kt = 0; kt < nk; ++kt) {
+  for (int kt = k0; kt < k0 + S - 1; ++kt)
+    if (kt < k1) stage(kt);
+  for (int kt = k0; kt < k1; ++kt) {
     // tile kt has landed (the S - 2 after it may be on their way), and every
     // wave is done with the buffer that the next one goes to
-    if (kt + S - 2 < nk)
+    if (kt + S - 2 < k1)
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(
                        (S - 2) * 2 * LOADS)
                    : "memory");
     else
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const char* img = lds + (kt % S) * 2 * IMG;
+    const char* img = lds + (kt - k0) % S * 2 * IMG;
     f16x8 ph[F], pw[F], qh[F], ql[F];
     #pragma unroll
     for (int i = 0; i < F; ++i) {
@@ -265,7 +376,7 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup g, int from,
       pw[i] = frag(img, wr * W + row, 1);
       ql[i] = frag(img + IMG, wc * W + row, 1);
     }
-    if (kt + S - 1 < nk) stage(kt + S - 1);
+    if (kt + S - 1 < k1) stage(kt + S - 1);
     // kind by kind: an accumulator's next use is F * F instructions away
     auto products = [&](const f16x8 (&p)[F], const f16x8 (&q)[F]) {
       #pragma unroll
@@ -279,94 +390,192 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup g, int from,
     products(ph, ql);
     products(pw, qh);
   }
+  __syncthreads();  // the staging buffers are free from here on
 
-  // a lane holds rows r..r+3 of column c
-  f16* rowsOut = KIND == GRAM ? pl.a() : KIND == POLY ? pl.b() : pl.x(from ^ 1);
-  f16* colsOut = KIND == APPLY ? pl.y(from ^ 1) : rowsOut;
-  const f16* source = KIND == POLY ? pl.a() : pl.y(from);
-  const int ldr = KIND == APPLY ? m.np : m.mp;
-  const bool both = KIND == APPLY || ti != tj;
+  if (splits > 1) {
+    // Parts are written through to where all dies see them (agent-scope
+    // stores), and have arrived there before the counter goes up: no cache
+    // needs writing back. The last block drops what its die holds of others'.
+    typedef unsigned long long u64;
+    u64* part = (u64*)(g.parts + kd.part + (long)cut * splits * T * T);
+    const int mine = wave * F * F * 128 + lane;
+    #pragma unroll
+    for (int i = 0; i < F * F; ++i) {
+      const f32x4& v = acc[i / F][i % F];
+      u64* to = part + (long)slice * (T * T / 2) + mine + i * 128;
+      __hip_atomic_store(to, __builtin_bit_cast(u64, f32x2{v[0], v[1]}),
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(to + 64, __builtin_bit_cast(u64, f32x2{v[2], v[3]}),
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    unsigned* last = (unsigned*)lds;
+    if (threadIdx.x == 0)
+      *last = __hip_atomic_fetch_add(g.slots + kd.slot + cut, 1u,
+                                     __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const bool join = *last == (unsigned)splits - 1;
+    if (!join) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    __syncthreads();  // all have read it
+    if (threadIdx.x == 0)
+      __hip_atomic_store(g.slots + kd.slot + cut, 0u, __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+    f32x4 own[F * F];
+    #pragma unroll
+    for (int i = 0; i < F * F; ++i) {
+      own[i] = acc[i / F][i % F];
+      acc[i / F][i % F] = f32x4{};
+    }
+    for (int q = 0; q < splits; ++q) {
+      u64* from = part + (long)q * (T * T / 2) + mine;
+      #pragma unroll
+      for (int i = 0; i < F * F; ++i) {
+        f32x4 v = own[i];
+        if (q != slice) {
+          const f32x2 a = __builtin_bit_cast(
+              f32x2, __hip_atomic_load(from + i * 128, __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT));
+          const f32x2 b = __builtin_bit_cast(
+              f32x2, __hip_atomic_load(from + i * 128 + 64, __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT));
+          v = f32x4{a.x, a.y, b.x, b.y};
+        }
+        acc[i / F][i % F] += v;
+      }
+    }
+  }
+
+  // a lane holds rows r..r+3 of column c of each fragment; each wave turns its
+  // square in its own part of LDS, so that it can write whole lines by rows
+  // and by columns
+  constexpr int PITCH = W + 4;
+  unsigned* sq = (unsigned*)lds + wave * W * PITCH;
+  const int rw = ti * T + wr * W, cw = tj * T + wc * W;
   #pragma unroll
   for (int i = 0; i < F; ++i)
     #pragma unroll
     for (int j = 0; j < F; ++j) {
-      const int r = ti * T + wr * W + i * 16 + (lane >> 4) * 4;
-      const int c = tj * T + wc * W + j * 16 + (lane & 15);
-      const long col = split_at(c, r, m.mp);
-      f32x4 v = acc[i][j] * alpha;
-      if (KIND != GRAM) {
-        const f16x4 sh = *(const f16x4*)(source + col);
-        const f16x4 sl = *(const f16x4*)(source + col + 32);
+      const int r = i * 16 + (lane >> 4) * 4, c = j * 16 + (lane & 15);
+      f32x4 v = acc[i][j] * pr.alpha;
+      if (KIND == NS_POLY) {
+        // A is symmetric: its row c holds the four in a line
+        typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+        const f16* s = pl.a() + split_at(cw + c, rw + r, m.mp);
+        const f16x4 sh = *(const f16x4*)s, sl = *(const f16x4*)(s + 32);
         #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] += beta * ((float)sh[e] + (float)sl[e]);
+        for (int e = 0; e < 4; ++e) {
+          v[e] += pr.beta * ((float)sh[e] + (float)sl[e]);
+          if (rw + r + e == cw + c) v[e] += pr.diag;
+        }
       }
-      f16x4 hi, lo;
       #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        f16 h, l;
-        split(v[e], h, l);
-        hi[e] = h;
-        lo[e] = l;
-        const long at = split_at(r + e, c, ldr);
-        rowsOut[at] = h;
-        rowsOut[at + 32] = l;
-      }
-      if (both) {
-        *(f16x4*)(colsOut + col) = hi;
-        *(f16x4*)(colsOut + col + 32) = lo;
+        const float x = v[e];
+        sq[(r + e) * PITCH + c] = FINAL ? __builtin_bit_cast(unsigned, x)
+                                        : pack(x);
       }
     }
-}
-
-// the result in the input's own layout, 32 columns of a row per 8 threads
-template <typename T>
-__global__ __launch_bounds__(256) void ns_store_kernel(NsGroup g, int from,
-                                                       float unscale,
-                                                       NsOutput out) {
-  long t = blockIdx.x;
-  const NsMat m = find(g, g.chunk_starts, g.chunks, t);
-  const Planes p = planes(m, g.ws);
+  // only this wave reads its square, after its own writes
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   const bool tall = m.rows > m.cols;
-  const f16* src = tall ? p.y(from) : p.x(from);
-  const int ld = tall ? m.mp : m.np;
-  const long size = (long)m.rows * m.cols;
-  const long e1 = min(size, (t + 1) * kNsChunk);
-  const float step = out.lr * m.gain;
-  for (long e = t * kNsChunk + threadIdx.x; e < e1; e += 256) {
-    const long row = e / m.cols;
-    const long at = split_at(row, (int)(e - row * m.cols), ld);
-    const float o = ((float)src[at] + (float)src[at + 32]) * unscale;
-    const long i = m.src + e;
-    if (out.master) {
-      const float w = out.master[i] * out.keep - step * o;
-      out.master[i] = w;
-      ((bf16*)out.mirror)[i] = tobf16(w);
-    } else {
-      ((T*)out.out)[i] = (T)o;
+  // 8 values by rows: (r, c) .. (r, c + 7); by columns: (r, c) .. (r + 7, c)
+  auto along_row = [&](int idx, int& r, int& c, u32x4& a, u32x4& b) {
+    r = idx / (W / 8);
+    c = idx % (W / 8) * 8;
+    a = *(const u32x4*)(sq + r * PITCH + c);
+    b = *(const u32x4*)(sq + r * PITCH + c + 4);
+  };
+  auto along_col = [&](int idx, int& r, int& c, u32x4& a, u32x4& b) {
+    r = (idx >> 4) % (W / 8) * 8;
+    c = (idx >> 4) / (W / 8) * 16 + (idx & 15);
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a[j] = sq[(r + j) * PITCH + c];
+      b[j] = sq[(r + 4 + j) * PITCH + c];
+    }
+  };
+  if constexpr (FINAL) {
+    const float step = out.lr * m.gain;
+    #pragma unroll 2
+    for (int idx = lane; idx < W * W / 8; idx += 64) {
+      int r, c;
+      u32x4 a, b;
+      if (tall) along_col(idx, r, c, a, b);
+      else along_row(idx, r, c, a, b);
+      const int row = tall ? cw + c : rw + r, col = tall ? rw + r : cw + c;
+      if (row >= m.rows) continue;
+      #pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int n = m.cols - col - h * 4;
+        if (n <= 0) continue;
+        const f32x4 o = __builtin_bit_cast(f32x4, h ? b : a);
+        const long i = m.src + (long)row * m.cols + col + h * 4;
+        if (out.master) {
+          const f32x4 w = load4(out.master, i, n) * out.keep - step * o;
+          store4(out.master, i, n, w);
+          store4((bf16*)out.mirror, i, n, w);
+        } else {
+          store4((O*)out.out, i, n, o);
+        }
+      }
+    }
+  } else {
+    f16* rows = KIND == NS_GRAM   ? pl.a()
+                : KIND == NS_POLY ? pl.c()
+                                  : pl.x(pr.from ^ 1);
+    f16* cols = KIND == NS_APPLY ? pl.y(pr.from ^ 1) : rows;
+    const int ldr = KIND == NS_APPLY ? m.np : m.mp;
+    #pragma unroll 4
+    for (int idx = lane; idx < W * W / 8; idx += 64) {
+      int r, c;
+      u32x4 a, b;
+      f16x8 hi, lo;
+      along_row(idx, r, c, a, b);
+      unpack8(a, b, hi, lo);
+      f16* to = rows + split_at(rw + r, cw + c, ldr);
+      *(f16x8*)to = hi;
+      *(f16x8*)(to + 32) = lo;
+      if (KIND == NS_APPLY || ti != tj) {
+        along_col(idx, r, c, a, b);
+        unpack8(a, b, hi, lo);
+        to = cols + split_at(cw + c, rw + r, m.mp);
+        *(f16x8*)to = hi;
+        *(f16x8*)(to + 32) = lo;
+      }
     }
   }
 }
 
-template <int T, int KIND>
-void product(const NsGroup& g, int from, float alpha, float beta,
-             hipStream_t s) {
-  const long blocks = KIND == APPLY ? g.all_rects : g.all_tris;
-  constexpr int S = T == 64 ? 4 : 2;
-  hipLaunchKernelGGL((ns_product_kernel<T, KIND, S>), dim3(blocks), dim3(256),
-                     S * 2 * T * 128, s, g, from, alpha, beta);
+template <int KIND, typename O, bool FINAL>
+__global__ __launch_bounds__(256, 2) void ns_product_kernel(NsGroup g,
+                                                            NsProduct pr,
+                                                            NsOutput out) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  // equal matrices: neighbouring tiles on one die, for its cache (the split
+  // tiles of a single one are spread over all dies); a table's order, longest
+  // sums first, is kept
+  int id = blockIdx.x;
+  const int whole = g.count == 1 ? g.one.kind[KIND].whole : (int)gridDim.x;
+  if (!g.mats && id < whole) id = xcd_swizzle(id, whole);
+  int at;
+  const NsMat m = find(g, g.kind_blocks[KIND], g.kinds[KIND], id, at);
+  if (m.tile == 128)
+    product_tile<128, KIND, 2, O, FINAL>(g, m, at, pr, out, lds);
+  else
+    product_tile<64, KIND, 4, O, FINAL>(g, m, at, pr, out, lds);
 }
 
-template <int T>
-int steps(const NsGroup& g, const NsStep* st, int n, hipStream_t s) {
-  int from = 0;
-  for (int i = 0; i < n; ++i, from ^= 1) {
-    const NsStep& k = st[i];
-    product<T, GRAM>(g, from, k.sa / (k.sx * k.sx), 0.f, s);
-    product<T, POLY>(g, from, k.c * k.sb / (k.sa * k.sa), k.b * k.sb / k.sa, s);
-    product<T, APPLY>(g, from, k.sn / (k.sb * k.sx), k.a * k.sn / k.sx, s);
-  }
-  return from;
+// both tile sizes' staging buffers take 64 KiB; 128's squares need 4 KiB more
+constexpr int kNsLds = 4 * 64 * (64 + 4) * 4;
+
+template <int KIND, typename O, bool FINAL>
+void product(const NsGroup& g, const NsProduct& pr, const NsOutput& out,
+             hipStream_t s) {
+  hipLaunchKernelGGL((ns_product_kernel<KIND, O, FINAL>),
+                     dim3(g.all_kinds[KIND]), dim3(256), kNsLds, s, g, pr, out);
 }
 
 template <typename T>
@@ -376,10 +585,19 @@ void run(const NsGroup& g, const NsInput& in, const NsStep* st, int n,
                      g, in);
   hipLaunchKernelGGL(ns_split_kernel<T>, dim3(g.all_splits), dim3(256), 0, s, g,
                      in, st[0].sx, eps);
-  const int from = g.tile == 128 ? steps<128>(g, st, n, s)
-                                 : steps<64>(g, st, n, s);
-  hipLaunchKernelGGL(ns_store_kernel<T>, dim3(g.all_chunks), dim3(256), 0, s, g,
-                     from, 1.f / st[n - 1].sn, out);
+  for (int i = 0; i < n; ++i) {
+    const NsStep& k = st[i];
+    const int from = i & 1;
+    product<NS_GRAM, float, false>(g, {from, k.sa / (k.sx * k.sx), 0.f, 0.f}, out,
+                               s);
+    product<NS_POLY, float, false>(
+        g, {from, k.c * k.sc / (k.sa * k.sa), k.b * k.sc / k.sa, k.a * k.sc},
+        out, s);
+    const float next = i + 1 < n ? k.sn : 1.f;
+    const NsProduct pr{from, next / (k.sc * k.sx), 0.f, 0.f};
+    if (i + 1 < n) product<NS_APPLY, float, false>(g, pr, out, s);
+    else product<NS_APPLY, T, true>(g, pr, out, s);
+  }
 }
 
 }  // namespace

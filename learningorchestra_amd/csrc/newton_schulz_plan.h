@@ -1,0 +1,164 @@
+// Host side of newton_schulz.hip: how the products are scaled and shared out.
+#pragma once
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <stdexcept>
+#include <vector>
+
+#include "newton_schulz.h"
+
+namespace lo {
+
+constexpr int64_t kNsSide = 1 << 20;
+constexpr int64_t kNsSlots = 512;  // blocks that run at once: two on each CU
+
+inline int64_t ns_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// The coefficients (a, b, c of each step) with the scales that keep every
+// stored value below 2^15: with singular values in [0, s] before a step, X's
+// entries stay below s, A's below s^2, C's below max |a + b q + c q^2| over
+// q in [0, s^2] and the next X's below max t |a + b t^2 + c t^4| over [0, s].
+inline std::vector<NsStep> ns_steps(const std::vector<double>& coeffs) {
+  if (coeffs.empty() || coeffs.size() % 3)
+    throw std::invalid_argument(
+        "coefficients come in threes, for one step at least");
+  auto scale = [](double bound) {
+    if (!(bound < 1048576.0))
+      throw std::invalid_argument(
+          "these coefficients let the singular values grow past 2^20");
+    int e;
+    std::frexp(std::max(bound * 1.001, 1e-3), &e);  // bound < 2^e
+    return (float)std::ldexp(1.0, 15 - e);
+  };
+  std::vector<NsStep> st(coeffs.size() / 3);
+  double s = 1.001;
+  float sx = scale(s);
+  for (size_t i = 0; i < st.size(); ++i) {
+    const double a = coeffs[3 * i], b = coeffs[3 * i + 1], c = coeffs[3 * i + 2];
+    const double end = s * s;
+    double most_c = 0, most_x = 0;
+    auto try_at = [&](double q) {
+      if (!(q >= 0 && q <= end)) return;
+      const double v = std::abs(a + b * q + c * q * q);
+      most_c = std::max(most_c, v);
+      most_x = std::max(most_x, std::sqrt(q) * v);
+    };
+    try_at(0);
+    try_at(end);
+    if (c != 0) {  // where either one's derivative in q is zero
+      try_at(-b / (2 * c));
+      const double d = 9 * b * b - 20 * a * c;
+      if (d >= 0) {
+        try_at((-3 * b + std::sqrt(d)) / (10 * c));
+        try_at((-3 * b - std::sqrt(d)) / (10 * c));
+      }
+    } else if (b != 0) {
+      try_at(-a / (3 * b));
+    }
+    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c))
+      throw std::invalid_argument("coefficients must be finite");
+    st[i] = {(float)a, (float)b, (float)c, sx, scale(end), scale(most_c),
+             scale(most_x)};
+    sx = st[i].sn;
+    s = most_x * 1.001;
+  }
+  return st;
+}
+
+// what a plan's matrices need together
+struct NsNeeds {
+  int64_t halfs = 0, chunks = 0, splits = 0, parts = 0, slots = 0;
+  int64_t kinds[NS_KINDS] = {};
+};
+
+inline int64_t ns_tiles(const NsMat& m, int kind) {
+  const int64_t tm = m.mp / m.tile, tn = m.np / m.tile;
+  return kind == NS_APPLY ? tm * tn : tm * (tm + 1) / 2;
+}
+
+inline int64_t ns_depth(const NsMat& m, int kind) {
+  return (kind == NS_GRAM ? m.np : m.mp) / 32;
+}
+
+inline int64_t ns_blocks(const NsMat& m, int kind) {
+  const NsTiles& k = m.kind[kind];
+  return k.whole + (ns_tiles(m, kind) - k.whole) * k.splits;
+}
+
+// Shapes, tiles and sharing of `copies` of each of the matrices.
+inline std::vector<NsMat> ns_plan(
+    const std::vector<std::pair<int64_t, int64_t>>& sides, int64_t copies) {
+  int64_t big = 0;
+  for (auto [rows, cols] : sides)
+    big += ns_up(rows, 128) / 128 * (ns_up(cols, 128) / 128) * copies;
+  std::vector<NsMat> mats;
+  for (auto [rows, cols] : sides) {
+    NsMat m{};
+    m.rows = (int)rows;
+    m.cols = (int)cols;
+    m.tile = big >= 256 && std::min(rows, cols) > 64 ? 128 : 64;
+    m.mp = (int)ns_up(std::min(rows, cols), m.tile);
+    m.np = (int)ns_up(std::max(rows, cols), m.tile);
+    m.chunks = (int)(ns_up(rows * cols, kNsChunk) / kNsChunk);
+    m.gain = (float)std::sqrt(std::max(1.0, (double)rows / (double)cols));
+    mats.push_back(m);
+  }
+  for (int kind = 0; kind < NS_KINDS; ++kind) {
+    int64_t all = 0;
+    for (const NsMat& m : mats) all += ns_tiles(m, kind) * copies;
+    for (NsMat& m : mats) {
+      const int64_t tiles = ns_tiles(m, kind), depth = ns_depth(m, kind);
+      // s blocks take depth / s steps each and the last of them s additions
+      // of a tile; a step costs about as much as 2 additions (64) or one
+      const int64_t most = std::max<int64_t>(
+          1, (int64_t)std::sqrt((double)depth * (m.tile == 64 ? 2 : 1)));
+      NsTiles& k = m.kind[kind];
+      k.whole = (int)tiles;
+      k.splits = 1;
+      if (all < kNsSlots) {
+        const int64_t s = std::min({kNsSlots / all, most, depth});
+        if (s > 1) k.whole = 0, k.splits = (int)s;
+      } else if (mats.size() * copies == 1) {
+        // what full rounds of the chip leave over
+        const int64_t rest = all % kNsSlots;
+        const int64_t s =
+            rest ? std::min({kNsSlots / rest, most, depth}) : 1;
+        if (s > 1 && all < 4 * kNsSlots)
+          k.whole = (int)(tiles - rest), k.splits = (int)s;
+      }
+    }
+  }
+  return mats;
+}
+
+// gives the matrices their places, one after the other, and adds them up (the
+// products of a step run one after the other and share parts and slots)
+inline void ns_place(std::vector<NsMat>& mats, NsNeeds& sum) {
+  int64_t part[NS_KINDS] = {}, slot[NS_KINDS] = {};
+  for (NsMat& m : mats) {
+    m.ws = sum.halfs;
+    m.sum = (int)sum.chunks;
+    sum.halfs += 8l * m.mp * m.np + 4l * m.mp * m.mp;
+    sum.chunks += m.chunks;
+    sum.splits += (int64_t)(m.mp / 64) * (m.np / 64);
+    for (int k = 0; k < NS_KINDS; ++k) {
+      NsTiles& t = m.kind[k];
+      const int64_t cut = ns_tiles(m, k) - t.whole;
+      t.part = part[k];
+      t.slot = (int)slot[k];
+      part[k] += cut * t.splits * m.tile * m.tile;
+      slot[k] += cut;
+      sum.kinds[k] += ns_blocks(m, k);
+      sum.parts = std::max(sum.parts, part[k]);
+      sum.slots = std::max(sum.slots, slot[k]);
+    }
+  }
+  const int64_t most = INT32_MAX;
+  if (sum.chunks > most || sum.splits > most || sum.kinds[NS_APPLY] > most ||
+      sum.kinds[NS_GRAM] > most)
+    throw std::invalid_argument("too many elements for one plan");
+}
+
+}  // namespace lo
