@@ -863,6 +863,19 @@ void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
   if (g.numel() == 0) return;
   const c10::DeviceGuard guard(g.device());
   auto mats = lo::ns_plan({{rows, cols}}, g.size(0));
+  const lo::NsInput in{g.data_ptr(), nullptr, 1.f, 0.f, 0};
+  const lo::NsOutput o{out.data_ptr(), nullptr, nullptr, 0.f, 0.f};
+  if (lo::ns_fits_block(mats[0]) && (int)st.size() <= lo::kNsSmallSteps) {
+    lo::NsGroup ng{};
+    ng.one = mats[0];
+    ng.src_step = rows * cols;
+    ng.count = (int)g.size(0);
+    lo::launch_newton_schulz_small(ng, (int)std::max(rows, cols), code, in,
+                                   st.data(), (int)st.size(), (float)eps, o,
+                                   stream());
+    check_launch("orthogonalize");
+    return;
+  }
   lo::NsNeeds n;
   lo::ns_place(mats, n);
   // at most 4 GiB of workspace beyond one matrix's own
@@ -897,8 +910,6 @@ void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
     ng.all_slots = (int)(n.slots * count);
     for (int k = 0; k < lo::NS_KINDS; ++k) ng.all_kinds[k] = n.kinds[k] * count;
     ng.one.src = b0 * rows * cols;
-    const lo::NsInput in{g.data_ptr(), nullptr, 1.f, 0.f, 0};
-    const lo::NsOutput o{out.data_ptr(), nullptr, nullptr, 0.f, 0.f};
     lo::launch_newton_schulz(ng, code, in, st.data(), (int)st.size(),
                              (float)eps, o, stream());
     check_launch("orthogonalize");
@@ -910,6 +921,7 @@ struct MuonPlan {
   at::Tensor table, ws, sums, parts, slots;
   lo::NsGroup g{};
   int64_t numel;
+  int longest = 0;  // side, where all matrices fit a block
 
   MuonPlan(std::vector<std::array<int64_t, 3>> views, int64_t numel_,
            at::Device device)
@@ -934,6 +946,12 @@ struct MuonPlan {
     lo::NsNeeds n;
     lo::ns_place(mats, n);
     for (size_t i = 0; i < mats.size(); ++i) mats[i].src = views[i][0];
+    bool fit = true;
+    for (const lo::NsMat& m : mats) {
+      fit = fit && lo::ns_fits_block(m);
+      longest = std::max({longest, m.rows, m.cols});
+    }
+    if (!fit) longest = 0;
     // a block list for each pass; the products' longest sums first, so that
     // none of those starts last
     std::vector<lo::NsBlock> lists[2 + lo::NS_KINDS];
@@ -1013,8 +1031,12 @@ struct MuonPlan {
     const lo::NsOutput out{nullptr, master.data_ptr<float>(),
                            mirror.data_ptr(), (float)lr,
                            (float)(1.0 - lr * wd)};
-    lo::launch_newton_schulz(g, 2, in, st.data(), (int)st.size(), (float)eps,
-                             out, stream());
+    if (longest && (int)st.size() <= lo::kNsSmallSteps)
+      lo::launch_newton_schulz_small(g, longest, 2, in, st.data(),
+                                     (int)st.size(), (float)eps, out, stream());
+    else
+      lo::launch_newton_schulz(g, 2, in, st.data(), (int)st.size(), (float)eps,
+                               out, stream());
     check_launch("muon_step");
   }
 };

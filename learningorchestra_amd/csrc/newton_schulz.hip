@@ -36,6 +36,8 @@ namespace lo {
 namespace {
 
 typedef _Float16 f16;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -462,7 +464,6 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
       f32x4 v = acc[i][j] * pr.alpha;
       if (KIND == NS_POLY) {
         // A is symmetric: its row c holds the four in a line
-        typedef f16 f16x4 __attribute__((ext_vector_type(4)));
         const f16* s = pl.a() + split_at(cw + c, rw + r, m.mp);
         const f16x4 sh = *(const f16x4*)s, sl = *(const f16x4*)(s + 32);
         #pragma unroll
@@ -568,6 +569,330 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(NsGroup g,
     product_tile<64, KIND, 4, O, FINAL>(g, m, at, pr, out, lds);
 }
 
+// ------------------------------------------- matrices that fit one block ----
+// Up to 64 rows and 1024 columns: one block does the whole call, momentum and
+// norm included, with X in the registers of its eight waves.
+//
+// A wave owns groups of 32 columns. A lane's share of X serves as it is as an
+// operand of both products, because the order in which a sum is taken is free
+// as long as both operands follow it: the accumulator of X' = C X gives lane
+// (g, c) = (lane / 16, lane % 16) rows 16 b + 4 g + e of column c, and so the
+// sum over rows runs, in steps f of 32, over rows 32 f + 4 g + (0..3) and
+// 32 f + 16 + 4 g + (0..3); C is laid out in that order in LDS. Its transpose,
+// from the same operands swapped, is in the same way ready for X' X'^T. The
+// waves' shares of A meet in LDS, where C is made from it.
+//
+// A step of 64 x 800 takes 26 groups * 126 matrix instructions on one CU; the
+// other 255 are free for the rest of a batch.
+struct NsSmallSteps {
+  NsStep st[kNsSmallSteps];
+  int n;
+};
+
+// byte offset of the 16-byte piece (row, f, half, g) of a 64 x 64 image; the
+// exclusive or spreads a column of pieces over the banks
+LO_DEVICE int piece(int row, int f, int half, int g) {
+  return row * 256 + (((f * 8 + half * 4 + g) ^ (row & 15)) << 4);
+}
+
+// rows 16 b + 4 g + (0..3) of column c, four values, into row c of an image of
+// a symmetric matrix
+LO_DEVICE void put4(char* img, int c, int b, int g, const f32x4& v) {
+  f16x4 hi, lo;
+  #pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f16 h, l;
+    split(v[e], h, l);
+    hi[e] = h;
+    lo[e] = l;
+  }
+  *(f16x4*)(img + piece(c, b >> 1, 0, g) + (b & 1) * 8) = hi;
+  *(f16x4*)(img + piece(c, b >> 1, 1, g) + (b & 1) * 8) = lo;
+}
+
+// eight values as packed halves (kept as words: a vector of f16 that lives
+// across a loop is given a register an element)
+struct Halves {
+  u32x4 hi, lo;
+};
+
+LO_DEVICE Halves halves(const f32x4& a, const f32x4& b, float scale) {
+  Halves h;
+  #pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f16x2 hi, lo;
+    #pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = (j & 1) * 2 + e;
+      f16 vh, vl;
+      split((j < 2 ? a[i] : b[i]) * scale, vh, vl);
+      hi[e] = vh;
+      lo[e] = vl;
+    }
+    h.hi[j] = __builtin_bit_cast(unsigned, hi);
+    h.lo[j] = __builtin_bit_cast(unsigned, lo);
+  }
+  return h;
+}
+
+LO_DEVICE f32x4 mma(const u32x4& p, const u32x4& q, const f32x4& acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, p),
+                                                __builtin_bit_cast(f16x8, q),
+                                                acc, 0, 0, 0);
+}
+
+LO_DEVICE void mma3(f32x4& acc, const Halves& p, const Halves& q) {
+  acc = mma(p.lo, q.hi, acc);
+  acc = mma(p.hi, q.lo, acc);
+  acc = mma(p.hi, q.hi, acc);
+}
+
+// keeps what is read from LDS or computed for an address on its side: a group
+// of columns re-reads C rather than hold all of it in registers
+LO_DEVICE void keep_apart() { asm volatile("" ::: "memory"); }
+
+LO_DEVICE Halves get(const char* img, int row, int f, int g) {
+  return {*(const u32x4*)(img + piece(row, f, 0, g)),
+          *(const u32x4*)(img + piece(row, f, 1, g))};
+}
+
+constexpr int kNsTri = 10;  // 16 x 16 blocks of a 64 x 64 lower triangle
+constexpr int kNsSmallLds = 2 * 64 * 256 + 8 * kNsTri * 1024;
+
+// NG groups of 32 columns a wave
+template <typename T, int NG>
+__global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in,
+                                                          NsSmallSteps steps,
+                                                          float eps,
+                                                          NsOutput out) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  char* imgA = lds;
+  char* imgC = lds + 64 * 256;
+  f32x4* parts = (f32x4*)(lds + 2 * 64 * 256);  // [8][kNsTri][64]
+  __shared__ double red[8];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int g = lane >> 4, cl = lane & 15;
+  NsMat m = gr.mats ? gr.mats[blockIdx.x] : gr.one;
+  if (!gr.mats) m.src += blockIdx.x * gr.src_step;
+  const bool tall = m.rows > m.cols;
+  const int short_ = min(m.rows, m.cols), long_ = max(m.rows, m.cols);
+  const int groups = (long_ + 31) / 32;
+
+  // element (r, c) of X and its place in the input
+  auto inside = [&](int r, int c) { return r < short_ && c < long_; };
+  auto place = [&](int r, int c) {
+    return m.src + (tall ? (long)c * m.cols + r : (long)r * m.cols + c);
+  };
+
+  f32x4 u[NG][2][4];
+  double acc2 = 0.0;
+  #pragma unroll
+  for (int i = 0; i < NG; ++i)
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = (w + 8 * i) * 32 + h * 16 + cl;
+      keep_apart();
+      #pragma unroll
+      for (int b = 0; b < 4; ++b)
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = b * 16 + g * 4 + e;
+          float v = 0.f;
+          if (inside(r, c)) {
+            const long at = place(r, c);
+            v = (float)((const T*)in.grad)[at] * in.gscale;
+            if (in.mom) {
+              const float mo = in.mu * in.mom[at] + v;
+              in.mom[at] = mo;
+              v = in.nesterov ? v + in.mu * mo : mo;
+            }
+          }
+          u[i][h][b][e] = v;
+          acc2 += (double)v * (double)v;
+        }
+    }
+  for (int off = 32; off > 0; off >>= 1) acc2 += __shfl_xor(acc2, off);
+  if (lane == 0) red[w] = acc2;
+  // C starts as the identity
+  for (int i = threadIdx.x; i < 64 * 64 / 4; i += 512) {
+    const int c = i >> 4, r = (i & 15) * 4;
+    f32x4 v = {};
+    #pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = r + e == c ? 1.f : 0.f;
+    put4(imgC, c, r >> 4, (r >> 2) & 3, v);
+  }
+  __syncthreads();
+  double total = 0.0;
+  for (int i = 0; i < 8; ++i) total += red[i];
+  const float f0 = 1.f / ((float)sqrt(total) + eps);
+  const float sx = steps.st[0].sx;
+  Halves x[NG][2][2];  // [group][16 columns][32 rows]
+  #pragma unroll
+  for (int i = 0; i < NG; ++i)
+    #pragma unroll
+    for (int h = 0; h < 2; ++h)
+      #pragma unroll
+      for (int f = 0; f < 2; ++f)
+        x[i][h][f] = halves(u[i][h][2 * f] * f0, u[i][h][2 * f + 1] * f0, sx);
+
+  // C X of a group's columns
+  auto apply = [&](const Halves (&xi)[2][2], f32x4 (&d)[2][4]) {
+    #pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      keep_apart();
+      #pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const Halves c = get(imgC, b * 16 + cl, f, g);
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) mma3(d[h][b], c, xi[h][f]);
+      }
+    }
+  };
+  for (int s = 0; s < steps.n; ++s) {
+    const NsStep& k = steps.st[s];
+    // X <- C X, its scale from the last step's sc * sx to sx (the identity's
+    // is one), and A = X X^T of it
+    float scale = 1.f;
+    if (s > 0) {
+      const NsStep& last = steps.st[s - 1];
+      scale = last.sn / (last.sc * last.sx);
+    }
+    f32x4 gram[4][4];
+    #pragma unroll
+    for (int a = 0; a < 4; ++a)
+      #pragma unroll
+      for (int b = 0; b <= a; ++b) gram[a][b] = f32x4{};
+    #pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      if (w + 8 * i >= groups) continue;
+      Halves q[4];  // rows of X', 32 columns
+      #pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        keep_apart();
+        f32x4 d[2] = {};
+        #pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const Halves c = get(imgC, b * 16 + cl, f, g);
+          #pragma unroll
+          for (int h = 0; h < 2; ++h) mma3(d[h], x[i][h][f], c);
+        }
+        q[b] = halves(d[0], d[1], scale);
+      }
+      #pragma unroll
+      for (int a = 0; a < 4; ++a)
+        #pragma unroll
+        for (int b = 0; b <= a; ++b) mma3(gram[a][b], q[a], q[b]);
+      if (s > 0) {
+        f32x4 d[2][4] = {};
+        apply(x[i], d);
+        #pragma unroll
+        for (int h = 0; h < 2; ++h)
+          #pragma unroll
+          for (int f = 0; f < 2; ++f)
+            x[i][h][f] = halves(d[h][2 * f], d[h][2 * f + 1], scale);
+      }
+    }
+    #pragma unroll
+    for (int a = 0; a < 4; ++a)
+      #pragma unroll
+      for (int b = 0; b <= a; ++b)
+        parts[(w * kNsTri + a * (a + 1) / 2 + b) * 64 + lane] = gram[a][b];
+    __syncthreads();
+    // the waves' sums in their order; waves 8 and 9 of the ten blocks' are
+    // taken by the first two again
+    for (int t = w; t < kNsTri; t += 8) {
+      f32x4 v = {};
+      const int used = min(groups, 8);
+      for (int i = 0; i < used; ++i) v += parts[(i * kNsTri + t) * 64 + lane];
+      int a = 0;
+      while ((a + 1) * (a + 2) / 2 <= t) ++a;
+      const int b = t - a * (a + 1) / 2;
+      v *= k.sa / (k.sx * k.sx);
+      // v: rows 16 a + 4 g + e of column 16 b + cl
+      put4(imgA, b * 16 + cl, a, g, v);
+      if (a != b) {
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f16 hi, lo;
+          split(v[e], hi, lo);
+          const int at = (b & 1) * 8 + (cl & 3) * 2;
+          const int row = a * 16 + g * 4 + e;
+          *(f16*)(imgA + piece(row, b >> 1, 0, cl >> 2) + at) = hi;
+          *(f16*)(imgA + piece(row, b >> 1, 1, cl >> 2) + at) = lo;
+        }
+      }
+    }
+    __syncthreads();
+    const float alpha = k.c * k.sc / (k.sa * k.sa), beta = k.b * k.sc / k.sa;
+    const int a = w >> 1;
+    #pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int b = (w & 1) * 2 + j;
+      f32x4 d = {};
+      #pragma unroll
+      for (int f = 0; f < 2; ++f)
+        mma3(d, get(imgA, a * 16 + cl, f, g), get(imgA, b * 16 + cl, f, g));
+      const f16x4 hi =
+          *(const f16x4*)(imgA + piece(b * 16 + cl, a >> 1, 0, g) + (a & 1) * 8);
+      const f16x4 lo =
+          *(const f16x4*)(imgA + piece(b * 16 + cl, a >> 1, 1, g) + (a & 1) * 8);
+      #pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d[e] = d[e] * alpha + beta * ((float)hi[e] + (float)lo[e]);
+        if (a == b && g * 4 + e == cl) d[e] += k.a * k.sc;
+      }
+      put4(imgC, b * 16 + cl, a, g, d);
+    }
+    __syncthreads();
+  }
+
+  // the last X' = C X goes out
+  const NsStep& last = steps.st[steps.n - 1];
+  const float scale = 1.f / (last.sc * last.sx), step = out.lr * m.gain;
+  #pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    if (w + 8 * i >= groups) continue;
+    f32x4 d[2][4] = {};
+    apply(x[i], d);
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = (w + 8 * i) * 32 + h * 16 + cl;
+      #pragma unroll
+      for (int b = 0; b < 4; ++b)
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = b * 16 + g * 4 + e;
+          if (!inside(r, c)) continue;
+          const long at = place(r, c);
+          const float o = d[h][b][e] * scale;
+          if (out.master) {
+            const float v = out.master[at] * out.keep - step * o;
+            out.master[at] = v;
+            ((bf16*)out.mirror)[at] = (bf16)v;
+          } else {
+            ((T*)out.out)[at] = (T)o;
+          }
+        }
+    }
+  }
+}
+
+template <typename T, int NG>
+void run_small(const NsGroup& g, const NsInput& in, const NsSmallSteps& st,
+               float eps, const NsOutput& out, hipStream_t s) {
+  hipLaunchKernelGGL((ns_small_kernel<T, NG>), dim3(g.count), dim3(512),
+                     kNsSmallLds, s, g, in, st, eps, out);
+}
+
+template <typename T>
+void pick_small(const NsGroup& g, int longest, const NsInput& in,
+                const NsSmallSteps& st, float eps, const NsOutput& out,
+                hipStream_t s) {
+  if (longest <= 256) run_small<T, 1>(g, in, st, eps, out, s);
+  else if (longest <= 512) run_small<T, 2>(g, in, st, eps, out, s);
+  else run_small<T, 4>(g, in, st, eps, out, s);
+}
+
 // both tile sizes' staging buffers take 64 KiB; 128's squares need 4 KiB more
 constexpr int kNsLds = 4 * 64 * (64 + 4) * 4;
 
@@ -601,6 +926,18 @@ void run(const NsGroup& g, const NsInput& in, const NsStep* st, int n,
 }
 
 }  // namespace
+
+void launch_newton_schulz_small(const NsGroup& g, int longest, int dtype,
+                                const NsInput& in, const NsStep* st, int n,
+                                float eps, const NsOutput& out,
+                                hipStream_t s) {
+  NsSmallSteps all{};
+  all.n = n;
+  for (int i = 0; i < n; ++i) all.st[i] = st[i];
+  if (dtype == 0) pick_small<bf16>(g, longest, in, all, eps, out, s);
+  else if (dtype == 1) pick_small<f16>(g, longest, in, all, eps, out, s);
+  else pick_small<float>(g, longest, in, all, eps, out, s);
+}
 
 void launch_newton_schulz(const NsGroup& g, int dtype, const NsInput& in,
                           const NsStep* st, int n, float eps,

@@ -87,6 +87,11 @@ inline int64_t ns_blocks(const NsMat& m, int kind) {
   return k.whole + (ns_tiles(m, kind) - k.whole) * k.splits;
 }
 
+// A matrix that one block holds in its registers; see ns_small_kernel.
+inline bool ns_fits_block(const NsMat& m) {
+  return std::min(m.rows, m.cols) <= 64 && std::max(m.rows, m.cols) <= 1024;
+}
+
 // Shapes, tiles and sharing of `copies` of each of the matrices.
 inline std::vector<NsMat> ns_plan(
     const std::vector<std::pair<int64_t, int64_t>>& sides, int64_t copies) {
@@ -111,20 +116,25 @@ inline std::vector<NsMat> ns_plan(
     for (NsMat& m : mats) {
       const int64_t tiles = ns_tiles(m, kind), depth = ns_depth(m, kind);
       // s blocks take depth / s steps each and the last of them s additions
-      // of a tile; a step costs about as much as 2 additions (64) or one
+      // of a tile; a step costs about as much as 2 additions (64) or one. A
+      // part below 12 or 16 steps costs more to hand over than it saves: 256 x
+      // 3136 took 232 us with any depth split, 150 us so, 154 us from 16 or 32
+      // steps on; the ResNet-50's matrices 1486, 1436 and 1435 us.
+      const bool small = m.tile == 64;
       const int64_t most = std::max<int64_t>(
-          1, (int64_t)std::sqrt((double)depth * (m.tile == 64 ? 2 : 1)));
+          1, std::min((int64_t)std::sqrt((double)depth * (small ? 2 : 1)),
+                      depth / (small ? 12 : 16)));
       NsTiles& k = m.kind[kind];
       k.whole = (int)tiles;
       k.splits = 1;
       if (all < kNsSlots) {
-        const int64_t s = std::min({kNsSlots / all, most, depth});
+        const int64_t s = std::min(kNsSlots / all, most);
         if (s > 1) k.whole = 0, k.splits = (int)s;
       } else if (mats.size() * copies == 1) {
         // what full rounds of the chip leave over
         const int64_t rest = all % kNsSlots;
         const int64_t s =
-            rest ? std::min({kNsSlots / rest, most, depth}) : 1;
+            rest ? std::min(kNsSlots / rest, most) : 1;
         if (s > 1 && all < 4 * kNsSlots)
           k.whole = (int)(tiles - rest), k.splits = (int)s;
       }

@@ -61,7 +61,9 @@ def _matrix(shape, dtype=torch.float32, device="cpu", seed=0, scale=1e-3):
 
 
 SHAPES = [(1, 1), (1, 5), (7, 1), (2, 3), (8, 8), (16, 40), (63, 65), (64, 64),
-          (65, 63), (100, 300), (300, 100), (129, 257), (33, 1000), (512, 24)]
+          (65, 63), (100, 300), (300, 100), (129, 257), (33, 1000), (512, 24),
+          (64, 256), (64, 257), (40, 513), (64, 1024), (1024, 50), (64, 1025),
+          (1025, 3)]
 
 
 @pytest.mark.parametrize("m,n", SHAPES)
@@ -78,7 +80,7 @@ def test_orthogonalize(device, dtype, m, n):
 
 # both tile sizes, whole tiles and ragged ones, wide and tall, batches
 BIG = [(640, 1500), (1500, 640), (1100, 1130), (2050, 2100), (3, 128, 384),
-       (2, 4, 90, 70), (64, 130, 260), (70, 257, 129), (256, 96, 30)]
+       (2, 4, 90, 70), (64, 130, 260), (70, 257, 129), (256, 96, 30), (300, 20, 700)]
 
 
 @pytest.mark.gpu
@@ -109,6 +111,12 @@ def test_coefficients_of_each_step(device):
     _check(o, g, coeffs=coeffs, eps=1e-8)
     one = F.orthogonalize(g, steps=1, coeffs=[CUBIC])
     _check(one, g, coeffs=[CUBIC])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_more_steps_than_one_block_takes(device):
+    g = _matrix((20, 30), device=device)
+    _check(F.orthogonalize(g, steps=40, coeffs=CUBIC), g, coeffs=(CUBIC,) * 40)
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -266,6 +274,7 @@ def _muon_reference(views, st, lr, mu, wd, gscale, nesterov, coeffs, eps):
 
 MODELS = {
     "one": [(64, 800)],
+    "small": [(32, 25), (64, 300), (40, 64), (10, 64), (900, 17)],
     "textcnn": [(128, 384), (128, 512), (128, 640), (8, 384)],
     "mixed": [(1, 1), (3, 50), (200, 31), (64, 64), (65, 129), (1, 77),
               (90, 1)],
