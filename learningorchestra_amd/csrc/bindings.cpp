@@ -865,12 +865,15 @@ void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
   auto mats = lo::ns_plan({{rows, cols}}, g.size(0));
   const lo::NsInput in{g.data_ptr(), nullptr, 1.f, 0.f, 0};
   const lo::NsOutput o{out.data_ptr(), nullptr, nullptr, 0.f, 0.f};
-  if (lo::ns_fits_block(mats[0]) && (int)st.size() <= lo::kNsSmallSteps) {
+  const int shortest = (int)std::min(rows, cols);
+  const int longest = (int)std::max(rows, cols);
+  if (lo::ns_fit_block(shortest, longest) &&
+      (int)st.size() <= lo::kNsSmallSteps) {
     lo::NsGroup ng{};
     ng.one = mats[0];
     ng.src_step = rows * cols;
     ng.count = (int)g.size(0);
-    lo::launch_newton_schulz_small(ng, (int)std::max(rows, cols), code, in,
+    lo::launch_newton_schulz_small(ng, shortest, longest, code, in,
                                    st.data(), (int)st.size(), (float)eps, o,
                                    stream());
     check_launch("orthogonalize");
@@ -921,7 +924,7 @@ struct MuonPlan {
   at::Tensor table, ws, sums, parts, slots;
   lo::NsGroup g{};
   int64_t numel;
-  int longest = 0;  // side, where all matrices fit a block
+  int shortest = 0, longest = 0;  // the largest short and long sides
 
   MuonPlan(std::vector<std::array<int64_t, 3>> views, int64_t numel_,
            at::Device device)
@@ -946,12 +949,10 @@ struct MuonPlan {
     lo::NsNeeds n;
     lo::ns_place(mats, n);
     for (size_t i = 0; i < mats.size(); ++i) mats[i].src = views[i][0];
-    bool fit = true;
     for (const lo::NsMat& m : mats) {
-      fit = fit && lo::ns_fits_block(m);
-      longest = std::max({longest, m.rows, m.cols});
+      shortest = std::max(shortest, std::min(m.rows, m.cols));
+      longest = std::max(longest, std::max(m.rows, m.cols));
     }
-    if (!fit) longest = 0;
     // a block list for each pass; the products' longest sums first, so that
     // none of those starts last
     std::vector<lo::NsBlock> lists[2 + lo::NS_KINDS];
@@ -1031,8 +1032,9 @@ struct MuonPlan {
     const lo::NsOutput out{nullptr, master.data_ptr<float>(),
                            mirror.data_ptr(), (float)lr,
                            (float)(1.0 - lr * wd)};
-    if (longest && (int)st.size() <= lo::kNsSmallSteps)
-      lo::launch_newton_schulz_small(g, longest, 2, in, st.data(),
+    if (lo::ns_fit_block(shortest, longest) &&
+        (int)st.size() <= lo::kNsSmallSteps)
+      lo::launch_newton_schulz_small(g, shortest, longest, 2, in, st.data(),
                                      (int)st.size(), (float)eps, out, stream());
     else
       lo::launch_newton_schulz(g, 2, in, st.data(), (int)st.size(), (float)eps,

@@ -79,11 +79,13 @@ struct NsStep {
 
 constexpr int kNsSmallSteps = 32;  // of one ns_small_kernel
 
-// all of the group's matrices fit a block (ns_fits_block), `longest` being
-// their longest side; n <= kNsSmallSteps
-void launch_newton_schulz_small(const NsGroup& g, int longest, int dtype,
-                                const NsInput& in, const NsStep* st, int n,
-                                float eps, const NsOutput& out, hipStream_t s);
+// all of the group's matrices fit a block (ns_fit_block): `shortest` and
+// `longest` are the largest of their short and of their long sides;
+// n <= kNsSmallSteps
+void launch_newton_schulz_small(const NsGroup& g, int shortest, int longest,
+                                int dtype, const NsInput& in, const NsStep* st,
+                                int n, float eps, const NsOutput& out,
+                                hipStream_t s);
 
 void launch_newton_schulz(const NsGroup& g, int dtype, const NsInput& in,
                           const NsStep* st, int n, float eps,

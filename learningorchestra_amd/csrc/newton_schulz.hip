@@ -28,6 +28,8 @@
 // adds the parts, in their order, so that results do not depend on timing. No
 // block waits for another.
 
+#include <type_traits>
+
 #include "lo_common.h"
 #include "newton_schulz.h"
 
@@ -570,7 +572,7 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(NsGroup g,
 }
 
 // ------------------------------------------- matrices that fit one block ----
-// Up to 64 rows and 1024 columns: one block does the whole call, momentum and
+// Up to 64 x 1024 or 32 x 2048: one block does the whole call, momentum and
 // norm included, with X in the registers of its eight waves.
 //
 // A wave owns groups of 32 columns. A lane's share of X serves as it is as an
@@ -581,40 +583,22 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(NsGroup g,
 // 32 f + 16 + 4 g + (0..3); C is laid out in that order in LDS. Its transpose,
 // from the same operands swapped, is in the same way ready for X' X'^T. The
 // waves' shares of A meet in LDS, where C is made from it.
-//
-// A step of 64 x 800 takes 26 groups * 126 matrix instructions on one CU; the
-// other 255 are free for the rest of a batch.
 struct NsSmallSteps {
   NsStep st[kNsSmallSteps];
   int n;
 };
-
-// byte offset of the 16-byte piece (row, f, half, g) of a 64 x 64 image; the
-// exclusive or spreads a column of pieces over the banks
-LO_DEVICE int piece(int row, int f, int half, int g) {
-  return row * 256 + (((f * 8 + half * 4 + g) ^ (row & 15)) << 4);
-}
-
-// rows 16 b + 4 g + (0..3) of column c, four values, into row c of an image of
-// a symmetric matrix
-LO_DEVICE void put4(char* img, int c, int b, int g, const f32x4& v) {
-  f16x4 hi, lo;
-  #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    f16 h, l;
-    split(v[e], h, l);
-    hi[e] = h;
-    lo[e] = l;
-  }
-  *(f16x4*)(img + piece(c, b >> 1, 0, g) + (b & 1) * 8) = hi;
-  *(f16x4*)(img + piece(c, b >> 1, 1, g) + (b & 1) * 8) = lo;
-}
 
 // eight values as packed halves (kept as words: a vector of f16 that lives
 // across a loop is given a register an element)
 struct Halves {
   u32x4 hi, lo;
 };
+
+// scale is a power of two, so either is one rounding of v * scale
+LO_DEVICE void split_scaled(float v, float scale, f16& hi, f16& lo) {
+  hi = (f16)__builtin_fmaf(v, scale, 0.f);
+  lo = (f16)__builtin_fmaf(v, scale, -(float)hi);
+}
 
 LO_DEVICE Halves halves(const f32x4& a, const f32x4& b, float scale) {
   Halves h;
@@ -625,7 +609,7 @@ LO_DEVICE Halves halves(const f32x4& a, const f32x4& b, float scale) {
     for (int e = 0; e < 2; ++e) {
       const int i = (j & 1) * 2 + e;
       f16 vh, vl;
-      split((j < 2 ? a[i] : b[i]) * scale, vh, vl);
+      split_scaled(j < 2 ? a[i] : b[i], scale, vh, vl);
       hi[e] = vh;
       lo[e] = vl;
     }
@@ -647,28 +631,69 @@ LO_DEVICE void mma3(f32x4& acc, const Halves& p, const Halves& q) {
   acc = mma(p.hi, q.hi, acc);
 }
 
-// keeps what is read from LDS or computed for an address on its side: a group
-// of columns re-reads C rather than hold all of it in registers
+// a square image of 16 MB rows in LDS; its 16-byte pieces hold eight values in
+// the sum's order, and an exclusive or spreads a column of them over the banks
+template <int MB>
+struct Image {
+  static constexpr int UNITS = MB * 4;  // pieces a row
+  static constexpr int BYTES = MB * 16 * UNITS * 16;
+  char* p;
+  LO_DEVICE char* piece(int row, int f, int half, int g) const {
+    return p + row * UNITS * 16 +
+           (((f * 8 + half * 4 + g) ^ (row & (UNITS - 1))) << 4);
+  }
+  LO_DEVICE Halves get(int row, int f, int g) const {
+    return {*(const u32x4*)piece(row, f, 0, g),
+            *(const u32x4*)piece(row, f, 1, g)};
+  }
+  // rows 16 b + 4 g + (0..3) of column c, as row c of the symmetric matrix
+  LO_DEVICE void put4(int c, int b, int g, const f32x4& v) const {
+    f16x4 hi, lo;
+    #pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f16 h, l;
+      split(v[e], h, l);
+      hi[e] = h;
+      lo[e] = l;
+    }
+    *(f16x4*)(piece(c, b >> 1, 0, g) + (b & 1) * 8) = hi;
+    *(f16x4*)(piece(c, b >> 1, 1, g) + (b & 1) * 8) = lo;
+  }
+  LO_DEVICE void get4(int c, int b, int g, f32x4& v) const {
+    const f16x4 hi = *(const f16x4*)(piece(c, b >> 1, 0, g) + (b & 1) * 8);
+    const f16x4 lo = *(const f16x4*)(piece(c, b >> 1, 1, g) + (b & 1) * 8);
+    #pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)hi[e] + (float)lo[e];
+  }
+  LO_DEVICE void put1(int row, int k, float v) const {
+    f16 hi, lo;
+    split(v, hi, lo);
+    const int b = k >> 4, g = (k >> 2) & 3;
+    const int at = (b & 1) * 8 + (k & 3) * 2;
+    *(f16*)(piece(row, b >> 1, 0, g) + at) = hi;
+    *(f16*)(piece(row, b >> 1, 1, g) + at) = lo;
+  }
+};
+
+// keeps what is read from LDS on its side: a group of columns re-reads C
+// rather than hold all of it in registers
 LO_DEVICE void keep_apart() { asm volatile("" ::: "memory"); }
 
-LO_DEVICE Halves get(const char* img, int row, int f, int g) {
-  return {*(const u32x4*)(img + piece(row, f, 0, g)),
-          *(const u32x4*)(img + piece(row, f, 1, g))};
+template <int MB>
+constexpr int ns_small_lds() {
+  return 2 * Image<MB>::BYTES + 8 * (MB * (MB + 1) / 2) * 1024;
 }
 
-constexpr int kNsTri = 10;  // 16 x 16 blocks of a 64 x 64 lower triangle
-constexpr int kNsSmallLds = 2 * 64 * 256 + 8 * kNsTri * 1024;
-
-// NG groups of 32 columns a wave
-template <typename T, int NG>
+// 16 MB rows, NG groups of 32 columns a wave
+template <typename T, int MB, int NG>
 __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in,
                                                           NsSmallSteps steps,
                                                           float eps,
                                                           NsOutput out) {
+  constexpr int FB = MB / 2, TRI = MB * (MB + 1) / 2;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  char* imgA = lds;
-  char* imgC = lds + 64 * 256;
-  f32x4* parts = (f32x4*)(lds + 2 * 64 * 256);  // [8][kNsTri][64]
+  const Image<MB> imgA{lds}, imgC{lds + Image<MB>::BYTES};
+  f32x4* parts = (f32x4*)(lds + 2 * Image<MB>::BYTES);  // [8][TRI][64]
   __shared__ double red[8];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int g = lane >> 4, cl = lane & 15;
@@ -678,76 +703,97 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
   const int short_ = min(m.rows, m.cols), long_ = max(m.rows, m.cols);
   const int groups = (long_ + 31) / 32;
 
-  // element (r, c) of X and its place in the input
-  auto inside = [&](int r, int c) { return r < short_ && c < long_; };
+  // Rows r..r+3 of column c of X lie together in a tall input, a row apart in
+  // a wide one. Places outside the matrix read its first element and count as
+  // zero, which keeps the loads free of branches.
+  const long stride_r = tall ? 1 : m.cols, stride_c = tall ? m.cols : 1;
   auto place = [&](int r, int c) {
-    return m.src + (tall ? (long)c * m.cols + r : (long)r * m.cols + c);
+    const bool ok = r < short_ && c < long_;
+    return m.src + (ok ? r * stride_r + c * stride_c : 0);
+  };
+  auto inside = [&](int r, int c) { return r < short_ && c < long_; };
+  // four at once where all four are there and lie together
+  auto read4 = [&](const auto* p, int r, int c) {
+    f32x4 v;
+    if (tall && (short_ & 3) == 0) {
+      v = load4(p, place(r, c), 4);
+      if (!inside(r, c)) v = f32x4{};
+    } else {
+      #pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (float)p[place(r + e, c)];
+      #pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = inside(r + e, c) ? v[e] : 0.f;
+    }
+    return v;
+  };
+  auto write4 = [&](auto* p, int r, int c, const f32x4& v) {
+    typedef std::remove_reference_t<decltype(*p)> P;
+    if (tall && (short_ & 3) == 0) {
+      if (inside(r, c)) store4(p, place(r, c), 4, v);
+    } else {
+      #pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (inside(r + e, c)) p[place(r + e, c)] = (P)v[e];
+    }
   };
 
-  f32x4 u[NG][2][4];
+  f32x4 u[NG][2][MB];
   double acc2 = 0.0;
   #pragma unroll
-  for (int i = 0; i < NG; ++i)
+  for (int i = 0; i < NG; ++i) {
+    #pragma unroll
+    for (int h = 0; h < 2; ++h)
+      #pragma unroll
+      for (int b = 0; b < MB; ++b) u[i][h][b] = f32x4{};
+    if (w + 8 * i >= groups) continue;
     #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = (w + 8 * i) * 32 + h * 16 + cl;
-      keep_apart();
       #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < MB; ++b)
+        u[i][h][b] = read4((const T*)in.grad, b * 16 + g * 4, c) * in.gscale;
+      if (in.mom) {
+        f32x4 mo[MB];
         #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = b * 16 + g * 4 + e;
-          float v = 0.f;
-          if (inside(r, c)) {
-            const long at = place(r, c);
-            v = (float)((const T*)in.grad)[at] * in.gscale;
-            if (in.mom) {
-              const float mo = in.mu * in.mom[at] + v;
-              in.mom[at] = mo;
-              v = in.nesterov ? v + in.mu * mo : mo;
-            }
-          }
-          u[i][h][b][e] = v;
-          acc2 += (double)v * (double)v;
+        for (int b = 0; b < MB; ++b) mo[b] = read4(in.mom, b * 16 + g * 4, c);
+        #pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          mo[b] = in.mu * mo[b] + u[i][h][b];
+          write4(in.mom, b * 16 + g * 4, c, mo[b]);
+          u[i][h][b] = in.nesterov ? u[i][h][b] + in.mu * mo[b] : mo[b];
         }
+      }
+      #pragma unroll
+      for (int b = 0; b < MB; ++b)
+        #pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc2 += (double)u[i][h][b][e] * (double)u[i][h][b][e];
     }
+  }
   for (int off = 32; off > 0; off >>= 1) acc2 += __shfl_xor(acc2, off);
   if (lane == 0) red[w] = acc2;
   // C starts as the identity
-  for (int i = threadIdx.x; i < 64 * 64 / 4; i += 512) {
-    const int c = i >> 4, r = (i & 15) * 4;
-    f32x4 v = {};
+  for (int i = threadIdx.x; i < 16 * MB * 4 * MB; i += 512) {
+    const int c = i / (4 * MB), r = i % (4 * MB) * 4;
+    f32x4 v;
     #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = r + e == c ? 1.f : 0.f;
-    put4(imgC, c, r >> 4, (r >> 2) & 3, v);
+    imgC.put4(c, r >> 4, (r >> 2) & 3, v);
   }
   __syncthreads();
   double total = 0.0;
   for (int i = 0; i < 8; ++i) total += red[i];
   const float f0 = 1.f / ((float)sqrt(total) + eps);
   const float sx = steps.st[0].sx;
-  Halves x[NG][2][2];  // [group][16 columns][32 rows]
+  Halves x[NG][2][FB];  // [group][16 columns][32 rows]
   #pragma unroll
   for (int i = 0; i < NG; ++i)
     #pragma unroll
     for (int h = 0; h < 2; ++h)
       #pragma unroll
-      for (int f = 0; f < 2; ++f)
+      for (int f = 0; f < FB; ++f)
         x[i][h][f] = halves(u[i][h][2 * f] * f0, u[i][h][2 * f + 1] * f0, sx);
 
-  // C X of a group's columns
-  auto apply = [&](const Halves (&xi)[2][2], f32x4 (&d)[2][4]) {
-    #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      keep_apart();
-      #pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const Halves c = get(imgC, b * 16 + cl, f, g);
-        #pragma unroll
-        for (int h = 0; h < 2; ++h) mma3(d[h][b], c, xi[h][f]);
-      }
-    }
-  };
   for (int s = 0; s < steps.n; ++s) {
     const NsStep& k = steps.st[s];
     // X <- C X, its scale from the last step's sc * sx to sx (the identity's
@@ -757,91 +803,82 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
       const NsStep& last = steps.st[s - 1];
       scale = last.sn / (last.sc * last.sx);
     }
-    f32x4 gram[4][4];
+    f32x4 gram[MB][MB];
     #pragma unroll
-    for (int a = 0; a < 4; ++a)
+    for (int a = 0; a < MB; ++a)
       #pragma unroll
       for (int b = 0; b <= a; ++b) gram[a][b] = f32x4{};
     #pragma unroll
     for (int i = 0; i < NG; ++i) {
       if (w + 8 * i >= groups) continue;
-      Halves q[4];  // rows of X', 32 columns
+      Halves q[MB];  // rows of X', 32 columns
+      f32x4 d[2][MB];
       #pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < MB; ++b) {
         keep_apart();
-        f32x4 d[2] = {};
+        f32x4 t[2] = {};
+        d[0][b] = d[1][b] = f32x4{};
         #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const Halves c = get(imgC, b * 16 + cl, f, g);
+        for (int f = 0; f < FB; ++f) {
+          const Halves c = imgC.get(b * 16 + cl, f, g);
           #pragma unroll
-          for (int h = 0; h < 2; ++h) mma3(d[h], x[i][h][f], c);
+          for (int h = 0; h < 2; ++h) {
+            mma3(t[h], x[i][h][f], c);
+            mma3(d[h][b], c, x[i][h][f]);
+          }
         }
-        q[b] = halves(d[0], d[1], scale);
+        q[b] = halves(t[0], t[1], scale);
       }
       #pragma unroll
-      for (int a = 0; a < 4; ++a)
+      for (int a = 0; a < MB; ++a)
         #pragma unroll
         for (int b = 0; b <= a; ++b) mma3(gram[a][b], q[a], q[b]);
-      if (s > 0) {
-        f32x4 d[2][4] = {};
-        apply(x[i], d);
+      #pragma unroll
+      for (int h = 0; h < 2; ++h)
         #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          #pragma unroll
-          for (int f = 0; f < 2; ++f)
-            x[i][h][f] = halves(d[h][2 * f], d[h][2 * f + 1], scale);
-      }
+        for (int f = 0; f < FB; ++f)
+          x[i][h][f] = halves(d[h][2 * f], d[h][2 * f + 1], scale);
     }
     #pragma unroll
-    for (int a = 0; a < 4; ++a)
+    for (int a = 0; a < MB; ++a)
       #pragma unroll
       for (int b = 0; b <= a; ++b)
-        parts[(w * kNsTri + a * (a + 1) / 2 + b) * 64 + lane] = gram[a][b];
+        parts[(w * TRI + a * (a + 1) / 2 + b) * 64 + lane] = gram[a][b];
     __syncthreads();
-    // the waves' sums in their order; waves 8 and 9 of the ten blocks' are
-    // taken by the first two again
-    for (int t = w; t < kNsTri; t += 8) {
+    // the waves' sums in their order
+    const int used = min(groups, 8);
+    for (int t = w; t < TRI; t += 8) {
       f32x4 v = {};
-      const int used = min(groups, 8);
-      for (int i = 0; i < used; ++i) v += parts[(i * kNsTri + t) * 64 + lane];
+      #pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < used) v += parts[(i * TRI + t) * 64 + lane];
       int a = 0;
       while ((a + 1) * (a + 2) / 2 <= t) ++a;
       const int b = t - a * (a + 1) / 2;
       v *= k.sa / (k.sx * k.sx);
       // v: rows 16 a + 4 g + e of column 16 b + cl
-      put4(imgA, b * 16 + cl, a, g, v);
+      imgA.put4(b * 16 + cl, a, g, v);
       if (a != b) {
         #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          f16 hi, lo;
-          split(v[e], hi, lo);
-          const int at = (b & 1) * 8 + (cl & 3) * 2;
-          const int row = a * 16 + g * 4 + e;
-          *(f16*)(imgA + piece(row, b >> 1, 0, cl >> 2) + at) = hi;
-          *(f16*)(imgA + piece(row, b >> 1, 1, cl >> 2) + at) = lo;
-        }
+        for (int e = 0; e < 4; ++e)
+          imgA.put1(a * 16 + g * 4 + e, b * 16 + cl, v[e]);
       }
     }
     __syncthreads();
     const float alpha = k.c * k.sc / (k.sa * k.sa), beta = k.b * k.sc / k.sa;
-    const int a = w >> 1;
-    #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int b = (w & 1) * 2 + j;
-      f32x4 d = {};
+    for (int t = w; t < MB * MB; t += 8) {
+      const int a = t / MB, b = t % MB;
+      f32x4 d = {}, av;
       #pragma unroll
-      for (int f = 0; f < 2; ++f)
-        mma3(d, get(imgA, a * 16 + cl, f, g), get(imgA, b * 16 + cl, f, g));
-      const f16x4 hi =
-          *(const f16x4*)(imgA + piece(b * 16 + cl, a >> 1, 0, g) + (a & 1) * 8);
-      const f16x4 lo =
-          *(const f16x4*)(imgA + piece(b * 16 + cl, a >> 1, 1, g) + (a & 1) * 8);
+      for (int f = 0; f < FB; ++f)
+        mma3(d, imgA.get(a * 16 + cl, f, g), imgA.get(b * 16 + cl, f, g));
+      imgA.get4(b * 16 + cl, a, g, av);
       #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        d[e] = d[e] * alpha + beta * ((float)hi[e] + (float)lo[e]);
+        d[e] = d[e] * alpha + beta * av[e];
         if (a == b && g * 4 + e == cl) d[e] += k.a * k.sc;
       }
-      put4(imgC, b * 16 + cl, a, g, d);
+      imgC.put4(b * 16 + cl, a, g, d);
     }
     __syncthreads();
   }
@@ -852,45 +889,63 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
   #pragma unroll
   for (int i = 0; i < NG; ++i) {
     if (w + 8 * i >= groups) continue;
-    f32x4 d[2][4] = {};
-    apply(x[i], d);
+    f32x4 d[2][MB] = {};
+    #pragma unroll
+    for (int b = 0; b < MB; ++b) {
+      keep_apart();
+      #pragma unroll
+      for (int f = 0; f < FB; ++f) {
+        const Halves c = imgC.get(b * 16 + cl, f, g);
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) mma3(d[h][b], c, x[i][h][f]);
+      }
+    }
     #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = (w + 8 * i) * 32 + h * 16 + cl;
-      #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      if (out.master) {
+        f32x4 v[MB];
         #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = b * 16 + g * 4 + e;
-          if (!inside(r, c)) continue;
-          const long at = place(r, c);
-          const float o = d[h][b][e] * scale;
-          if (out.master) {
-            const float v = out.master[at] * out.keep - step * o;
-            out.master[at] = v;
-            ((bf16*)out.mirror)[at] = (bf16)v;
-          } else {
-            ((T*)out.out)[at] = (T)o;
-          }
+        for (int b = 0; b < MB; ++b)
+          v[b] = read4(out.master, b * 16 + g * 4, c) * out.keep -
+                 d[h][b] * (scale * step);
+        #pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          write4(out.master, b * 16 + g * 4, c, v[b]);
+          write4((bf16*)out.mirror, b * 16 + g * 4, c, v[b]);
         }
+      } else {
+        #pragma unroll
+        for (int b = 0; b < MB; ++b)
+          write4((T*)out.out, b * 16 + g * 4, c, d[h][b] * scale);
+      }
     }
   }
 }
 
-template <typename T, int NG>
+template <typename T, int MB, int NG>
 void run_small(const NsGroup& g, const NsInput& in, const NsSmallSteps& st,
                float eps, const NsOutput& out, hipStream_t s) {
-  hipLaunchKernelGGL((ns_small_kernel<T, NG>), dim3(g.count), dim3(512),
-                     kNsSmallLds, s, g, in, st, eps, out);
+  hipLaunchKernelGGL((ns_small_kernel<T, MB, NG>), dim3(g.count), dim3(512),
+                     ns_small_lds<MB>(), s, g, in, st, eps, out);
 }
 
 template <typename T>
-void pick_small(const NsGroup& g, int longest, const NsInput& in,
+void pick_small(const NsGroup& g, int shortest, int longest, const NsInput& in,
                 const NsSmallSteps& st, float eps, const NsOutput& out,
                 hipStream_t s) {
-  if (longest <= 256) run_small<T, 1>(g, in, st, eps, out, s);
-  else if (longest <= 512) run_small<T, 2>(g, in, st, eps, out, s);
-  else run_small<T, 4>(g, in, st, eps, out, s);
+  if (shortest <= 32) {
+    if (longest <= 256) run_small<T, 2, 1>(g, in, st, eps, out, s);
+    else if (longest <= 512) run_small<T, 2, 2>(g, in, st, eps, out, s);
+    else if (longest <= 1024) run_small<T, 2, 4>(g, in, st, eps, out, s);
+    else run_small<T, 2, 8>(g, in, st, eps, out, s);
+  } else if (longest <= 256) {
+    run_small<T, 4, 1>(g, in, st, eps, out, s);
+  } else if (longest <= 512) {
+    run_small<T, 4, 2>(g, in, st, eps, out, s);
+  } else {
+    run_small<T, 4, 4>(g, in, st, eps, out, s);
+  }
 }
 
 // both tile sizes' staging buffers take 64 KiB; 128's squares need 4 KiB more
@@ -927,16 +982,16 @@ void run(const NsGroup& g, const NsInput& in, const NsStep* st, int n,
 
 }  // namespace
 
-void launch_newton_schulz_small(const NsGroup& g, int longest, int dtype,
-                                const NsInput& in, const NsStep* st, int n,
-                                float eps, const NsOutput& out,
+void launch_newton_schulz_small(const NsGroup& g, int shortest, int longest,
+                                int dtype, const NsInput& in, const NsStep* st,
+                                int n, float eps, const NsOutput& out,
                                 hipStream_t s) {
   NsSmallSteps all{};
   all.n = n;
   for (int i = 0; i < n; ++i) all.st[i] = st[i];
-  if (dtype == 0) pick_small<bf16>(g, longest, in, all, eps, out, s);
-  else if (dtype == 1) pick_small<f16>(g, longest, in, all, eps, out, s);
-  else pick_small<float>(g, longest, in, all, eps, out, s);
+  if (dtype == 0) pick_small<bf16>(g, shortest, longest, in, all, eps, out, s);
+  else if (dtype == 1) pick_small<f16>(g, shortest, longest, in, all, eps, out, s);
+  else pick_small<float>(g, shortest, longest, in, all, eps, out, s);
 }
 
 void launch_newton_schulz(const NsGroup& g, int dtype, const NsInput& in,

@@ -87,9 +87,10 @@ inline int64_t ns_blocks(const NsMat& m, int kind) {
   return k.whole + (ns_tiles(m, kind) - k.whole) * k.splits;
 }
 
-// A matrix that one block holds in its registers; see ns_small_kernel.
-inline bool ns_fits_block(const NsMat& m) {
-  return std::min(m.rows, m.cols) <= 64 && std::max(m.rows, m.cols) <= 1024;
+// Whether one block's registers hold each matrix (see ns_small_kernel), given
+// the largest of their short and of their long sides
+inline bool ns_fit_block(int shortest, int longest) {
+  return shortest <= 32 ? longest <= 2048 : shortest <= 64 && longest <= 1024;
 }
 
 // Shapes, tiles and sharing of `copies` of each of the matrices.
