@@ -900,11 +900,9 @@ void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
   ng.sums = (double*)sums.data_ptr();
   ng.parts = (float*)parts.data_ptr();
   ng.slots = (unsigned*)slots.data_ptr();
-  for (int k = 0; k < lo::NS_KINDS; ++k) {
-    ng.kinds[k] = (int)n.kinds[k];
-    ng.slot_step[k] = (int)n.slots;
-    ng.part_step[k] = n.parts;
-  }
+  ng.slot_step = (int)n.slots;
+  ng.part_step = n.parts;
+  for (int k = 0; k < lo::NS_KINDS; ++k) ng.kinds[k] = (int)n.kinds[k];
   for (int64_t b0 = 0; b0 < g.size(0); b0 += group) {
     const int64_t count = std::min(group, g.size(0) - b0);
     ng.count = (int)count;
@@ -953,46 +951,34 @@ struct MuonPlan {
       shortest = std::max(shortest, std::min(m.rows, m.cols));
       longest = std::max(longest, std::max(m.rows, m.cols));
     }
-    // a block list for each pass; the products' longest sums first, so that
-    // none of those starts last
-    std::vector<lo::NsBlock> lists[2 + lo::NS_KINDS];
+    std::vector<lo::NsBlock> chunks, splits;
     for (int i = 0; i < (int)mats.size(); ++i) {
       const lo::NsMat& m = mats[i];
-      for (int at = 0; at < m.chunks; ++at) lists[0].push_back({i, at});
+      for (int at = 0; at < m.chunks; ++at) chunks.push_back({i, at});
       for (int at = 0; at < m.mp / 64 * (m.np / 64); ++at)
-        lists[1].push_back({i, at});
+        splits.push_back({i, at});
     }
-    for (int k = 0; k < lo::NS_KINDS; ++k) {
-      std::vector<int> order(mats.size());
-      for (int i = 0; i < (int)mats.size(); ++i) order[i] = i;
-      auto work = [&](int i) {
-        const lo::NsMat& m = mats[i];
-        return lo::ns_depth(m, k) * m.tile * m.tile / m.kind[k].splits;
-      };
-      std::stable_sort(order.begin(), order.end(),
-                       [&](int a, int b) { return work(a) > work(b); });
-      for (int i : order)
-        for (int at = 0; at < (int)lo::ns_blocks(mats[i], k); ++at)
-          lists[2 + k].push_back({i, at});
-    }
-    size_t bytes = mats.size() * sizeof(lo::NsMat);
-    for (const auto& l : lists) bytes += l.size() * sizeof(lo::NsBlock);
-    auto host = at::empty({(int64_t)bytes}, at::kByte);
-    table = at::empty({(int64_t)bytes}, at::TensorOptions(at::kByte).device(device));
-    auto *h = host.data_ptr<uint8_t>(), *d = table.data_ptr<uint8_t>();
-    size_t pos = mats.size() * sizeof(lo::NsMat);
-    std::memcpy(h, mats.data(), pos);
-    g.mats = (const lo::NsMat*)d;
-    const lo::NsBlock** to[] = {&g.chunk_blocks, &g.split_blocks,
-                                &g.kind_blocks[0], &g.kind_blocks[1],
-                                &g.kind_blocks[2]};
-    for (int i = 0; i < 2 + lo::NS_KINDS; ++i) {
-      const size_t b = lists[i].size() * sizeof(lo::NsBlock);
-      std::memcpy(h + pos, lists[i].data(), b);
-      *to[i] = (const lo::NsBlock*)(d + pos);
-      pos += b;
-    }
-    table.copy_(host);
+    // one table of them all, each part on a line of its own
+    std::vector<uint8_t> host;
+    auto put = [&](const auto& v) {
+      const size_t at = host.size(), bytes = v.size() * sizeof(v[0]);
+      host.resize(at + (bytes + 63) / 64 * 64);
+      std::memcpy(host.data() + at, v.data(), bytes);
+      return at;
+    };
+    const size_t at_mats = put(mats), at_chunks = put(chunks),
+                 at_splits = put(splits);
+    size_t at_tasks[lo::NS_KINDS];
+    for (int k = 0; k < lo::NS_KINDS; ++k) at_tasks[k] = put(lo::ns_tasks(mats, k));
+    table = at::empty({(int64_t)host.size()},
+                      at::TensorOptions(at::kByte).device(device));
+    table.copy_(at::from_blob(host.data(), {(int64_t)host.size()}, at::kByte));
+    auto* d = table.data_ptr<uint8_t>();
+    g.mats = (const lo::NsMat*)(d + at_mats);
+    g.chunk_blocks = (const lo::NsBlock*)(d + at_chunks);
+    g.split_blocks = (const lo::NsBlock*)(d + at_splits);
+    for (int k = 0; k < lo::NS_KINDS; ++k)
+      g.tasks[k] = (const lo::NsTask*)(d + at_tasks[k]);
     ws = at::empty({n.halfs * 2}, table.options());
     sums = at::empty({n.chunks * 8}, table.options());
     parts = at::empty({n.parts * 4}, table.options());

@@ -14,8 +14,6 @@ enum { NS_GRAM, NS_POLY, NS_APPLY, NS_KINDS };
 // the others `splits` blocks, each a part of the sum
 struct NsTiles {
   int whole, splits;
-  int slot;  // first split tile's counter
-  long part; // first split tile's partial sums (floats)
 };
 
 struct NsMat {
@@ -35,17 +33,29 @@ struct NsBlock {
   int mat, at;
 };
 
-// A group of matrices, by tables (mats; blocks of the momentum pass, of the
-// split and of the products) or, without them, count equal matrices spaced by
-// the steps.
+// all that a block of a product has to know: one 64-byte line
+struct alignas(64) NsTask {
+  long ws;    // the matrix's workspace
+  long part;  // a split tile's partial sums (floats)
+  int mat, tile, mp, np;
+  int ti, tj;  // tile row and column
+  int k0, k1;  // steps of 32 of the sum
+  int slice, splits;
+  int slot;  // a split tile's counter
+};
+
+// A group of matrices, by tables (mats; blocks of the momentum pass and of the
+// split; tasks of the products) or, without them, count equal matrices spaced
+// by the steps.
 struct NsGroup {
   const NsMat* mats;
-  const NsBlock *chunk_blocks, *split_blocks, *kind_blocks[NS_KINDS];
+  const NsBlock *chunk_blocks, *split_blocks;
+  const NsTask* tasks[NS_KINDS];
   int count;
   NsMat one;
-  long src_step, ws_step, part_step[NS_KINDS];
-  int sum_step, slot_step[NS_KINDS];
-  int chunks, splits, kinds[NS_KINDS];             // blocks of one of them
+  long src_step, ws_step, part_step;
+  int sum_step, slot_step;
+  int chunks, splits, kinds[NS_KINDS];               // blocks of one of them
   long all_chunks, all_splits, all_kinds[NS_KINDS];  // of the group
   void* ws;
   double* sums;

@@ -31,7 +31,7 @@
 #include <type_traits>
 
 #include "lo_common.h"
-#include "newton_schulz.h"
+#include "newton_schulz_plan.h"
 
 namespace lo {
 
@@ -91,11 +91,6 @@ LO_DEVICE NsMat find(const NsGroup& g, const NsBlock* __restrict__ table,
   m.src += i * g.src_step;
   m.ws += i * g.ws_step;
   m.sum += i * g.sum_step;
-  #pragma unroll
-  for (int k = 0; k < NS_KINDS; ++k) {
-    m.kind[k].slot += i * g.slot_step[k];
-    m.kind[k].part += i * g.part_step[k];
-  }
   return m;
 }
 
@@ -110,7 +105,8 @@ struct Planes {
   LO_DEVICE f16* c() const { return w + 4 * n + a_; }
 };
 
-LO_DEVICE Planes planes(const NsMat& m, void* ws) {
+template <typename M>  // NsMat or NsTask
+LO_DEVICE Planes planes(const M& m, void* ws) {
   return {(f16*)ws + m.ws, 2l * m.mp * m.np, 2l * m.mp * m.mp};
 }
 
@@ -255,75 +251,91 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup g, NsInput in,
   }
 }
 
-// Tile l of a product, in bands of eight tile rows, down a band's columns
-// first: 64 tiles in turn read 8 + 8 panels. KIND APPLY covers tm x tn tiles,
-// the symmetric ones the lower triangle of tm x tm.
-template <int KIND>
-LO_DEVICE void tile_at(int l, int tm, int tn, int& ti, int& tj) {
-  if (KIND == NS_APPLY) {
-    const int band = l / (8 * tn);
-    const int h = min(8, tm - 8 * band);
-    l -= band * 8 * tn;
-    tj = l / h;
-    ti = 8 * band + l - tj * h;
-    return;
-  }
-  // band b starts at tile 32 b (b - 1) + 36 b
-  int b = (int)sqrtf((float)l * (1.f / 32.f));
-  while (32 * b * (b - 1) + 36 * b > l) --b;
-  while (32 * b * (b + 1) + 36 * (b + 1) <= l) ++b;
-  l -= 32 * b * (b - 1) + 36 * b;
-  const int h = min(8, tm - 8 * b);
-  if (l < h * 8 * b) {
-    tj = l / h;
-    ti = 8 * b + l - tj * h;
-    return;
-  }
-  l -= h * 8 * b;
-  int r = 0;
-  while ((r + 1) * (r + 2) / 2 <= l) ++r;
-  ti = 8 * b + r;
-  tj = 8 * b + l - r * (r + 1) / 2;
-}
-
+// What a product's launch hands its blocks. The first lines are what each
+// block reads before it can start.
 struct NsProduct {
-  int from;                // the X and Y that the step reads
-  float alpha, beta, diag; // out = alpha * sum + beta * A (+ diag where i = j)
+  const NsTask* tasks;  // or null: equal matrices
+  void* ws;
+  int from;                 // the X and Y that the step reads
+  int mp, np, tile;         // equal matrices: their shape,
+  int blocks, whole, splits, count;  // blocks of one, and how shared out,
+  long ws_step, part_step;  // and their spacing
+  int slot_step;
+  float alpha, beta, diag;  // out = alpha * sum + beta * A (+ diag where i = j)
+  float* parts;
+  unsigned* slots;
 };
+
+// the last step's output
+struct NsFinal {
+  NsOutput out;
+  const NsMat* mats;
+  NsMat one;
+  long src_step;
+};
+
+template <int KIND>
+LO_DEVICE NsTask task_of(const NsProduct& pr) {
+  int id = blockIdx.x;
+  if (pr.tasks) return pr.tasks[id];
+  // neighbouring tiles on one die, for its cache (the split tiles of a single
+  // matrix are spread over all dies)
+  const int whole = pr.count == 1 ? pr.whole : (int)gridDim.x;
+  if (id < whole) id = xcd_swizzle(id, whole);
+  NsTask t;
+  t.mat = 0;
+  if (pr.count > 1) {
+    t.mat = id / pr.blocks;
+    id -= t.mat * pr.blocks;
+  }
+  t.ws = t.mat * pr.ws_step;
+  t.part = t.mat * pr.part_step;
+  t.slot = t.mat * pr.slot_step;
+  t.mp = pr.mp;
+  t.np = pr.np;
+  t.tile = pr.tile;
+  t.slice = 0;
+  t.splits = 1;
+  if (id >= pr.whole) {
+    t.splits = pr.splits;
+    const int cut = (id - pr.whole) / t.splits;
+    t.slice = id - pr.whole - cut * t.splits;
+    t.part += (long)cut * t.splits * t.tile * t.tile;
+    t.slot += cut;
+    id = pr.whole + cut;
+  }
+  const int shift = t.tile == 128 ? 7 : 6;
+  ns_tile_at(KIND, id, t.mp >> shift, t.np >> shift, t.ti, t.tj);
+  const int depth = (KIND == NS_GRAM ? t.np : t.mp) / 32;
+  t.k0 = 0;
+  t.k1 = depth;
+  if (t.splits > 1) {
+    t.k0 = depth * t.slice / t.splits;
+    t.k1 = depth * (t.slice + 1) / t.splits;
+  }
+  return t;
+}
 
 // One product on T x T tiles, four waves, S staged tiles of both operands (32
 // values of the sum each) in LDS. FINAL: the last step's X' goes to the output
 // in place of the workspace.
 template <int T, int KIND, int S, typename O, bool FINAL>
-LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
-                            const NsProduct& pr, const NsOutput& out,
-                            char* lds) {
+LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
+                            const NsFinal& fin, char* lds) {
   constexpr int W = T / 2;      // a wave's square
   constexpr int F = W / 16;     // its 16 x 16 fragments a side
   constexpr int IMG = T * 128;  // bytes of one operand's tile: T rows, 32 k
   constexpr int LOADS = T / 32; // a wave's loads of one operand's tile
-  const Planes pl = planes(m, g.ws);
-  const NsTiles& kd = m.kind[KIND];
-  int slice = 0, splits = 1, l = at, cut = -1;
-  if (at >= kd.whole) {
-    splits = kd.splits;
-    cut = (at - kd.whole) / splits;
-    slice = at - kd.whole - cut * splits;
-    l = kd.whole + cut;
-  }
-  int ti, tj;
-  tile_at<KIND>(l, m.mp / T, m.np / T, ti, tj);
-  const int ld = KIND == NS_GRAM ? m.np : m.mp;  // values a row of operands
-  const int nk = ld / 32;
-  const int k0 = nk * slice / splits, k1 = nk * (slice + 1) / splits;
+  const Planes pl = planes(t, pr.ws);
+  const int ti = t.ti, tj = t.tj, splits = t.splits, slice = t.slice;
+  const int k0 = t.k0, k1 = t.k1;
+  const int ld = KIND == NS_GRAM ? t.np : t.mp;  // values a row of operands
   const f16* P = KIND == NS_GRAM   ? pl.x(pr.from)
                  : KIND == NS_POLY ? pl.a()
                                    : pl.c();
   const f16* Q = KIND == NS_GRAM   ? pl.x(pr.from)
                  : KIND == NS_POLY ? pl.a()
                                    : pl.y(pr.from);
-  P += (long)ti * T * 2 * ld;
-  Q += (long)tj * T * 2 * ld;
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wr = wave >> 1, wc = wave & 1;
@@ -331,68 +343,109 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
   // 1 KiB (8 rows of 128 bytes) an instruction; the 16-byte piece that lands
   // at place p of a row is piece p ^ (row & 7), which spreads a column of
   // pieces over the banks
+  const long lane_off = (long)(wave * LOADS * 8 + lane / 8) * 2 * ld +
+                        ((lane % 8) ^ (lane / 8)) * 8;
+  P += (long)ti * T * 2 * ld + lane_off;
+  Q += (long)tj * T * 2 * ld + lane_off;
   auto stage = [&](int kt) {
-    char* buf = lds + (kt - k0) % S * 2 * IMG;
+    char* buf = lds + (kt - k0) % S * 2 * IMG + wave * LOADS * 1024;
     #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int seg = wave * LOADS + i;
-      const int row = seg * 8 + lane / 8;
-      const long off = (long)row * 2 * ld + kt * 64 + ((lane % 8) ^ (row & 7)) * 8;
+      const long off = (long)i * 16 * ld + kt * 64;
       __builtin_amdgcn_global_load_lds(
           (const __attribute__((address_space(1))) unsigned int*)(P + off),
-          (__attribute__((address_space(3))) unsigned int*)(buf + seg * 1024),
+          (__attribute__((address_space(3))) unsigned int*)(buf + i * 1024),
           16, 0, 0);
       __builtin_amdgcn_global_load_lds(
           (const __attribute__((address_space(1))) unsigned int*)(Q + off),
           (__attribute__((address_space(3))) unsigned int*)(buf + IMG +
-                                                            seg * 1024),
+                                                            i * 1024),
           16, 0, 0);
     }
+  };
+  struct Frags {
+    f16x8 ph[F], pw[F], qh[F], ql[F];
   };
   auto frag = [&](const char* img, int row, int half) {
     return *(const f16x8*)(img + row * 128 +
                            ((half * 64 + (lane >> 4) * 16) ^ ((row & 7) << 4)));
   };
-
+  auto read = [&](int kt, Frags& s) {
+    const char* img = lds + (kt - k0) % S * 2 * IMG;
+    #pragma unroll
+    for (int i = 0; i < F; ++i) {
+      const int row = i * 16 + (lane & 15);
+      s.ph[i] = frag(img, wr * W + row, 0);
+      s.qh[i] = frag(img + IMG, wc * W + row, 0);
+    }
+    #pragma unroll
+    for (int i = 0; i < F; ++i) {
+      const int row = i * 16 + (lane & 15);
+      s.ql[i] = frag(img + IMG, wc * W + row, 1);
+      s.pw[i] = frag(img, wr * W + row, 1);
+    }
+  };
   f32x4 acc[F][F] = {};
-  for (int kt = k0; kt < k0 + S - 1; ++kt)
-    if (kt < k1) stage(kt);
-  for (int kt = k0; kt < k1; ++kt) {
-    // tile kt has landed (the S - 2 after it may be on their way), and every
-    // wave is done with the buffer that the next one goes to
-    if (kt + S - 2 < k1)
+  // kind by kind: an accumulator's next use is F * F instructions away
+  auto products = [&](const f16x8 (&p)[F], const f16x8 (&q)[F]) {
+    #pragma unroll
+    for (int i = 0; i < F; ++i)
+      #pragma unroll
+      for (int j = 0; j < F; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[i], q[j],
+                                                           acc[i][j], 0, 0, 0);
+  };
+  auto add = [&](const Frags& s) {
+    products(s.ph, s.qh);
+    products(s.ph, s.ql);
+    products(s.pw, s.qh);
+  };
+
+  // A's part of C: A is symmetric, so its row c holds a lane's four values in
+  // a line. Small tiles fetch it while the sum is taken (large ones have no
+  // registers to spare, and more to do meanwhile).
+  constexpr bool EARLY = KIND == NS_POLY && T == 64;
+  f16x4 ah[EARLY ? F * F : 1], al[EARLY ? F * F : 1];
+  auto fetch = [&](int i, int j, f16x4& hi, f16x4& lo) {
+    const int r = ti * T + wr * W + i * 16 + (lane >> 4) * 4;
+    const int c = tj * T + wc * W + j * 16 + (lane & 15);
+    const f16* s = pl.a() + split_at(c, r, t.mp);
+    hi = *(const f16x4*)s;
+    lo = *(const f16x4*)(s + 32);
+  };
+  if constexpr (EARLY) {
+    #pragma unroll
+    for (int i = 0; i < F * F; ++i) fetch(i / F, i % F, ah[i], al[i]);
+  }
+
+  // The loop adds a tile's fragments while the next one's are read from LDS
+  // and S - 1 more are on their way. `ready` waits until tile kt has landed
+  // and every wave has read the one before, whose buffer is then free.
+  auto ready = [&](int kt, int newest) {
+    if (newest < k1)
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(
                        (S - 2) * 2 * LOADS)
                    : "memory");
     else
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const char* img = lds + (kt - k0) % S * 2 * IMG;
-    f16x8 ph[F], pw[F], qh[F], ql[F];
-    #pragma unroll
-    for (int i = 0; i < F; ++i) {
-      const int row = i * 16 + (lane & 15);
-      ph[i] = frag(img, wr * W + row, 0);
-      qh[i] = frag(img + IMG, wc * W + row, 0);
+  };
+  for (int kt = k0; kt < k0 + S - 1; ++kt)
+    if (kt < k1) stage(kt);
+  Frags a, b;
+  ready(k0, k0 + S - 2);
+  read(k0, a);
+  if (k0 + S - 1 < k1) stage(k0 + S - 1);
+  auto step = [&](int kt, const Frags& now, Frags& next) {
+    if (kt + 1 < k1) {
+      ready(kt + 1, kt + S - 1);
+      read(kt + 1, next);
+      if (kt + S < k1) stage(kt + S);
     }
-    #pragma unroll
-    for (int i = 0; i < F; ++i) {
-      const int row = i * 16 + (lane & 15);
-      pw[i] = frag(img, wr * W + row, 1);
-      ql[i] = frag(img + IMG, wc * W + row, 1);
-    }
-    if (kt + S - 1 < k1) stage(kt + S - 1);
-    // kind by kind: an accumulator's next use is F * F instructions away
-    auto products = [&](const f16x8 (&p)[F], const f16x8 (&q)[F]) {
-      #pragma unroll
-      for (int i = 0; i < F; ++i)
-        #pragma unroll
-        for (int j = 0; j < F; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[i], q[j],
-                                                             acc[i][j], 0, 0, 0);
-    };
-    products(ph, qh);
-    products(ph, ql);
-    products(pw, qh);
+    add(now);
+  };
+  for (int kt = k0; kt < k1; kt += 2) {
+    step(kt, a, b);
+    if (kt + 1 < k1) step(kt + 1, b, a);
   }
   __syncthreads();  // the staging buffers are free from here on
 
@@ -401,7 +454,7 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
     // stores), and have arrived there before the counter goes up: no cache
     // needs writing back. The last block drops what its die holds of others'.
     typedef unsigned long long u64;
-    u64* part = (u64*)(g.parts + kd.part + (long)cut * splits * T * T);
+    u64* part = (u64*)(pr.parts + t.part);
     const int mine = wave * F * F * 128 + lane;
     #pragma unroll
     for (int i = 0; i < F * F; ++i) {
@@ -416,7 +469,7 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
     __syncthreads();
     unsigned* last = (unsigned*)lds;
     if (threadIdx.x == 0)
-      *last = __hip_atomic_fetch_add(g.slots + kd.slot + cut, 1u,
+      *last = __hip_atomic_fetch_add(pr.slots + t.slot, 1u,
                                      __ATOMIC_RELAXED,
                                      __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
@@ -425,7 +478,7 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     __syncthreads();  // all have read it
     if (threadIdx.x == 0)
-      __hip_atomic_store(g.slots + kd.slot + cut, 0u, __ATOMIC_RELAXED,
+      __hip_atomic_store(pr.slots + t.slot, 0u, __ATOMIC_RELAXED,
                          __HIP_MEMORY_SCOPE_AGENT);
     f32x4 own[F * F];
     #pragma unroll
@@ -464,13 +517,13 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
     for (int j = 0; j < F; ++j) {
       const int r = i * 16 + (lane >> 4) * 4, c = j * 16 + (lane & 15);
       f32x4 v = acc[i][j] * pr.alpha;
-      if (KIND == NS_POLY) {
-        // A is symmetric: its row c holds the four in a line
-        const f16* s = pl.a() + split_at(cw + c, rw + r, m.mp);
-        const f16x4 sh = *(const f16x4*)s, sl = *(const f16x4*)(s + 32);
+      if constexpr (KIND == NS_POLY) {
+        f16x4 hi, lo;
+        if constexpr (EARLY) hi = ah[i * F + j], lo = al[i * F + j];
+        else fetch(i, j, hi, lo);
         #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] += pr.beta * ((float)sh[e] + (float)sl[e]);
+          v[e] += pr.beta * ((float)hi[e] + (float)lo[e]);
           if (rw + r + e == cw + c) v[e] += pr.diag;
         }
       }
@@ -483,7 +536,6 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
     }
   // only this wave reads its square, after its own writes
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  const bool tall = m.rows > m.cols;
   // 8 values by rows: (r, c) .. (r, c + 7); by columns: (r, c) .. (r + 7, c)
   auto along_row = [&](int idx, int& r, int& c, u32x4& a, u32x4& b) {
     r = idx / (W / 8);
@@ -501,7 +553,12 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
     }
   };
   if constexpr (FINAL) {
-    const float step = out.lr * m.gain;
+    const NsOutput& out = fin.out;
+    const NsMat* m = fin.mats ? fin.mats + t.mat : &fin.one;
+    const int nrows = m->rows, ncols = m->cols;
+    const long src = m->src + (fin.mats ? 0 : t.mat * fin.src_step);
+    const bool tall = nrows > ncols;
+    const float step = out.lr * m->gain;
     #pragma unroll 2
     for (int idx = lane; idx < W * W / 8; idx += 64) {
       int r, c;
@@ -509,13 +566,13 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
       if (tall) along_col(idx, r, c, a, b);
       else along_row(idx, r, c, a, b);
       const int row = tall ? cw + c : rw + r, col = tall ? rw + r : cw + c;
-      if (row >= m.rows) continue;
+      if (row >= nrows) continue;
       #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int n = m.cols - col - h * 4;
+        const int n = ncols - col - h * 4;
         if (n <= 0) continue;
         const f32x4 o = __builtin_bit_cast(f32x4, h ? b : a);
-        const long i = m.src + (long)row * m.cols + col + h * 4;
+        const long i = src + (long)row * ncols + col + h * 4;
         if (out.master) {
           const f32x4 w = load4(out.master, i, n) * out.keep - step * o;
           store4(out.master, i, n, w);
@@ -530,7 +587,7 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
                 : KIND == NS_POLY ? pl.c()
                                   : pl.x(pr.from ^ 1);
     f16* cols = KIND == NS_APPLY ? pl.y(pr.from ^ 1) : rows;
-    const int ldr = KIND == NS_APPLY ? m.np : m.mp;
+    const int ldr = KIND == NS_APPLY ? t.np : t.mp;
     #pragma unroll 4
     for (int idx = lane; idx < W * W / 8; idx += 64) {
       int r, c;
@@ -544,7 +601,7 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
       if (KIND == NS_APPLY || ti != tj) {
         along_col(idx, r, c, a, b);
         unpack8(a, b, hi, lo);
-        to = cols + split_at(cw + c, rw + r, m.mp);
+        to = cols + split_at(cw + c, rw + r, t.mp);
         *(f16x8*)to = hi;
         *(f16x8*)(to + 32) = lo;
       }
@@ -553,22 +610,12 @@ LO_DEVICE void product_tile(const NsGroup& g, const NsMat& m, int at,
 }
 
 template <int KIND, typename O, bool FINAL>
-__global__ __launch_bounds__(256, 2) void ns_product_kernel(NsGroup g,
-                                                            NsProduct pr,
-                                                            NsOutput out) {
+__global__ __launch_bounds__(256, 2) void ns_product_kernel(NsProduct pr,
+                                                            NsFinal fin) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  // equal matrices: neighbouring tiles on one die, for its cache (the split
-  // tiles of a single one are spread over all dies); a table's order, longest
-  // sums first, is kept
-  int id = blockIdx.x;
-  const int whole = g.count == 1 ? g.one.kind[KIND].whole : (int)gridDim.x;
-  if (!g.mats && id < whole) id = xcd_swizzle(id, whole);
-  int at;
-  const NsMat m = find(g, g.kind_blocks[KIND], g.kinds[KIND], id, at);
-  if (m.tile == 128)
-    product_tile<128, KIND, 2, O, FINAL>(g, m, at, pr, out, lds);
-  else
-    product_tile<64, KIND, 4, O, FINAL>(g, m, at, pr, out, lds);
+  const NsTask t = task_of<KIND>(pr);
+  if (t.tile == 128) product_tile<128, KIND, 2, O, FINAL>(t, pr, fin, lds);
+  else product_tile<64, KIND, 4, O, FINAL>(t, pr, fin, lds);
 }
 
 // ------------------------------------------- matrices that fit one block ----
@@ -952,10 +999,20 @@ void pick_small(const NsGroup& g, int shortest, int longest, const NsInput& in,
 constexpr int kNsLds = 4 * 64 * (64 + 4) * 4;
 
 template <int KIND, typename O, bool FINAL>
-void product(const NsGroup& g, const NsProduct& pr, const NsOutput& out,
-             hipStream_t s) {
+void product(const NsGroup& g, int from, float alpha, float beta, float diag,
+             const NsFinal& fin, hipStream_t s) {
+  const NsMat& m = g.one;
+  const NsProduct pr{g.tasks[KIND],     g.ws,
+                     from,              m.mp,
+                     m.np,              m.tile,
+                     g.kinds[KIND],     m.kind[KIND].whole,
+                     m.kind[KIND].splits, g.count,
+                     g.ws_step,         g.part_step,
+                     g.slot_step,       alpha,
+                     beta,              diag,
+                     g.parts,           g.slots};
   hipLaunchKernelGGL((ns_product_kernel<KIND, O, FINAL>),
-                     dim3(g.all_kinds[KIND]), dim3(256), kNsLds, s, g, pr, out);
+                     dim3(g.all_kinds[KIND]), dim3(256), kNsLds, s, pr, fin);
 }
 
 template <typename T>
@@ -965,18 +1022,20 @@ void run(const NsGroup& g, const NsInput& in, const NsStep* st, int n,
                      g, in);
   hipLaunchKernelGGL(ns_split_kernel<T>, dim3(g.all_splits), dim3(256), 0, s, g,
                      in, st[0].sx, eps);
+  const NsFinal fin{out, g.mats, g.one, g.src_step};
   for (int i = 0; i < n; ++i) {
     const NsStep& k = st[i];
     const int from = i & 1;
-    product<NS_GRAM, float, false>(g, {from, k.sa / (k.sx * k.sx), 0.f, 0.f}, out,
-                               s);
-    product<NS_POLY, float, false>(
-        g, {from, k.c * k.sc / (k.sa * k.sa), k.b * k.sc / k.sa, k.a * k.sc},
-        out, s);
-    const float next = i + 1 < n ? k.sn : 1.f;
-    const NsProduct pr{from, next / (k.sc * k.sx), 0.f, 0.f};
-    if (i + 1 < n) product<NS_APPLY, float, false>(g, pr, out, s);
-    else product<NS_APPLY, T, true>(g, pr, out, s);
+    product<NS_GRAM, float, false>(g, from, k.sa / (k.sx * k.sx), 0.f, 0.f,
+                                   fin, s);
+    product<NS_POLY, float, false>(g, from, k.c * k.sc / (k.sa * k.sa),
+                                   k.b * k.sc / k.sa, k.a * k.sc, fin, s);
+    if (i + 1 < n)
+      product<NS_APPLY, float, false>(g, from, k.sn / (k.sc * k.sx), 0.f, 0.f,
+                                      fin, s);
+    else
+      product<NS_APPLY, T, true>(g, from, 1.f / (k.sc * k.sx), 0.f, 0.f, fin,
+                                 s);
   }
 }
 

@@ -82,6 +82,37 @@ inline int64_t ns_depth(const NsMat& m, int kind) {
   return (kind == NS_GRAM ? m.np : m.mp) / 32;
 }
 
+// Tile l of a product, in bands of eight tile rows, down a band's columns
+// first: 64 tiles in turn read 8 + 8 panels. APPLY covers tm x tn tiles, the
+// symmetric ones the lower triangle of tm x tm.
+__host__ __device__ inline void ns_tile_at(int kind, int l, int tm, int tn,
+                                           int& ti, int& tj) {
+  int band = 0, left = 0;  // the band, and the columns left of its triangle
+  if (kind == NS_APPLY) {
+    if (tm > 8) band = l / (8 * tn);
+    l -= band * 8 * tn;
+    left = tn;
+  } else if (tm > 8) {
+    // band b starts at tile 32 b (b - 1) + 36 b
+    band = (int)sqrtf((float)l * (1.f / 32.f));
+    while (32 * band * (band - 1) + 36 * band > l) --band;
+    while (32 * band * (band + 1) + 36 * (band + 1) <= l) ++band;
+    l -= 32 * band * (band - 1) + 36 * band;
+    left = 8 * band;
+  }
+  const int h = tm - 8 * band < 8 ? tm - 8 * band : 8;
+  if (l < h * left) {
+    tj = l / h;
+    ti = 8 * band + l - tj * h;
+    return;
+  }
+  l -= h * left;
+  const int r = (l >= 1) + (l >= 3) + (l >= 6) + (l >= 10) + (l >= 15) +
+                (l >= 21) + (l >= 28);
+  ti = 8 * band + r;
+  tj = 8 * band + l - r * (r + 1) / 2;
+}
+
 inline int64_t ns_blocks(const NsMat& m, int kind) {
   const NsTiles& k = m.kind[kind];
   return k.whole + (ns_tiles(m, kind) - k.whole) * k.splits;
@@ -155,11 +186,8 @@ inline void ns_place(std::vector<NsMat>& mats, NsNeeds& sum) {
     sum.chunks += m.chunks;
     sum.splits += (int64_t)(m.mp / 64) * (m.np / 64);
     for (int k = 0; k < NS_KINDS; ++k) {
-      NsTiles& t = m.kind[k];
-      const int64_t cut = ns_tiles(m, k) - t.whole;
-      t.part = part[k];
-      t.slot = (int)slot[k];
-      part[k] += cut * t.splits * m.tile * m.tile;
+      const int64_t cut = ns_tiles(m, k) - m.kind[k].whole;
+      part[k] += cut * m.kind[k].splits * m.tile * m.tile;
       slot[k] += cut;
       sum.kinds[k] += ns_blocks(m, k);
       sum.parts = std::max(sum.parts, part[k]);
@@ -170,6 +198,45 @@ inline void ns_place(std::vector<NsMat>& mats, NsNeeds& sum) {
   if (sum.chunks > most || sum.splits > most || sum.kinds[NS_APPLY] > most ||
       sum.kinds[NS_GRAM] > most)
     throw std::invalid_argument("too many elements for one plan");
+}
+
+// the blocks of one product over placed matrices, longest sums first, so that
+// none of those starts last
+inline std::vector<NsTask> ns_tasks(const std::vector<NsMat>& mats, int kind) {
+  std::vector<int> order(mats.size());
+  for (size_t i = 0; i < mats.size(); ++i) order[i] = (int)i;
+  auto work = [&](int i) {
+    const NsMat& m = mats[i];
+    return ns_depth(m, kind) * m.tile * m.tile / m.kind[kind].splits;
+  };
+  std::stable_sort(order.begin(), order.end(),
+                   [&](int a, int b) { return work(a) > work(b); });
+  std::vector<NsTask> tasks;
+  int64_t part = 0, slot = 0;
+  for (int i : order) {
+    const NsMat& m = mats[i];
+    const int whole = m.kind[kind].whole, splits = m.kind[kind].splits;
+    const int tiles = (int)ns_tiles(m, kind), depth = (int)ns_depth(m, kind);
+    for (int l = 0; l < tiles; ++l) {
+      NsTask t{};
+      t.ws = m.ws;
+      t.mat = i;
+      t.tile = m.tile;
+      t.mp = m.mp;
+      t.np = m.np;
+      ns_tile_at(kind, l, m.mp / m.tile, m.np / m.tile, t.ti, t.tj);
+      t.splits = l < whole ? 1 : splits;
+      t.part = part;
+      t.slot = (int)slot;
+      for (t.slice = 0; t.slice < t.splits; ++t.slice) {
+        t.k0 = (int)((int64_t)depth * t.slice / t.splits);
+        t.k1 = (int)((int64_t)depth * (t.slice + 1) / t.splits);
+        tasks.push_back(t);
+      }
+      if (l >= whole) part += (int64_t)splits * m.tile * m.tile, ++slot;
+    }
+  }
+  return tasks;
 }
 
 }  // namespace lo
