@@ -13,6 +13,7 @@ enum { NS_GRAM, NS_POLY, NS_APPLY, NS_KINDS };
 // how a product's tiles are shared out: the first `whole` take one block each,
 // the others `splits` blocks, each a part of the sum
 struct NsTiles {
+  int tile;  // 32, 64 or 128
   int whole, splits;
 };
 
@@ -20,7 +21,6 @@ struct NsMat {
   long src;        // first element in the input
   long ws;         // first half of its workspace
   int rows, cols;  // as stored
-  int tile;        // 64 or 128
   int mp, np;      // short and long side, padded to whole tiles
   int sum;         // first of its partial norms
   int chunks;      // how many

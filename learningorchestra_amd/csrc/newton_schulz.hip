@@ -304,14 +304,14 @@ LO_DEVICE NsTask task_of(const NsProduct& pr) {
     t.slot += cut;
     id = pr.whole + cut;
   }
-  const int shift = t.tile == 128 ? 7 : 6;
+  const int shift = t.tile == 128 ? 7 : t.tile == 64 ? 6 : 5;
   ns_tile_at(KIND, id, t.mp >> shift, t.np >> shift, t.ti, t.tj);
   const int depth = (KIND == NS_GRAM ? t.np : t.mp) / 32;
   t.k0 = 0;
   t.k1 = depth;
   if (t.splits > 1) {
-    t.k0 = depth * t.slice / t.splits;
-    t.k1 = depth * (t.slice + 1) / t.splits;
+    t.k0 = depth / 2 * t.slice / t.splits * 2;
+    t.k1 = depth / 2 * (t.slice + 1) / t.splits * 2;
   }
   return t;
 }
@@ -319,7 +319,7 @@ LO_DEVICE NsTask task_of(const NsProduct& pr) {
 // One product on T x T tiles, four waves, S staged tiles of both operands (32
 // values of the sum each) in LDS. FINAL: the last step's X' goes to the output
 // in place of the workspace.
-template <int T, int KIND, int S, typename O, bool FINAL>
+template <int T, int KIND, int S, int KB, typename O, bool FINAL>
 LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
                             const NsFinal& fin, char* lds) {
   constexpr int W = T / 2;      // a wave's square
@@ -348,20 +348,21 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
   P += (long)ti * T * 2 * ld + lane_off;
   Q += (long)tj * T * 2 * ld + lane_off;
   auto stage = [&](int kt) {
-    char* buf = lds + (kt - k0) % S * 2 * IMG + wave * LOADS * 1024;
+    char* buf = lds + (kt - k0) / KB % S * (2 * KB * IMG) + wave * LOADS * 1024;
     #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const long off = (long)i * 16 * ld + kt * 64;
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) unsigned int*)(P + off),
-          (__attribute__((address_space(3))) unsigned int*)(buf + i * 1024),
-          16, 0, 0);
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) unsigned int*)(Q + off),
-          (__attribute__((address_space(3))) unsigned int*)(buf + IMG +
-                                                            i * 1024),
-          16, 0, 0);
-    }
+    for (int h = 0; h < KB; ++h)
+      #pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const long off = (long)i * 16 * ld + (kt + h) * 64;
+        char* to = buf + h * 2 * IMG + i * 1024;
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) unsigned int*)(P + off),
+            (__attribute__((address_space(3))) unsigned int*)to, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) unsigned int*)(Q + off),
+            (__attribute__((address_space(3))) unsigned int*)(to + IMG), 16, 0,
+            0);
+      }
   };
   struct Frags {
     f16x8 ph[F], pw[F], qh[F], ql[F];
@@ -371,7 +372,7 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
                            ((half * 64 + (lane >> 4) * 16) ^ ((row & 7) << 4)));
   };
   auto read = [&](int kt, Frags& s) {
-    const char* img = lds + (kt - k0) % S * 2 * IMG;
+    const char* img = lds + ((kt - k0) / KB % S * KB + (kt - k0) % KB) * 2 * IMG;
     #pragma unroll
     for (int i = 0; i < F; ++i) {
       const int row = i * 16 + (lane & 15);
@@ -404,7 +405,7 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
   // A's part of C: A is symmetric, so its row c holds a lane's four values in
   // a line. Small tiles fetch it while the sum is taken (large ones have no
   // registers to spare, and more to do meanwhile).
-  constexpr bool EARLY = KIND == NS_POLY && T == 64;
+  constexpr bool EARLY = KIND == NS_POLY && T < 128;
   f16x4 ah[EARLY ? F * F : 1], al[EARLY ? F * F : 1];
   auto fetch = [&](int i, int j, f16x4& hi, f16x4& lo) {
     const int r = ti * T + wr * W + i * 16 + (lane >> 4) * 4;
@@ -418,41 +419,46 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
     for (int i = 0; i < F * F; ++i) fetch(i / F, i % F, ah[i], al[i]);
   }
 
-  // The loop adds a tile's fragments while the next one's are read from LDS
-  // and S - 1 more are on their way. `ready` waits until tile kt has landed
-  // and every wave has read the one before, whose buffer is then free.
-  auto ready = [&](int kt, int newest) {
+  // KB steps a stage and barrier. The loop adds a step's fragments while the
+  // next one's are read from LDS and S - 1 stages are on their way. `ready`
+  // waits until the stage at kt has landed and every wave has read the one
+  // before, whose buffer is then free.
+  auto ready = [&](int newest) {
     if (newest < k1)
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(
-                       (S - 2) * 2 * LOADS)
+                       (S - 2) * 2 * LOADS * KB)
                    : "memory");
     else
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
-  for (int kt = k0; kt < k0 + S - 1; ++kt)
+  for (int kt = k0; kt < k0 + (S - 1) * KB; kt += KB)
     if (kt < k1) stage(kt);
   Frags a, b;
-  ready(k0, k0 + S - 2);
+  ready(k0 + (S - 2) * KB);
   read(k0, a);
-  if (k0 + S - 1 < k1) stage(k0 + S - 1);
-  auto step = [&](int kt, const Frags& now, Frags& next) {
+  if (k0 + (S - 1) * KB < k1) stage(k0 + (S - 1) * KB);
+  auto step = [&](int kt, bool fresh, const Frags& now, Frags& next) {
     if (kt + 1 < k1) {
-      ready(kt + 1, kt + S - 1);
+      if (fresh) ready(kt + 1 + (S - 2) * KB);
       read(kt + 1, next);
-      if (kt + S < k1) stage(kt + S);
+      if (fresh && kt + 1 + (S - 1) * KB < k1) stage(kt + 1 + (S - 1) * KB);
     }
     add(now);
   };
+  // k1 - k0 is a multiple of KB
   for (int kt = k0; kt < k1; kt += 2) {
-    step(kt, a, b);
-    if (kt + 1 < k1) step(kt + 1, b, a);
+    step(kt, KB == 1, a, b);
+    if (KB > 1 || kt + 1 < k1) step(kt + 1, true, b, a);
   }
   __syncthreads();  // the staging buffers are free from here on
 
   if (splits > 1) {
     // Parts are written through to where all dies see them (agent-scope
-    // stores), and have arrived there before the counter goes up: no cache
-    // needs writing back. The last block drops what its die holds of others'.
+    // stores), and have arrived there before the counter goes up, so that no
+    // cache needs writing back. Nor has any cache an older copy to drop: the
+    // last block is the first of this launch to read these lines, and what
+    // earlier launches left went where this one began. (A release and an
+    // acquire cost 8 us a launch instead, at 36 tiles.)
     typedef unsigned long long u64;
     u64* part = (u64*)(pr.parts + t.part);
     const int mine = wave * F * F * 128 + lane;
@@ -475,7 +481,7 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
     __syncthreads();
     const bool join = *last == (unsigned)splits - 1;
     if (!join) return;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
     __syncthreads();  // all have read it
     if (threadIdx.x == 0)
       __hip_atomic_store(pr.slots + t.slot, 0u, __ATOMIC_RELAXED,
@@ -614,8 +620,9 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(NsProduct pr,
                                                             NsFinal fin) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const NsTask t = task_of<KIND>(pr);
-  if (t.tile == 128) product_tile<128, KIND, 2, O, FINAL>(t, pr, fin, lds);
-  else product_tile<64, KIND, 4, O, FINAL>(t, pr, fin, lds);
+  if (t.tile == 128) product_tile<128, KIND, 2, 1, O, FINAL>(t, pr, fin, lds);
+  else if (t.tile == 64) product_tile<64, KIND, 4, 1, O, FINAL>(t, pr, fin, lds);
+  else product_tile<32, KIND, 4, 2, O, FINAL>(t, pr, fin, lds);
 }
 
 // ------------------------------------------- matrices that fit one block ----
@@ -995,7 +1002,7 @@ void pick_small(const NsGroup& g, int shortest, int longest, const NsInput& in,
   }
 }
 
-// both tile sizes' staging buffers take 64 KiB; 128's squares need 4 KiB more
+// every tile size's staging buffers take 64 KiB; 128's squares need 4 KiB more
 constexpr int kNsLds = 4 * 64 * (64 + 4) * 4;
 
 template <int KIND, typename O, bool FINAL>
@@ -1004,7 +1011,7 @@ void product(const NsGroup& g, int from, float alpha, float beta, float diag,
   const NsMat& m = g.one;
   const NsProduct pr{g.tasks[KIND],     g.ws,
                      from,              m.mp,
-                     m.np,              m.tile,
+                     m.np,              m.kind[KIND].tile,
                      g.kinds[KIND],     m.kind[KIND].whole,
                      m.kind[KIND].splits, g.count,
                      g.ws_step,         g.part_step,

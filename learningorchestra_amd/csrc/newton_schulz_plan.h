@@ -74,7 +74,7 @@ struct NsNeeds {
 };
 
 inline int64_t ns_tiles(const NsMat& m, int kind) {
-  const int64_t tm = m.mp / m.tile, tn = m.np / m.tile;
+  const int64_t tm = m.mp / m.kind[kind].tile, tn = m.np / m.kind[kind].tile;
   return kind == NS_APPLY ? tm * tn : tm * (tm + 1) / 2;
 }
 
@@ -124,7 +124,47 @@ inline bool ns_fit_block(int shortest, int longest) {
   return shortest <= 32 ? longest <= 2048 : shortest <= 64 && longest <= 1024;
 }
 
-// Shapes, tiles and sharing of `copies` of each of the matrices.
+// What a tile size costs, in microseconds, fitted to launches of single
+// products (36 shapes within 15 %): a launch with its first loads and its end;
+// a step of 32 values of the sum on a CU of its own, which the way to memory
+// bounds (8, 16 and 32 KiB, about 53 GB/s a CU, for operands that other dies
+// wrote); handing over the parts of a split sum, for each part that the last
+// block adds and for each part on the chip.
+struct NsCost {
+  int tile;
+  double launch, step, join, add, part;
+};
+constexpr NsCost kNsCosts[] = {{32, 3.2, 0.15, 1.5, 0.3, 0.006},
+                               {64, 3.6, 0.306, 2.5, 0.4, 0.004},
+                               {128, 5.0, 0.6, 4.0, 1.2, 0.02}};
+constexpr double kNsBytes = 8.5e6;  // bytes a microsecond that all CUs load
+
+// the cost of one product over the matrices (copies of each), every sum cut
+// into parts of at most `most` steps; fills in how
+inline double ns_share(std::vector<NsMat>& mats, int64_t copies, int kind,
+                       const NsCost& want, int64_t most) {
+  double longest = 0, bytes = 0, join = 0, parts = 0;
+  for (NsMat& m : mats) {
+    const bool fits = m.mp % want.tile == 0 && m.np % want.tile == 0;
+    const NsCost& c = fits ? want : kNsCosts[1];
+    NsTiles& k = m.kind[kind];
+    k.tile = c.tile;
+    const int64_t tiles = ns_tiles(m, kind), depth = ns_depth(m, kind);
+    const int64_t s = std::min((depth + most - 1) / most, depth / 2);
+    k.splits = (int)s;
+    k.whole = s > 1 ? 0 : (int)tiles;
+    longest = std::max(longest, (double)depth / s * c.step);
+    bytes += (double)(tiles * copies * depth) * c.tile * 256;
+    if (s > 1) {
+      join = std::max(join, c.join + c.add * s);
+      parts += c.part * (double)(tiles * copies * s);
+    }
+  }
+  return want.launch + std::max(longest, bytes / kNsBytes) + join + parts;
+}
+
+// Shapes, and for each product the tiles and their sharing, of `copies` of
+// each of the matrices: the cheapest tile size and cut of the sums for all.
 inline std::vector<NsMat> ns_plan(
     const std::vector<std::pair<int64_t, int64_t>>& sides, int64_t copies) {
   int64_t big = 0;
@@ -135,41 +175,35 @@ inline std::vector<NsMat> ns_plan(
     NsMat m{};
     m.rows = (int)rows;
     m.cols = (int)cols;
-    m.tile = big >= 256 && std::min(rows, cols) > 64 ? 128 : 64;
-    m.mp = (int)ns_up(std::min(rows, cols), m.tile);
-    m.np = (int)ns_up(std::max(rows, cols), m.tile);
+    // whole tiles of 128 only where there will be many of them
+    const int64_t pad = big >= 256 && std::min(rows, cols) > 64 ? 128 : 64;
+    m.mp = (int)ns_up(std::min(rows, cols), pad);
+    m.np = (int)ns_up(std::max(rows, cols), pad);
     m.chunks = (int)(ns_up(rows * cols, kNsChunk) / kNsChunk);
     m.gain = (float)std::sqrt(std::max(1.0, (double)rows / (double)cols));
     mats.push_back(m);
   }
   for (int kind = 0; kind < NS_KINDS; ++kind) {
-    int64_t all = 0;
-    for (const NsMat& m : mats) all += ns_tiles(m, kind) * copies;
-    for (NsMat& m : mats) {
-      const int64_t tiles = ns_tiles(m, kind), depth = ns_depth(m, kind);
-      // s blocks take depth / s steps each and the last of them s additions
-      // of a tile; a step costs about as much as 2 additions (64) or one. A
-      // part below 12 or 16 steps costs more to hand over than it saves: 256 x
-      // 3136 took 232 us with any depth split, 150 us so, 154 us from 16 or 32
-      // steps on; the ResNet-50's matrices 1486, 1436 and 1435 us.
-      const bool small = m.tile == 64;
-      const int64_t most = std::max<int64_t>(
-          1, std::min((int64_t)std::sqrt((double)depth * (small ? 2 : 1)),
-                      depth / (small ? 12 : 16)));
-      NsTiles& k = m.kind[kind];
-      k.whole = (int)tiles;
-      k.splits = 1;
-      if (all < kNsSlots) {
-        const int64_t s = std::min(kNsSlots / all, most);
-        if (s > 1) k.whole = 0, k.splits = (int)s;
-      } else if (mats.size() * copies == 1) {
-        // what full rounds of the chip leave over
-        const int64_t rest = all % kNsSlots;
-        const int64_t s =
-            rest ? std::min(kNsSlots / rest, most) : 1;
-        if (s > 1 && all < 4 * kNsSlots)
-          k.whole = (int)(tiles - rest), k.splits = (int)s;
+    const NsCost* tile = &kNsCosts[1];
+    int64_t cut = kNsSide;
+    double best = 1e300;
+    for (const NsCost& c : kNsCosts) {
+      if (c.tile == 128 && big < 256) continue;
+      for (int64_t most : {kNsSide, 96l, 64l, 48l, 32l, 24l, 16l, 12l, 8l}) {
+        const double cost = ns_share(mats, copies, kind, c, most);
+        if (cost < best) best = cost, tile = &c, cut = most;
       }
+    }
+    ns_share(mats, copies, kind, *tile, cut);
+    // a single matrix's tiles beyond full rounds of the chip, if those are few
+    NsTiles& k = mats[0].kind[kind];
+    const int64_t tiles = ns_tiles(mats[0], kind), rest = tiles % kNsSlots;
+    if (mats.size() * copies == 1 && k.splits == 1 && tiles > kNsSlots &&
+        tiles < 4 * kNsSlots && rest) {
+      const int64_t depth = ns_depth(mats[0], kind);
+      const int64_t s = std::min(
+          {kNsSlots / rest, (int64_t)std::sqrt((double)depth), depth / 16});
+      if (s > 1) k.whole = (int)(tiles - rest), k.splits = (int)s;
     }
   }
   return mats;
@@ -187,7 +221,7 @@ inline void ns_place(std::vector<NsMat>& mats, NsNeeds& sum) {
     sum.splits += (int64_t)(m.mp / 64) * (m.np / 64);
     for (int k = 0; k < NS_KINDS; ++k) {
       const int64_t cut = ns_tiles(m, k) - m.kind[k].whole;
-      part[k] += cut * m.kind[k].splits * m.tile * m.tile;
+      part[k] += cut * m.kind[k].splits * m.kind[k].tile * m.kind[k].tile;
       slot[k] += cut;
       sum.kinds[k] += ns_blocks(m, k);
       sum.parts = std::max(sum.parts, part[k]);
@@ -207,7 +241,8 @@ inline std::vector<NsTask> ns_tasks(const std::vector<NsMat>& mats, int kind) {
   for (size_t i = 0; i < mats.size(); ++i) order[i] = (int)i;
   auto work = [&](int i) {
     const NsMat& m = mats[i];
-    return ns_depth(m, kind) * m.tile * m.tile / m.kind[kind].splits;
+    const NsTiles& k = m.kind[kind];
+    return ns_depth(m, kind) * k.tile * k.tile / k.splits;
   };
   std::stable_sort(order.begin(), order.end(),
                    [&](int a, int b) { return work(a) > work(b); });
@@ -215,25 +250,25 @@ inline std::vector<NsTask> ns_tasks(const std::vector<NsMat>& mats, int kind) {
   int64_t part = 0, slot = 0;
   for (int i : order) {
     const NsMat& m = mats[i];
-    const int whole = m.kind[kind].whole, splits = m.kind[kind].splits;
+    const auto [tile, whole, splits] = m.kind[kind];
     const int tiles = (int)ns_tiles(m, kind), depth = (int)ns_depth(m, kind);
     for (int l = 0; l < tiles; ++l) {
       NsTask t{};
       t.ws = m.ws;
       t.mat = i;
-      t.tile = m.tile;
+      t.tile = tile;
       t.mp = m.mp;
       t.np = m.np;
-      ns_tile_at(kind, l, m.mp / m.tile, m.np / m.tile, t.ti, t.tj);
+      ns_tile_at(kind, l, m.mp / tile, m.np / tile, t.ti, t.tj);
       t.splits = l < whole ? 1 : splits;
       t.part = part;
       t.slot = (int)slot;
       for (t.slice = 0; t.slice < t.splits; ++t.slice) {
-        t.k0 = (int)((int64_t)depth * t.slice / t.splits);
-        t.k1 = (int)((int64_t)depth * (t.slice + 1) / t.splits);
+        t.k0 = depth / 2 * t.slice / t.splits * 2;
+        t.k1 = depth / 2 * (t.slice + 1) / t.splits * 2;
         tasks.push_back(t);
       }
-      if (l >= whole) part += (int64_t)splits * m.tile * m.tile, ++slot;
+      if (l >= whole) part += (int64_t)splits * tile * tile, ++slot;
     }
   }
   return tasks;
