@@ -136,7 +136,7 @@ struct NsCost {
 };
 constexpr NsCost kNsCosts[] = {{32, 3.2, 0.15, 1.5, 0.3, 0.006},
                                {64, 3.6, 0.306, 2.5, 0.4, 0.004},
-                               {128, 5.0, 0.6, 4.0, 1.2, 0.02}};
+                               {128, 5.0, 1.0, 4.0, 1.2, 0.02}};
 constexpr double kNsBytes = 8.5e6;  // bytes a microsecond that all CUs load
 
 // the cost of one product over the matrices (copies of each), every sum cut
