@@ -13,10 +13,14 @@
 // mean and variance come from two reductions over those registers (the second
 // over squared differences, so a large mean costs no digits), and the backward
 // pass forms dx and its share of dgamma/dbeta from the same loads. A block
-// walks rows blockIdx, blockIdx + grid, ... with gamma, beta and the two
-// gradient sums in registers; the blocks' sums go to a [blocks, 2, cols]
-// workspace that a second small kernel adds in a fixed order, so results do
-// not depend on timing. With one block the sums are written directly.
+// walks rows blockIdx, blockIdx + grid, ..., backwards with the next row's
+// loads on their way; its gradient sums stay in registers and go to a
+// [blocks, 2, cols] workspace that a second small kernel adds in a fixed
+// order, so results do not depend on timing. With one block the sums are
+// written directly. Where a block has few rows, its sums are more to write
+// than the rows were to read, and rows of more than 16 elements a thread
+// (16384 columns) have no registers left for them: there a kernel of its own
+// takes the sums down the columns, at the price of a second reading.
 //
 // Columns need not be a multiple of VE: the vector that would cross the row's
 // end is moved back to end with it, and the elements it shares with its
@@ -51,37 +55,71 @@ LO_DEVICE void load_f32(const float* __restrict__ p, float (&o)[VE]) {
   for (int j = 0; j < VE; ++j) o[j] = p[j];
 }
 
-// sums over the TPR threads that share a row; every one of them gets both.
+// v + the value of the lane that a DPP pattern names
+template <int CTRL>
+LO_DEVICE float add_dpp(float v) {
+  const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL,
+                                            0xf, 0xf, false);
+  return v + __builtin_bit_cast(float, o);
+}
+
+// The sum over aligned groups of N lanes, in every lane. Within 16 lanes by
+// DPP (1, 2 apart, then the mirror images of 8 and of 16), then by swapping
+// rows of 16 and halves: a tenth of the way through LDS that shuffles take.
+template <int N>
+LO_DEVICE float lane_sum(float v) {
+  if constexpr (N >= 2) v = add_dpp<0xb1>(v);    // quad_perm 1 0 3 2
+  if constexpr (N >= 4) v = add_dpp<0x4e>(v);    // quad_perm 2 3 0 1
+  if constexpr (N >= 8) v = add_dpp<0x141>(v);   // row_half_mirror
+  if constexpr (N >= 16) v = add_dpp<0x140>(v);  // row_mirror
+  if constexpr (N >= 32) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned a = p[0], b = p[1];
+    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+  }
+  if constexpr (N >= 64) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned a = p[0], b = p[1];
+    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+  }
+  return v;
+}
+
+// K sums over the TPR threads that share a row; every one of them gets all.
 // For TPR > 64 the LDS slots alternate between calls, so one barrier per call
 // is enough: a slot is rewritten two calls later, past the barrier that its
 // last readers reach before the next call's.
-template <int TPR>
-LO_DEVICE void row_sum2(float& a, float& b, float* red, int& turn) {
+template <int TPR, int K>
+LO_DEVICE void row_sum(float (&v)[K], float* red, int& turn) {
   #pragma unroll
-  for (int off = (TPR < 64 ? TPR : 64) / 2; off > 0; off >>= 1) {
-    a += __shfl_xor(a, off);
-    b += __shfl_xor(b, off);
-  }
+  for (int k = 0; k < K; ++k) v[k] = lane_sum<(TPR < 64 ? TPR : 64)>(v[k]);
   if constexpr (TPR > 64) {
     constexpr int W = TPR / 64;
     float* slot = red + (turn & 1) * 2 * W;
     ++turn;
     if ((threadIdx.x & 63) == 0) {
-      slot[threadIdx.x >> 6] = a;
-      slot[W + (threadIdx.x >> 6)] = b;
+      #pragma unroll
+      for (int k = 0; k < K; ++k) slot[k * W + (threadIdx.x >> 6)] = v[k];
     }
     __syncthreads();
-    a = 0.f;
-    b = 0.f;
     #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      a += slot[w];
-      b += slot[W + w];
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0.f;
+      #pragma unroll
+      for (int w = 0; w < W; ++w) v[k] += slot[k * W + w];
     }
   }
 }
 
 constexpr int ln_block(int tpr) { return tpr > 256 ? tpr : 256; }
+
+// gamma and beta stay in registers for all of a block's rows, but where a row
+// fills those: then they come from the cache each time, and the backward pass
+// does without the next row's loads
+template <int VE, int TPR, int NV>
+constexpr bool ln_hoist() { return TPR < 1024 || NV * VE <= 8; }
 
 template <typename T, int VE, int TPR, int NV>
 __global__ __launch_bounds__(ln_block(TPR)) void layernorm_fwd_kernel(
@@ -91,70 +129,80 @@ __global__ __launch_bounds__(ln_block(TPR)) void layernorm_fwd_kernel(
     float* __restrict__ invstd, long rows, int cols, float eps) {
   typedef typename RowVec<T, VE>::type V;
   constexpr int RPB = ln_block(TPR) / TPR;
+  constexpr bool HOIST = ln_hoist<VE, TPR, NV>();
   __shared__ float red[TPR > 64 ? 4 * (TPR / 64) : 1];
   const int t = threadIdx.x % TPR;
   const float n = (float)cols;
   int base[NV], skip[NV];
-  float gm[NV][VE], bt[NV][VE];
+  float gm[HOIST ? NV : 1][VE], bt[HOIST ? NV : 1][VE];
   #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c0 = (i * TPR + t) * VE;
     base[i] = min(c0, cols - VE);
     skip[i] = min(c0 - base[i], VE);
-    load_f32<VE>(gamma + base[i], gm[i]);
-    load_f32<VE>(beta + base[i], bt[i]);
+    if constexpr (HOIST) {
+      load_f32<VE>(gamma + base[i], gm[i]);
+      load_f32<VE>(beta + base[i], bt[i]);
+    }
   }
   int turn = 0;
-  for (long r = (long)blockIdx.x * RPB + threadIdx.x / TPR; r < rows;
-       r += (long)gridDim.x * RPB) {
-    V xv[NV];
+  const long step = (long)gridDim.x * RPB;
+  long r = (long)blockIdx.x * RPB + threadIdx.x / TPR;
+  for (; r < rows; r += step) {
+    V s[NV];
     #pragma unroll
-    for (int i = 0; i < NV; ++i) xv[i] = *(const V*)(x + r * ldx + base[i]);
+    for (int i = 0; i < NV; ++i) s[i] = *(const V*)(x + r * ldx + base[i]);
     if (res) {
       #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const V rv = *(const V*)(res + r * ldr + base[i]);
         if constexpr (VE == 1) {
-          xv[i] = (T)((float)xv[i] + (float)rv);
+          s[i] = (T)((float)s[i] + (float)rv);
         } else {
           #pragma unroll
           for (int j = 0; j < VE; ++j)
-            xv[i][j] = (T)((float)xv[i][j] + (float)rv[j]);
+            s[i][j] = (T)((float)s[i][j] + (float)rv[j]);
         }
       }
     }
-    float s1 = 0.f, s2 = 0.f;
+    float acc[1] = {0.f};
     #pragma unroll
     for (int i = 0; i < NV; ++i)
       #pragma unroll
       for (int j = 0; j < VE; ++j)
-        s1 += j >= skip[i] ? elem<VE>(xv[i], j) : 0.f;
-    row_sum2<TPR>(s1, s2, red, turn);
-    const float mu = s1 / n;
-    s1 = 0.f;
-    s2 = 0.f;
+        acc[0] += j >= skip[i] ? elem<VE>(s[i], j) : 0.f;
+    row_sum<TPR>(acc, red, turn);
+    const float mu = acc[0] / n;
+    acc[0] = 0.f;
     #pragma unroll
     for (int i = 0; i < NV; ++i)
       #pragma unroll
       for (int j = 0; j < VE; ++j) {
-        const float d = elem<VE>(xv[i], j) - mu;
-        s1 += j >= skip[i] ? d * d : 0.f;
+        const float d = elem<VE>(s[i], j) - mu;
+        acc[0] += j >= skip[i] ? d * d : 0.f;
       }
-    row_sum2<TPR>(s1, s2, red, turn);
-    const float is = 1.f / sqrtf(s1 / n + eps);
+    row_sum<TPR>(acc, red, turn);
+    const float is = 1.f / sqrtf(acc[0] / n + eps);
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (skip[i] >= VE) continue;
-      V o;
-      if constexpr (VE == 1) {
-        o = (T)(((float)xv[i] - mu) * is * gm[i][0] + bt[i][0]);
-      } else {
+      float g[VE], b[VE];
+      if constexpr (HOIST) {
         #pragma unroll
-        for (int j = 0; j < VE; ++j)
-          o[j] = (T)(((float)xv[i][j] - mu) * is * gm[i][j] + bt[i][j]);
+        for (int j = 0; j < VE; ++j) g[j] = gm[i][j], b[j] = bt[i][j];
+      } else {
+        load_f32<VE>(gamma + base[i], g);
+        load_f32<VE>(beta + base[i], b);
+      }
+      V o;
+      #pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        const float v = (elem<VE>(s[i], j) - mu) * is * g[j] + b[j];
+        if constexpr (VE == 1) o = (T)v;
+        else o[j] = (T)v;
       }
       *(V*)(y + r * ldy + base[i]) = o;
-      if (sum) *(V*)(sum + r * lds + base[i]) = xv[i];
+      if (sum) *(V*)(sum + r * lds + base[i]) = s[i];
     }
     if (t == 0 && mean) {
       mean[r] = mu;
@@ -164,8 +212,9 @@ __global__ __launch_bounds__(ln_block(TPR)) void layernorm_fwd_kernel(
 }
 
 // part: [gridDim.x, 2, cols] sums of dy * xhat and of dy, or null with one
-// block, which then writes dgamma/dbeta itself
-template <typename T, int VE, int TPR, int NV>
+// block, which then writes dgamma/dbeta itself. SUMS: whether they are taken
+// here at all.
+template <typename T, int VE, int TPR, int NV, bool SUMS>
 __global__ __launch_bounds__(ln_block(TPR)) void layernorm_bwd_kernel(
     const T* dy, long ldy, const T* x, long ldx,
     const T* skipg, long ldk, const float* __restrict__ mean,
@@ -174,53 +223,90 @@ __global__ __launch_bounds__(ln_block(TPR)) void layernorm_bwd_kernel(
     float* __restrict__ dbeta, long rows, int cols) {
   typedef typename RowVec<T, VE>::type V;
   constexpr int RPB = ln_block(TPR) / TPR;
+  constexpr bool HOIST = ln_hoist<VE, TPR, NV>();
   __shared__ float red[TPR > 64 ? 4 * (TPR / 64) : 1];
   extern __shared__ __attribute__((aligned(16))) float acc[];  // [2][cols]
   const int t = threadIdx.x % TPR;
   const float n = (float)cols;
   int base[NV], skip[NV];
-  float gm[NV][VE], dg[NV][VE] = {}, db[NV][VE] = {};
+  float gm[HOIST ? NV : 1][VE];
+  float dg[SUMS ? NV : 1][VE] = {}, db[SUMS ? NV : 1][VE] = {};
   #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c0 = (i * TPR + t) * VE;
     base[i] = min(c0, cols - VE);
     skip[i] = min(c0 - base[i], VE);
-    load_f32<VE>(gamma + base[i], gm[i]);
+    if constexpr (HOIST) load_f32<VE>(gamma + base[i], gm[i]);
   }
   int turn = 0;
-  for (long r = (long)blockIdx.x * RPB + threadIdx.x / TPR; r < rows;
-       r += (long)gridDim.x * RPB) {
-    V xv[NV], gv[NV], kv[NV];
+  const long step = (long)gridDim.x * RPB;
+  long r = (long)blockIdx.x * RPB + threadIdx.x / TPR;
+  V nx[NV], ng[NV];
+  float nmu = 0.f, nis = 0.f;
+  auto load = [&](long at) {
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      xv[i] = *(const V*)(x + r * ldx + base[i]);
-      gv[i] = *(const V*)(dy + r * ldy + base[i]);
-      if (skipg) kv[i] = *(const V*)(skipg + r * ldk + base[i]);
+      nx[i] = *(const V*)(x + at * ldx + base[i]);
+      ng[i] = *(const V*)(dy + at * ldy + base[i]);
     }
-    const float mu = mean[r], is = invstd[r];
-    float s1 = 0.f, s2 = 0.f;
+    nmu = mean[at];
+    nis = invstd[at];
+  };
+  auto gammas = [&](int i, float (&ga)[VE]) {
+    if constexpr (HOIST) {
+      #pragma unroll
+      for (int j = 0; j < VE; ++j) ga[j] = gm[i][j];
+    } else {
+      // an address that is new to the compiler: it would keep both readings
+      const float* p = gamma + base[i];
+      asm volatile("" : "+v"(p));
+      load_f32<VE>(p, ga);
+    }
+  };
+  if (HOIST && r < rows) load(r);
+  for (; r < rows; r += step) {
+    if (!HOIST) load(r);
+    V xv[NV], gv[NV], kv[NV];
     #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) xv[i] = nx[i], gv[i] = ng[i];
+    const float mu = nmu, is = nis;
+    if (HOIST && r + step < rows) load(r + step);
+    if (skipg) {
+      #pragma unroll
+      for (int i = 0; i < NV; ++i)
+        kv[i] = *(const V*)(skipg + r * ldk + base[i]);
+    }
+    float s[2] = {0.f, 0.f};
+    #pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float ga[VE];
+      gammas(i, ga);
       #pragma unroll
       for (int j = 0; j < VE; ++j) {
         const float g = j >= skip[i] ? elem<VE>(gv[i], j) : 0.f;
         const float xh = (elem<VE>(xv[i], j) - mu) * is;
-        const float h = g * gm[i][j];
-        s1 += h;
-        s2 += j >= skip[i] ? h * xh : 0.f;
-        db[i][j] += g;
-        dg[i][j] += j >= skip[i] ? g * xh : 0.f;
+        const float h = g * ga[j];
+        s[0] += h;
+        s[1] += j >= skip[i] ? h * xh : 0.f;
+        if constexpr (SUMS) {
+          db[i][j] += g;
+          dg[i][j] += j >= skip[i] ? g * xh : 0.f;
+        }
       }
-    row_sum2<TPR>(s1, s2, red, turn);
-    const float c1 = s1 / n, c2 = s2 / n;
+    }
+    row_sum<TPR>(s, red, turn);
+    const float c1 = s[0] / n, c2 = s[1] / n;
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (skip[i] >= VE) continue;
+      float ga[VE];
+      gammas(i, ga);
       V o;
       #pragma unroll
       for (int j = 0; j < VE; ++j) {
         const float xh = (elem<VE>(xv[i], j) - mu) * is;
-        float d = is * (elem<VE>(gv[i], j) * gm[i][j] - c1 - xh * c2);
+        const float h = elem<VE>(gv[i], j) * ga[j];
+        float d = is * (h - c1 - xh * c2);
         if (skipg) d += elem<VE>(kv[i], j);
         if constexpr (VE == 1) o = (T)d;
         else o[j] = (T)d;
@@ -230,7 +316,8 @@ __global__ __launch_bounds__(ln_block(TPR)) void layernorm_bwd_kernel(
   }
   float* og = part ? part + (long)blockIdx.x * 2 * cols : dgamma;
   float* ob = part ? og + cols : dbeta;
-  if constexpr (TPR >= ln_block(TPR)) {
+  if constexpr (!SUMS) {
+  } else if constexpr (TPR >= ln_block(TPR)) {
     // one row group per block: each column has one owner
     #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -269,6 +356,51 @@ __global__ __launch_bounds__(ln_block(TPR)) void layernorm_bwd_kernel(
     for (int c = threadIdx.x; c < cols; c += blockDim.x) {
       og[c] = acc[c];
       ob[c] = acc[cols + c];
+    }
+  }
+}
+
+// The gradient sums alone, down the columns: a block takes 64 vectors of VE
+// columns and every gridDim.y-th group of four rows, a wave a row at a time.
+// The sums go to part [gridDim.y, 2, cols].
+template <typename T, int VE>
+__global__ __launch_bounds__(256) void layernorm_sums_kernel(
+    const T* __restrict__ dy, long ldy, const T* __restrict__ x, long ldx,
+    const float* __restrict__ mean, const float* __restrict__ invstd,
+    float* __restrict__ part, long rows, int cols) {
+  typedef typename RowVec<T, VE>::type V;
+  __shared__ float join[4][2][64 * VE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c0 = (blockIdx.x * 64 + lane) * VE;
+  const int base = min(c0, cols - VE);
+  float dg[VE] = {}, db[VE] = {};
+  #pragma unroll 2
+  for (long r = blockIdx.y * 4 + wave; r < rows; r += gridDim.y * 4) {
+    const V xv = *(const V*)(x + r * ldx + base);
+    const V gv = *(const V*)(dy + r * ldy + base);
+    const float mu = mean[r], is = invstd[r];
+    #pragma unroll
+    for (int j = 0; j < VE; ++j) {
+      const float g = elem<VE>(gv, j);
+      db[j] += g;
+      dg[j] += g * ((elem<VE>(xv, j) - mu) * is);
+    }
+  }
+  #pragma unroll
+  for (int j = 0; j < VE; ++j) {
+    join[wave][0][lane * VE + j] = dg[j];
+    join[wave][1][lane * VE + j] = db[j];
+  }
+  __syncthreads();
+  // a vector moved back at the row's end writes the columns that are its own
+  if (wave < 2 && c0 < cols) {
+    float* to = part + ((long)blockIdx.y * 2 + wave) * cols;
+    #pragma unroll
+    for (int j = 0; j < VE; ++j) {
+      float v = 0.f;
+      #pragma unroll
+      for (int w = 0; w < 4; ++w) v += join[w][wave][lane * VE + j];
+      if (base + j >= c0) to[base + j] = v;
     }
   }
 }
@@ -319,25 +451,64 @@ struct LnConfig {
                        (const T*)res, ldr, gamma, beta, (T*)y, ldy, (T*)sum,
                        lds, mean, invstd, rows, cols, eps);
   }
+  // blocks that run at once: one more round would wait for a whole one, and
+  // each has a set of sums to hand over
   static int blocks(long rows) {
-    const long most = TPR > 256 ? 512 : 1024;
+    const long most = TPR > 256 ? 256 : 768;
     return (int)min((rows + rpb - 1) / rpb, most);
+  }
+  // whether the gradient sums are taken along with dx: then 16 bytes a column
+  // and block are written and read, otherwise the two arrays read again
+  static bool along(long rows) {
+    if (TPR < 64) return true;
+    if (TPR == 1024 && NV * VE > 16) return false;
+    return blocks(rows) == 1 || rows * sizeof(T) > 8l * blocks(rows);
+  }
+  static int parts(long rows) {
+    if (!along(rows)) return (int)min((rows + 15) / 16, 64L);
+    const int n = blocks(rows);
+    return n > 1 ? n : 0;
+  }
+  template <bool SUMS>
+  static void dx_pass(const void* dy, long ldy, const void* x, long ldx,
+                      const void* skip, long ldk, const float* mean,
+                      const float* invstd, const float* gamma, void* dx,
+                      long ldd, float* part, float* dgamma, float* dbeta,
+                      long rows, int cols, hipStream_t s) {
+    const size_t lds = SUMS && TPR < ln_block(TPR) ? 8ul * cols : 0;
+    hipLaunchKernelGGL((layernorm_bwd_kernel<T, VE, TPR, NV, SUMS>),
+                       dim3(blocks(rows)), dim3(ln_block(TPR)), lds, s,
+                       (const T*)dy, ldy, (const T*)x, ldx, (const T*)skip, ldk,
+                       mean, invstd, gamma, (T*)dx, ldd, part, dgamma, dbeta,
+                       rows, cols);
   }
   static void bwd(const void* dy, long ldy, const void* x, long ldx,
                   const void* skip, long ldk, const float* mean,
                   const float* invstd, const float* gamma, void* dx, long ldd,
                   float* part, float* dgamma, float* dbeta, long rows,
                   int cols, hipStream_t s) {
-    const int grid = blocks(rows);
-    const size_t lds = TPR < ln_block(TPR) ? 8ul * cols : 0;
-    hipLaunchKernelGGL((layernorm_bwd_kernel<T, VE, TPR, NV>), dim3(grid),
-                       dim3(ln_block(TPR)), lds, s, (const T*)dy, ldy,
-                       (const T*)x, ldx, (const T*)skip, ldk, mean, invstd,
-                       gamma, (T*)dx, ldd, grid > 1 ? part : nullptr, dgamma,
-                       dbeta, rows, cols);
-    if (grid > 1)
+    const int n = parts(rows);
+    bool done = false;
+    if constexpr (TPR >= 64) {
+      if (!along(rows)) {
+        // the sums first: dx may be written where dy or x lie
+        hipLaunchKernelGGL((layernorm_sums_kernel<T, VE>),
+                           dim3((cols + 64 * VE - 1) / (64 * VE), n), dim3(256),
+                           0, s, (const T*)dy, ldy, (const T*)x, ldx, mean,
+                           invstd, part, rows, cols);
+        dx_pass<false>(dy, ldy, x, ldx, skip, ldk, mean, invstd, gamma, dx, ldd,
+                       nullptr, nullptr, nullptr, rows, cols, s);
+        done = true;
+      }
+    }
+    if constexpr (TPR < 1024 || NV * VE <= 16) {
+      if (!done)
+        dx_pass<true>(dy, ldy, x, ldx, skip, ldk, mean, invstd, gamma, dx, ldd,
+                      n ? part : nullptr, dgamma, dbeta, rows, cols, s);
+    }
+    if (n)
       hipLaunchKernelGGL(layernorm_join_kernel, dim3((2 * cols + 31) / 32),
-                         dim3(1024), 0, s, part, dgamma, dbeta, grid, cols);
+                         dim3(1024), 0, s, part, dgamma, dbeta, n, cols);
   }
 };
 
@@ -345,7 +516,7 @@ struct LnConfig {
 template <typename T, typename F>
 auto ln_pick(int cols, F f) {
   constexpr int VE = 16 / sizeof(T);
-  if (cols < VE) return f(LnConfig<T, 1, 8, 1>{});
+  if (cols < VE) return f(LnConfig<T, 1, 1, VE - 1>{});
   const int nv = (cols + VE - 1) / VE;
   if (nv <= 1) return f(LnConfig<T, VE, 1, 1>{});
   if (nv <= 2) return f(LnConfig<T, VE, 2, 1>{});
@@ -390,9 +561,7 @@ void launch_layernorm_fwd(int dtype, const void* x, long ldx, const void* res,
 
 // rows of the [n, 2, cols] workspace that the backward pass wants (0: none)
 int layernorm_bwd_parts(int dtype, long rows, int cols) {
-  const int n = ln_typed(dtype, cols,
-                         [&](auto cfg) { return cfg.blocks(rows); });
-  return n > 1 ? n : 0;
+  return ln_typed(dtype, cols, [&](auto cfg) { return cfg.parts(rows); });
 }
 
 void launch_layernorm_bwd(int dtype, const void* dy, long ldy, const void* x,
