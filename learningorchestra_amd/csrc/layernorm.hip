@@ -405,22 +405,25 @@ __global__ __launch_bounds__(256) void layernorm_sums_kernel(
   }
 }
 
-// column sums of part [n, width]: 32 columns a block, 32 threads to a column
+// column sums of part [n, 2 cols]: C columns a block, 1024 / C threads to a
+// column (8 for narrow sums, which would not fill the chip otherwise)
+template <int C>
 __global__ __launch_bounds__(1024) void layernorm_join_kernel(
     const float* __restrict__ part, float* __restrict__ dgamma,
     float* __restrict__ dbeta, int n, int cols) {
-  __shared__ float s[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  constexpr int R = 1024 / C;
+  __shared__ float s[R][C + 1];
+  const int tx = threadIdx.x % C, ty = threadIdx.x / C;
   const int width = 2 * cols;
-  const int c = blockIdx.x * 32 + tx;
+  const int c = blockIdx.x * C + tx;
   float a = 0.f;
   if (c < width) {
     // eight loads on their way at a time
-    for (int r0 = ty; r0 < n; r0 += 256) {
+    for (int r0 = ty; r0 < n; r0 += 8 * R) {
       float v[8];
       #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int r = r0 + 32 * i;
+        const int r = r0 + R * i;
         v[i] = r < n ? part[(long)r * width + c] : 0.f;
       }
       #pragma unroll
@@ -429,6 +432,14 @@ __global__ __launch_bounds__(1024) void layernorm_join_kernel(
   }
   s[ty][tx] = a;
   __syncthreads();
+  if constexpr (R > 32) {
+    if (ty < 32) {
+      #pragma unroll
+      for (int i = 32; i < R; i += 32) a += s[ty + i][tx];
+      s[ty][tx] = a;
+    }
+    __syncthreads();
+  }
   if (ty == 0 && c < width) {
     a = 0.f;
     #pragma unroll
@@ -454,7 +465,7 @@ struct LnConfig {
   // blocks that run at once: one more round would wait for a whole one, and
   // each has a set of sums to hand over
   static int blocks(long rows) {
-    const long most = TPR > 256 ? 256 : 768;
+    const long most = TPR > 256 ? 256 : TPR < 64 ? 1024 : 768;
     return (int)min((rows + rpb - 1) / rpb, most);
   }
   // whether the gradient sums are taken along with dx: then 16 bytes a column
@@ -506,8 +517,11 @@ struct LnConfig {
         dx_pass<true>(dy, ldy, x, ldx, skip, ldk, mean, invstd, gamma, dx, ldd,
                       n ? part : nullptr, dgamma, dbeta, rows, cols, s);
     }
-    if (n)
-      hipLaunchKernelGGL(layernorm_join_kernel, dim3((2 * cols + 31) / 32),
+    if (n && cols <= 256)
+      hipLaunchKernelGGL(layernorm_join_kernel<8>, dim3((2 * cols + 7) / 8),
+                         dim3(1024), 0, s, part, dgamma, dbeta, n, cols);
+    else if (n)
+      hipLaunchKernelGGL(layernorm_join_kernel<32>, dim3((2 * cols + 31) / 32),
                          dim3(1024), 0, s, part, dgamma, dbeta, n, cols);
   }
 };
