@@ -629,14 +629,14 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(NsProduct pr,
 // Up to 64 x 1024 or 32 x 2048: one block does the whole call, momentum and
 // norm included, with X in the registers of its eight waves.
 //
-// A wave owns groups of 32 columns. A lane's share of X serves as it is as an
-// operand of both products, because the order in which a sum is taken is free
-// as long as both operands follow it: the accumulator of X' = C X gives lane
+// A wave owns groups of 32 columns. A lane's share of X' = C X serves as it is
+// as an operand of the next product, because the order in which a sum is taken
+// is free as long as both operands follow it: the accumulator gives lane
 // (g, c) = (lane / 16, lane % 16) rows 16 b + 4 g + e of column c, and so the
 // sum over rows runs, in steps f of 32, over rows 32 f + 4 g + (0..3) and
-// 32 f + 16 + 4 g + (0..3); C is laid out in that order in LDS. Its transpose,
-// from the same operands swapped, is in the same way ready for X' X'^T. The
-// waves' shares of A meet in LDS, where C is made from it.
+// 32 f + 16 + 4 g + (0..3); C is laid out in that order in LDS. For X' X'^T a
+// group is turned in LDS, each wave in its own part, where the waves' shares
+// of A then meet and C is made from them.
 struct NsSmallSteps {
   NsStep st[kNsSmallSteps];
   int n;
@@ -733,9 +733,15 @@ struct Image {
 // rather than hold all of it in registers
 LO_DEVICE void keep_apart() { asm volatile("" ::: "memory"); }
 
+// a wave's part of LDS: its blocks of A (16 x 16 of the lower triangle, 1 KiB
+// each), or before those the group of X that it turns (16 MB rows of 36 words)
+template <int MB>
+constexpr int ns_small_part() {
+  return MB == 2 ? 32 * 36 * 4 : MB * (MB + 1) / 2 * 1024;
+}
 template <int MB>
 constexpr int ns_small_lds() {
-  return 2 * Image<MB>::BYTES + 8 * (MB * (MB + 1) / 2) * 1024;
+  return 2 * Image<MB>::BYTES + 8 * ns_small_part<MB>();
 }
 
 // 16 MB rows, NG groups of 32 columns a wave
@@ -747,7 +753,8 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
   constexpr int FB = MB / 2, TRI = MB * (MB + 1) / 2;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const Image<MB> imgA{lds}, imgC{lds + Image<MB>::BYTES};
-  f32x4* parts = (f32x4*)(lds + 2 * Image<MB>::BYTES);  // [8][TRI][64]
+  constexpr int PART = ns_small_part<MB>() / 16;
+  f32x4* parts = (f32x4*)(lds + 2 * Image<MB>::BYTES);  // [8][PART]
   __shared__ double red[8];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int g = lane >> 4, cl = lane & 15;
@@ -826,14 +833,6 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
   }
   for (int off = 32; off > 0; off >>= 1) acc2 += __shfl_xor(acc2, off);
   if (lane == 0) red[w] = acc2;
-  // C starts as the identity
-  for (int i = threadIdx.x; i < 16 * MB * 4 * MB; i += 512) {
-    const int c = i / (4 * MB), r = i % (4 * MB) * 4;
-    f32x4 v;
-    #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = r + e == c ? 1.f : 0.f;
-    imgC.put4(c, r >> 4, (r >> 2) & 3, v);
-  }
   __syncthreads();
   double total = 0.0;
   for (int i = 0; i < 8; ++i) total += red[i];
@@ -848,15 +847,30 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
       for (int f = 0; f < FB; ++f)
         x[i][h][f] = halves(u[i][h][2 * f] * f0, u[i][h][2 * f + 1] * f0, sx);
 
+  // C X of a group's columns
+  auto apply = [&](const Halves (&xi)[2][FB], f32x4 (&d)[2][MB]) {
+    #pragma unroll
+    for (int b = 0; b < MB; ++b) {
+      keep_apart();
+      d[0][b] = d[1][b] = f32x4{};
+      #pragma unroll
+      for (int f = 0; f < FB; ++f) {
+        const Halves c = imgC.get(b * 16 + cl, f, g);
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) mma3(d[h][b], c, xi[h][f]);
+      }
+    }
+  };
+  // a group of X as [rows][32 columns] words (hi below lo), 4 words between
+  // rows: no two lanes of a write meet in a bank
+  constexpr int PITCH = 36;
+  unsigned* turn = (unsigned*)(parts + w * PART);
+  static_assert(16 * MB * PITCH <= PART * 4 && TRI * 64 <= PART);
+
   for (int s = 0; s < steps.n; ++s) {
     const NsStep& k = steps.st[s];
-    // X <- C X, its scale from the last step's sc * sx to sx (the identity's
-    // is one), and A = X X^T of it
-    float scale = 1.f;
-    if (s > 0) {
-      const NsStep& last = steps.st[s - 1];
-      scale = last.sn / (last.sc * last.sx);
-    }
+    // X <- C X (but before the first C), its scale from the last step's
+    // sc * sx to sx, and A = X X^T of it
     f32x4 gram[MB][MB];
     #pragma unroll
     for (int a = 0; a < MB; ++a)
@@ -865,39 +879,57 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
     #pragma unroll
     for (int i = 0; i < NG; ++i) {
       if (w + 8 * i >= groups) continue;
-      Halves q[MB];  // rows of X', 32 columns
-      f32x4 d[2][MB];
-      #pragma unroll
-      for (int b = 0; b < MB; ++b) {
-        keep_apart();
-        f32x4 t[2] = {};
-        d[0][b] = d[1][b] = f32x4{};
+      if (s > 0) {
+        const NsStep& last = steps.st[s - 1];
+        const float scale = last.sn / (last.sc * last.sx);
+        f32x4 d[2][MB];
+        apply(x[i], d);
         #pragma unroll
-        for (int f = 0; f < FB; ++f) {
-          const Halves c = imgC.get(b * 16 + cl, f, g);
+        for (int h = 0; h < 2; ++h)
           #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            mma3(t[h], x[i][h][f], c);
-            mma3(d[h][b], c, x[i][h][f]);
+          for (int f = 0; f < FB; ++f)
+            x[i][h][f] = halves(d[h][2 * f], d[h][2 * f + 1], scale);
+      }
+      // only this wave's lanes meet here; LDS serves them in order
+      keep_apart();
+      #pragma unroll
+      for (int h = 0; h < 2; ++h)
+        #pragma unroll
+        for (int f = 0; f < FB; ++f)
+          #pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int row = f * 32 + (j >> 1) * 16 + g * 4 + (j & 1) * 2;
+            const unsigned hi = x[i][h][f].hi[j], lo = x[i][h][f].lo[j];
+            turn[row * PITCH + h * 16 + cl] =
+                __builtin_amdgcn_perm(lo, hi, 0x05040100);
+            turn[(row + 1) * PITCH + h * 16 + cl] =
+                __builtin_amdgcn_perm(lo, hi, 0x07060302);
           }
+      keep_apart();
+      Halves q[MB];  // rows of X, 32 columns
+      #pragma unroll
+      for (int a = 0; a < MB; ++a) {
+        const unsigned* row = turn + (a * 16 + cl) * PITCH + g * 4;
+        const u32x4 u0 = *(const u32x4*)row, u1 = *(const u32x4*)(row + 16);
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned even = j < 2 ? u0[2 * j] : u1[2 * j - 4];
+          const unsigned odd = j < 2 ? u0[2 * j + 1] : u1[2 * j - 3];
+          q[a].hi[j] = __builtin_amdgcn_perm(odd, even, 0x05040100);
+          q[a].lo[j] = __builtin_amdgcn_perm(odd, even, 0x07060302);
         }
-        q[b] = halves(t[0], t[1], scale);
       }
       #pragma unroll
       for (int a = 0; a < MB; ++a)
         #pragma unroll
         for (int b = 0; b <= a; ++b) mma3(gram[a][b], q[a], q[b]);
-      #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        #pragma unroll
-        for (int f = 0; f < FB; ++f)
-          x[i][h][f] = halves(d[h][2 * f], d[h][2 * f + 1], scale);
     }
+    keep_apart();
     #pragma unroll
     for (int a = 0; a < MB; ++a)
       #pragma unroll
       for (int b = 0; b <= a; ++b)
-        parts[(w * TRI + a * (a + 1) / 2 + b) * 64 + lane] = gram[a][b];
+        parts[w * PART + (a * (a + 1) / 2 + b) * 64 + lane] = gram[a][b];
     __syncthreads();
     // the waves' sums in their order
     const int used = min(groups, 8);
@@ -905,7 +937,7 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
       f32x4 v = {};
       #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i < used) v += parts[(i * TRI + t) * 64 + lane];
+        if (i < used) v += parts[i * PART + t * 64 + lane];
       int a = 0;
       while ((a + 1) * (a + 2) / 2 <= t) ++a;
       const int b = t - a * (a + 1) / 2;
@@ -943,17 +975,8 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
   #pragma unroll
   for (int i = 0; i < NG; ++i) {
     if (w + 8 * i >= groups) continue;
-    f32x4 d[2][MB] = {};
-    #pragma unroll
-    for (int b = 0; b < MB; ++b) {
-      keep_apart();
-      #pragma unroll
-      for (int f = 0; f < FB; ++f) {
-        const Halves c = imgC.get(b * 16 + cl, f, g);
-        #pragma unroll
-        for (int h = 0; h < 2; ++h) mma3(d[h][b], c, x[i][h][f]);
-      }
-    }
+    f32x4 d[2][MB];
+    apply(x[i], d);
     #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = (w + 8 * i) * 32 + h * 16 + cl;
