@@ -859,6 +859,7 @@ void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
               "out must be contiguous and of g's shape, type and device");
   const int64_t rows = g.size(1), cols = g.size(2);
   TORCH_CHECK(rows <= lo::kNsSide && cols <= lo::kNsSide, "sides end at ", lo::kNsSide);
+  TORCH_CHECK(eps >= 0, "eps must not be negative");
   const auto st = lo::ns_steps(coeffs);
   if (g.numel() == 0) return;
   const c10::DeviceGuard guard(g.device());
@@ -872,11 +873,14 @@ void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
     lo::NsGroup ng{};
     ng.one = mats[0];
     ng.src_step = rows * cols;
-    ng.count = (int)g.size(0);
-    lo::launch_newton_schulz_small(ng, shortest, longest, code, in,
-                                   st.data(), (int)st.size(), (float)eps, o,
-                                   stream());
-    check_launch("orthogonalize");
+    const int64_t most = 1 << 22;  // blocks of 512 threads in one launch
+    for (int64_t b0 = 0; b0 < g.size(0); b0 += most) {
+      ng.count = (int)std::min(most, g.size(0) - b0);
+      ng.one.src = b0 * rows * cols;
+      lo::launch_newton_schulz_small(ng, shortest, longest, code, in, st.data(),
+                                     (int)st.size(), (float)eps, o, stream());
+      check_launch("orthogonalize");
+    }
     return;
   }
   lo::NsNeeds n;
@@ -1006,6 +1010,7 @@ struct MuonPlan {
       TORCH_CHECK(t.device() == table.device(), "the plan is on ",
                   table.device());
     }
+    TORCH_CHECK(eps >= 0, "eps must not be negative");
     const auto st = lo::ns_steps(coeffs);
     const c10::DeviceGuard guard(table.device());
     // the step may run on another stream than the plan was made on

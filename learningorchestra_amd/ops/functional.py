@@ -372,8 +372,10 @@ def adam_ranges(ranges: AdamRanges, master: torch.Tensor, grad: torch.Tensor,
 NS_COEFFS = (3.4445, -4.7750, 2.0315)
 
 
-def _ns_coeffs(steps: int, coeffs) -> list:
+def _ns_coeffs(steps: int, coeffs, eps: float) -> list:
     """[a, b, c] per step, flat, from one triple or one triple per step."""
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
     if int(steps) != steps or not 1 <= steps <= 100:
         raise ValueError("Newton-Schulz takes 1 to 100 steps")
     rows = [coeffs] * int(steps) if len(coeffs) == 3 and not hasattr(
@@ -421,7 +423,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS,
     and type (it may be g). ``coeffs``: (a, b, c), or a triple for each step;
     such that grow singular values past 2^20 are refused. A zero matrix stays
     zero. A view that is not contiguous is copied first."""
-    flat = _ns_coeffs(steps, coeffs)
+    flat = _ns_coeffs(steps, coeffs, eps)
     if g.dim() < 2:
         raise ValueError("g must be a matrix or a batch of them")
     if g.dtype not in (torch.bfloat16, torch.float16, torch.float32):
@@ -471,6 +473,9 @@ class MuonPlan:
             self._native = require_ext().MuonPlan(
                 [list(t) for t in self.views], self.numel, str(dev))
 
+    def __reduce__(self):   # copies and pickles are plans of their own
+        return MuonPlan, (self.views, self.numel, str(self.device))
+
 
 def muon_step(plan: MuonPlan, master: torch.Tensor, grad: torch.Tensor,
               mom: torch.Tensor, mirror: torch.Tensor, lr: float,
@@ -485,7 +490,7 @@ def muon_step(plan: MuonPlan, master: torch.Tensor, grad: torch.Tensor,
 
     Elements outside the matrices stay as they are. Every rank that starts
     from the same values ends with the same values."""
-    flat = _ns_coeffs(steps, coeffs)
+    flat = _ns_coeffs(steps, coeffs, eps)
     if plan._native is not None:
         plan._native.step(master, grad, mom, mirror, lr, mu, wd, gscale,
                           nesterov, flat, eps)

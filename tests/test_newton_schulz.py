@@ -11,6 +11,7 @@ relative error of 2^-21 a step grows by at most s p'(s) / p(s) < 2.4 near one,
 2^-21 (1 + 2.4 + ... + 2.4^4) = 55 * 8 * 2^-24 < 512 * 2^-24. The output's own
 rounding adds half a step of every element.
 """
+import copy
 import math
 
 import pytest
@@ -29,7 +30,7 @@ def _exact(g, coeffs, eps):
     x = x / (torch.linalg.matrix_norm(x)[..., None, None] + eps)
     tall = x.shape[-2] > x.shape[-1]
     if tall:
-        x = x.mT
+        x = x.mT.contiguous()
     for a, b, c in coeffs:
         s = x @ x.mT.contiguous()
         x = a * x + (b * s + c * (s @ s)) @ x
@@ -37,7 +38,8 @@ def _exact(g, coeffs, eps):
 
 
 def _check(got, g, coeffs=(F.NS_COEFFS,) * 5, eps=1e-7):
-    g = g.cpu()
+    if g.numel() < 2_000_000:   # larger references stay on the GPU
+        g = g.cpu()
     flat = [v for t in coeffs for v in t]
     ref = _exact(g, coeffs, eps)
     f32 = F._newton_schulz_ref(g.float(), flat, eps).double()
@@ -46,7 +48,7 @@ def _check(got, g, coeffs=(F.NS_COEFFS,) * 5, eps=1e-7):
     tol = 8 * norm(f32 - ref) + (512 * U + half) * norm(ref) + 1e-12
     if g.dtype == torch.float16:   # steps below the normal range
         tol = tol + 2.0 ** -25 * math.sqrt(ref.shape[-1] * ref.shape[-2])
-    err = norm(got.double().cpu() - ref)
+    err = norm(got.double().to(ref.device) - ref)
     assert bool((err <= tol).all()), f"off by {(err / tol).max():.2f} tolerances"
 
 
@@ -78,8 +80,10 @@ def test_orthogonalize(device, dtype, m, n):
     _check(o, g)
 
 
-# both tile sizes, whole tiles and ragged ones, wide and tall, batches
-BIG = [(640, 1500), (1500, 640), (1100, 1130), (2050, 2100), (3, 128, 384),
+# all tile sizes with whole sums and split ones, what full rounds of the chip
+# leave over (2900 x 3000), ragged sides, wide and tall, batches
+BIG = [(256, 3136), (512, 3000), (5000, 65), (16, 512, 700), (2900, 3000),
+       (40, 300, 1030), (640, 1500), (1500, 640), (1100, 1130), (2050, 2100), (3, 128, 384),
        (2, 4, 90, 70), (64, 130, 260), (70, 257, 129), (256, 96, 30), (300, 20, 700)]
 
 
@@ -183,6 +187,8 @@ def test_orthogonalize_refusals(device):
             lambda: F.orthogonalize(g.long()),
             lambda: F.orthogonalize(g, steps=0),
             lambda: F.orthogonalize(g, steps=2.5),
+            lambda: F.orthogonalize(g, eps=-1e-3),
+            lambda: F.orthogonalize(g, eps=float("nan")),
             lambda: F.orthogonalize(g, steps=101),
             lambda: F.orthogonalize(g, coeffs=(1.0, 2.0)),
             lambda: F.orthogonalize(g, steps=3, coeffs=[CUBIC] * 2),
@@ -205,6 +211,22 @@ def test_workspace_in_groups():
     assert torch.equal(o[0], o[199]) and torch.equal(o[3], o[0])
     _check(o[0], one[0])
     _check(o[100], one[1])
+
+
+@pytest.mark.gpu
+def test_more_small_matrices_than_one_launch_takes():
+    """A row's direction does not change, and its length follows the
+    polynomial: from 1, five steps end at p(p(p(p(p(1)))))."""
+    n = (1 << 22) + 5
+    g = torch.randn(n, 1, 2, generator=torch.Generator("cuda").manual_seed(1),
+                    device="cuda")
+    o = F.orthogonalize(g, eps=0.0)
+    a, b, c = F.NS_COEFFS
+    p = 1.0
+    for _ in range(5):
+        p = a * p + b * p ** 3 + c * p ** 5
+    unit = g.double() / g.double().norm(dim=-1, keepdim=True)
+    assert (o.double() - p * unit).abs().max() <= 512 * U * p
 
 
 @pytest.mark.gpu
@@ -378,4 +400,42 @@ def test_muon_refusals(device):
     with pytest.raises((ValueError, RuntimeError)):
         F.muon_step(plan, *args, lr=0.1, steps=0)
     with pytest.raises((ValueError, RuntimeError)):
+        F.muon_step(plan, *args, lr=0.1, eps=-1.0)
+    with pytest.raises((ValueError, RuntimeError)):
         F.muon_step(plan, *args, lr=0.1, coeffs=(9.0, 9.0, 9.0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_copied_plan(device):
+    """A copy is a plan of its own that does the same."""
+    views, total, a = _arena(MODELS["mixed"], device)
+    b = {k: v.clone() for k, v in a.items()}
+    plan = F.MuonPlan(views, total, device)
+    for st, p in ((a, plan), (b, copy.deepcopy(plan))):
+        F.muon_step(p, st["master"], st["grad"], st["mom"], st["mirror"], **KW)
+    assert torch.equal(a["master"], b["master"])
+
+
+@pytest.mark.gpu
+def test_two_plans_on_two_streams():
+    """Steps of two plans at once, each on its own stream."""
+    views, total, a = _arena(MODELS["textcnn"], "cuda")
+    states = [a, {k: v.clone() for k, v in a.items()}]
+    want = {k: v.clone() for k, v in a.items()}
+    plans = [F.MuonPlan(views, total, "cuda") for _ in range(2)]
+    one = F.MuonPlan(views, total, "cuda")
+    for _ in range(3):
+        F.muon_step(one, want["master"], want["grad"], want["mom"],
+                    want["mirror"], **KW)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for s, p, st in zip(streams, plans, states):
+            with torch.cuda.stream(s):
+                F.muon_step(p, st["master"], st["grad"], st["mom"],
+                            st["mirror"], **KW)
+    torch.cuda.synchronize()
+    for st in states:
+        for k in want:
+            assert torch.equal(st[k], want[k]), k
