@@ -337,31 +337,34 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
                  : KIND == NS_POLY ? pl.a()
                                    : pl.y(pr.from);
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave >> 1, wc = wave & 1;
 
   // 1 KiB (8 rows of 128 bytes) an instruction; the 16-byte piece that lands
   // at place p of a row is piece p ^ (row & 7), which spreads a column of
-  // pieces over the banks
-  const long lane_off = (long)(wave * LOADS * 8 + lane / 8) * 2 * ld +
-                        ((lane % 8) ^ (lane / 8)) * 8;
-  P += (long)ti * T * 2 * ld + lane_off;
-  Q += (long)tj * T * 2 * ld + lane_off;
-  auto stage = [&](int kt) {
-    char* buf = lds + (kt - k0) / KB % S * (2 * KB * IMG) + wave * LOADS * 1024;
+  // pieces over the banks. Addresses are a scalar base and a lane's offset, and
+  // the loop below is unrolled over the S buffers: with one wave a SIMD, what
+  // is computed between the loads would be waited for.
+  const unsigned lane_off =
+      (unsigned)(lane / 8) * 4 * ld + ((lane % 8) ^ (lane / 8)) * 16;
+  const char* Pb = (const char*)(P + (long)(ti * T + wave * LOADS * 8) * 2 * ld);
+  const char* Qb = (const char*)(Q + (long)(tj * T + wave * LOADS * 8) * 2 * ld);
+  auto stage = [&](int buf, int kt) {
+    char* to = lds + buf * (2 * KB * IMG) + wave * LOADS * 1024;
+    auto load = [&](const char* from, char* at) {
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) unsigned int*)(from +
+                                                                  lane_off),
+          (__attribute__((address_space(3))) unsigned int*)at, 16, 0, 0);
+    };
     #pragma unroll
     for (int h = 0; h < KB; ++h)
       #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const long off = (long)i * 16 * ld + (kt + h) * 64;
-        char* to = buf + h * 2 * IMG + i * 1024;
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) unsigned int*)(P + off),
-            (__attribute__((address_space(3))) unsigned int*)to, 16, 0, 0);
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) unsigned int*)(Q + off),
-            (__attribute__((address_space(3))) unsigned int*)(to + IMG), 16, 0,
-            0);
+        const long off = (long)i * 32 * ld + (long)(kt + h) * 128;
+        load(Pb + off, to + h * 2 * IMG + i * 1024);
+        load(Qb + off, to + h * 2 * IMG + IMG + i * 1024);
       }
   };
   struct Frags {
@@ -371,8 +374,8 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
     return *(const f16x8*)(img + row * 128 +
                            ((half * 64 + (lane >> 4) * 16) ^ ((row & 7) << 4)));
   };
-  auto read = [&](int kt, Frags& s) {
-    const char* img = lds + ((kt - k0) / KB % S * KB + (kt - k0) % KB) * 2 * IMG;
+  auto read = [&](int buf, int h, Frags& s) {
+    const char* img = lds + (buf * KB + h) * 2 * IMG;
     #pragma unroll
     for (int i = 0; i < F; ++i) {
       const int row = i * 16 + (lane & 15);
@@ -431,25 +434,31 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
     else
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
-  for (int kt = k0; kt < k0 + (S - 1) * KB; kt += KB)
-    if (kt < k1) stage(kt);
-  Frags a, b;
+  #pragma unroll
+  for (int s = 0; s < S - 1; ++s)
+    if (k0 + s * KB < k1) stage(s, k0 + s * KB);
+  Frags even, odd;
   ready(k0 + (S - 2) * KB);
-  read(k0, a);
-  if (k0 + (S - 1) * KB < k1) stage(k0 + (S - 1) * KB);
-  auto step = [&](int kt, bool fresh, const Frags& now, Frags& next) {
-    if (kt + 1 < k1) {
-      if (fresh) ready(kt + 1 + (S - 2) * KB);
-      read(kt + 1, next);
-      if (fresh && kt + 1 + (S - 1) * KB < k1) stage(kt + 1 + (S - 1) * KB);
+  read(0, 0, even);
+  if (k0 + (S - 1) * KB < k1) stage(S - 1, k0 + (S - 1) * KB);
+  [&] {
+    for (int k = k0;; k += S * KB) {
+      #pragma unroll
+      for (int n = 0; n < S * KB; ++n) {
+        const int kt = k + n, s = n / KB, next = (n + 1) % (S * KB);
+        if (kt + 1 < k1) {
+          const bool fresh = next % KB == 0;
+          if (fresh) ready(kt + 1 + (S - 2) * KB);
+          read(next / KB, next % KB, n % 2 ? even : odd);
+          // k1 - k0 is a multiple of KB
+          if (fresh && kt + 1 + (S - 1) * KB < k1)
+            stage(s, kt + 1 + (S - 1) * KB);
+        }
+        add(n % 2 ? odd : even);
+        if (kt + 1 >= k1) return;
+      }
     }
-    add(now);
-  };
-  // k1 - k0 is a multiple of KB
-  for (int kt = k0; kt < k1; kt += 2) {
-    step(kt, KB == 1, a, b);
-    if (KB > 1 || kt + 1 < k1) step(kt + 1, true, b, a);
-  }
+  }();
   __syncthreads();  // the staging buffers are free from here on
 
   if (splits > 1) {
