@@ -125,27 +125,33 @@ inline bool ns_fit_block(int shortest, int longest) {
 }
 
 // What a tile size costs, in microseconds, fitted to launches of single
-// products with 3 to 784 tiles and 8 to 98 steps, to rank the choices by: a
-// launch with its first loads and its end; a step of 32 values of the sum on a
-// CU of its own, which the way to memory bounds (8, 16 and 32 KiB of operands
-// that other dies wrote, about 53 GB/s a CU); handing over the parts of a
-// split sum, for each part that the last block adds and for each part on the
+// products with 3 to 1300 tiles and 8 to 128 steps, to rank the choices by: a
+// launch with its first loads and its end; a step of 32 values of the sum (8,
+// 16 or 32 KiB of operands) in a block alone on its CU; a step and a block's
+// own start and end where several blocks share one; handing over the parts of
+// a split sum, for each part that the last block adds and for each part on the
 // chip. So 256 x 3136 took 232 us with every sum split, 150 us with only deep
-// ones split on 64 x 64 tiles, and takes 121 us with A and C on 32 x 32.
+// ones split on 64 x 64 tiles, and 115 us with A and C on 32 x 32; 512 x 512
+// 148 us on 64 x 64 tiles and 95 us on 32 x 32.
 struct NsCost {
   int tile;
-  double launch, step, join, add, part;
+  double launch, alone, step, block, join, add, part;
 };
-constexpr NsCost kNsCosts[] = {{32, 3.2, 0.15, 1.5, 0.3, 0.006},
-                               {64, 3.6, 0.306, 2.5, 0.4, 0.004},
-                               {128, 5.0, 1.0, 4.0, 1.2, 0.02}};
-constexpr double kNsBytes = 8.5e6;  // bytes a microsecond that all CUs load
+constexpr NsCost kNsCosts[] = {{32, 3.4, 0.10, 0.10, 0.35, 1.0, 0.3, 0.004},
+                               {64, 4.1, 0.21, 0.22, 1.0, 1.0, 0.5, 0.006},
+                               {128, 5.0, 1.0, 0.62, 2.0, 4.0, 1.2, 0.02}};
+constexpr int64_t kNsCus = 256;
 
 // the cost of one product over the matrices (copies of each), every sum cut
 // into parts of at most `most` steps; fills in how
 inline double ns_share(std::vector<NsMat>& mats, int64_t copies, int kind,
                        const NsCost& want, int64_t most) {
-  double longest = 0, bytes = 0, join = 0, parts = 0;
+  // small tiles of different matrices share fewer panels in the caches:
+  // ResNet-50's group takes 1276 us with A's on 128 x 128 and C's on 64 x 64
+  // tiles, 1317 us with both on 128 x 128, 1420 us with both on 64 x 64
+  const double apart = mats.size() > 1 && want.tile < 128 ? 1.3 : 1;
+  double longest = 0, sum = 0, join = 0, parts = 0;
+  int64_t blocks = 0;
   for (NsMat& m : mats) {
     const bool fits = m.mp % want.tile == 0 && m.np % want.tile == 0;
     const NsCost& c = fits ? want : kNsCosts[1];
@@ -155,14 +161,25 @@ inline double ns_share(std::vector<NsMat>& mats, int64_t copies, int kind,
     const int64_t s = std::min((depth + most - 1) / most, depth / 2);
     k.splits = (int)s;
     k.whole = s > 1 ? 0 : (int)tiles;
-    longest = std::max(longest, (double)depth / s * c.step);
-    bytes += (double)(tiles * copies * depth) * c.tile * 256;
+    const double steps = (double)depth / s;
+    longest = std::max(longest, steps * c.alone);
+    blocks += tiles * copies * s;
+    sum += (double)(tiles * copies * s) * (steps * c.step * apart + c.block);
     if (s > 1) {
       join = std::max(join, c.join + c.add * s);
       parts += c.part * (double)(tiles * copies * s);
     }
   }
-  return want.launch + std::max(longest, bytes / kNsBytes) + join + parts;
+  // a CU's share: whole blocks of the average length while those are few and
+  // alike (of different ones the short fill the gaps; and what is left over of
+  // a single matrix's large tiles is split, see ns_plan)
+  const bool even = blocks > 8 * kNsCus || mats.size() > 1 ||
+                    (want.tile == 128 && copies == 1);
+  const double share =
+      blocks <= kNsCus ? 0
+                       : (even ? (double)blocks : (double)ns_up(blocks, kNsCus)) /
+                             kNsCus * (sum / blocks);
+  return want.launch + std::max(longest, share) + join + parts;
 }
 
 // Shapes, and for each product the tiles and their sharing, of `copies` of
