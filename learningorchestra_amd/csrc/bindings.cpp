@@ -596,6 +596,15 @@ void adam_step(at::Tensor master, at::Tensor grad, at::Tensor m1, at::Tensor m2,
                   (float)wd, (float)gscale, stream());
 }
 
+// what an object keeps may be used on another stream than it was made on: its
+// memory is not given to others before this stream is done with it
+void used_here(std::initializer_list<at::Tensor> kept) {
+  for (const at::Tensor& t : kept) {
+    const c10::impl::VirtualGuardImpl impl(t.device().type());
+    if (t.numel()) t.record_stream(impl.getStream(t.device()));
+  }
+}
+
 // the same step on parts of the arena only: ranges [k, 2] (start, end), int64
 // on the GPU, the longest of them long
 void adam_ranges(at::Tensor master, at::Tensor grad, at::Tensor m1,
@@ -621,6 +630,7 @@ void adam_ranges(at::Tensor master, at::Tensor grad, at::Tensor m1,
               "ranges must be int64 [k, 2] on the arena's GPU");
   if (ranges.size(0) == 0 || longest <= 0) return;
   const c10::DeviceGuard guard(master.device());
+  used_here({ranges});
   lo::launch_adam(master.data_ptr(), grad.data_ptr(), m1.data_ptr(), m2.data_ptr(),
                   mirror.data_ptr(), step_dev.data_ptr(), ranges.data_ptr(),
                   (int)ranges.size(0), longest, master.numel(), (float)lr,
@@ -757,6 +767,24 @@ void check_rows(const at::Tensor& t, const at::Tensor& like, const char* name,
               out ? " must not overlap itself" : " has a negative row stride");
 }
 
+// out may be an input, or lie beside it (columns of one wider buffer, say), but
+// not be a part of it: other blocks would read rows that are written already
+void check_apart(const at::Tensor& out, const at::Tensor& in,
+                 const char* name) {
+  if (out.numel() == 0) return;
+  const int64_t rows = out.size(0), cols = out.size(1), size = out.itemsize();
+  const int64_t ldo = rows > 1 ? out.stride(0) : cols;
+  const int64_t ldi = rows > 1 ? in.stride(0) : cols;
+  const auto a = (int64_t)out.data_ptr(), b = (int64_t)in.data_ptr();
+  if (a == b && ldo == ldi) return;
+  const int64_t end_a = a + ((rows - 1) * ldo + cols) * size;
+  const int64_t end_b = b + ((rows - 1) * ldi + cols) * size;
+  if (end_a <= b || end_b <= a) return;
+  const int64_t row = ldo * size, off = ((a - b) % row + row) % row;
+  TORCH_CHECK(ldo == ldi && off >= cols * size && off <= row - cols * size,
+              name, " may be an input, but not overlap one in part");
+}
+
 void check_vec(const at::Tensor& t, const at::Tensor& like, int64_t n,
                const char* name) {
   check_f32(t, name);
@@ -793,10 +821,15 @@ void layernorm_fwd(at::Tensor x, at::Tensor gamma, at::Tensor beta, double eps,
   }
   TORCH_CHECK(!sum_out || residual, "sum_out needs a residual");
   if (residual) check_rows(*residual, x, "residual", false);
+  check_apart(out, x, "out");
+  if (residual) check_apart(out, *residual, "out");
   if (sum_out) {
     check_rows(*sum_out, x, "sum_out", true);
     TORCH_CHECK(rows == 0 || sum_out->data_ptr() != out.data_ptr(),
                 "out and sum_out must be two tensors");
+    check_apart(*sum_out, x, "sum_out");
+    check_apart(*sum_out, *residual, "sum_out");
+    check_apart(*sum_out, out, "sum_out");
   }
   if (rows == 0) return;
   const c10::DeviceGuard guard(x.device());
@@ -822,6 +855,9 @@ void layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor mean,
   check_rows(dy, x, "dy", false);
   check_rows(dx, x, "dx", true);
   if (dskip) check_rows(*dskip, x, "dskip", false);
+  check_apart(dx, x, "dx");
+  check_apart(dx, dy, "dx");
+  if (dskip) check_apart(dx, *dskip, "dx");
   check_vec(mean, x, rows, "mean");
   check_vec(invstd, x, rows, "invstd");
   check_vec(gamma, x, cols, "gamma");
@@ -862,6 +898,7 @@ void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
   TORCH_CHECK(eps >= 0, "eps must not be negative");
   const auto st = lo::ns_steps(coeffs);
   if (g.numel() == 0) return;
+  check_apart(out.view({1, -1}), g.view({1, -1}), "out");
   const c10::DeviceGuard guard(g.device());
   auto mats = lo::ns_plan({{rows, cols}}, g.size(0));
   const lo::NsInput in{g.data_ptr(), nullptr, 1.f, 0.f, 0};
@@ -1013,11 +1050,7 @@ struct MuonPlan {
     TORCH_CHECK(eps >= 0, "eps must not be negative");
     const auto st = lo::ns_steps(coeffs);
     const c10::DeviceGuard guard(table.device());
-    // the step may run on another stream than the plan was made on
-    const c10::impl::VirtualGuardImpl impl(table.device().type());
-    const c10::Stream now = impl.getStream(table.device());
-    for (const at::Tensor& t : {table, ws, sums, parts, slots})
-      if (t.numel()) t.record_stream(now);
+    used_here({table, ws, sums, parts, slots});
     const lo::NsInput in{grad.data_ptr(), mom.data_ptr<float>(), (float)gscale,
                          (float)mu, nesterov ? 1 : 0};
     const lo::NsOutput out{nullptr, master.data_ptr<float>(),

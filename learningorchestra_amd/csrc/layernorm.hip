@@ -25,8 +25,9 @@
 // Columns need not be a multiple of VE: the vector that would cross the row's
 // end is moved back to end with it, and the elements it shares with its
 // neighbour (skip of them) count only there. gfx950 loads 16 bytes from any
-// element-aligned address, so odd strides take the same path. A row's reads
-// all come before its writes, so an output may be one of the inputs.
+// element-aligned address, so odd strides take the same path. What a row's
+// results need is read before it is written, so an output may be one of the
+// inputs.
 
 #include "lo_common.h"
 
@@ -311,7 +312,19 @@ __global__ __launch_bounds__(ln_block(TPR)) void layernorm_bwd_kernel(
         if constexpr (VE == 1) o = (T)d;
         else o[j] = (T)d;
       }
-      *(V*)(dx + r * ldd + base[i]) = o;
+      T* to = dx + r * ldd + base[i];
+      if constexpr (VE > 1) {
+        // dx may lie where dskip does: another wave may have written the
+        // elements that a moved vector shares with its neighbour before this
+        // one's of dskip were read
+        if (skipg && skip[i] > 0) {
+          #pragma unroll
+          for (int j = 0; j < VE; ++j)
+            if (j >= skip[i]) to[j] = o[j];
+          continue;
+        }
+      }
+      *(V*)to = o;
     }
   }
   float* og = part ? part + (long)blockIdx.x * 2 * cols : dgamma;

@@ -140,6 +140,22 @@ LO_DEVICE void store4(T* p, long i, int n, const f32x4& v) {
   }
 }
 
+// X = U f 2^-e from the sum of U's squares: 1 / (norm + eps), so that neither
+// tiny nor huge updates leave fp32's range on the way
+struct NsNorm {
+  float f;
+  int e;
+  LO_DEVICE NsNorm(double squares, float eps) {
+    const double m = frexp(sqrt(squares) + (double)eps, &e);
+    f = (float)(1.0 / m);
+  }
+  LO_DEVICE f32x4 operator()(f32x4 u) const {
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = ldexpf(u[j], -e) * f;
+    return u;
+  }
+};
+
 // the update's elements, from the momentum that the step has brought forward
 template <typename T>
 LO_DEVICE f32x4 update4(const NsInput& in, long i, int n) {
@@ -215,14 +231,14 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup g, NsInput in,
   for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
   __syncthreads();
-  const float norm = (float)sqrt(red[0] + red[1] + red[2] + red[3]);
-  const float f = 1.f / (norm + eps);
+  const NsNorm norm(red[0] + red[1] + red[2] + red[3], eps);
   #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int a = i * 16 + threadIdx.x / 16;
+    v[i] = norm(v[i]);
     #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float x = v[i][j] * f * scale;
+      const float x = v[i][j] * scale;
       if (tall) tile[b + j][a] = x;
       else tile[a][b + j] = x;
     }
@@ -845,7 +861,7 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
   __syncthreads();
   double total = 0.0;
   for (int i = 0; i < 8; ++i) total += red[i];
-  const float f0 = 1.f / ((float)sqrt(total) + eps);
+  const NsNorm norm(total, eps);
   const float sx = steps.st[0].sx;
   Halves x[NG][2][FB];  // [group][16 columns][32 rows]
   #pragma unroll
@@ -854,7 +870,7 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(NsGroup gr, NsInput in
     for (int h = 0; h < 2; ++h)
       #pragma unroll
       for (int f = 0; f < FB; ++f)
-        x[i][h][f] = halves(u[i][h][2 * f] * f0, u[i][h][2 * f + 1] * f0, sx);
+        x[i][h][f] = halves(norm(u[i][h][2 * f]), norm(u[i][h][2 * f + 1]), sx);
 
   // C X of a group's columns
   auto apply = [&](const Halves (&xi)[2][FB], f32x4 (&d)[2][MB]) {

@@ -340,6 +340,9 @@ class AdamRanges:
             if not 0 <= a < b <= numel or a % 8 or b % 8:
                 raise ValueError("ranges must be multiples of 8 within the "
                                  "arena")
+        ordered = sorted(self.ranges)
+        if any(a[1] > b[0] for a, b in zip(ordered, ordered[1:])):
+            raise ValueError("ranges must not overlap")
         self.numel = int(numel)
         self.longest = max((b - a for a, b in self.ranges), default=0)
         self._table = torch.tensor(self.ranges, dtype=torch.int64,
@@ -370,6 +373,7 @@ def adam_ranges(ranges: AdamRanges, master: torch.Tensor, grad: torch.Tensor,
 # quintic whose five steps bring singular values from about 0.005 up to
 # between 0.7 and 1.2: the steepest start, at the price of not settling at 1
 NS_COEFFS = (3.4445, -4.7750, 2.0315)
+NS_SIDE = 1 << 20       # the longest side that a matrix may have
 
 
 def _ns_coeffs(steps: int, coeffs, eps: float) -> list:
@@ -405,7 +409,8 @@ def _newton_schulz_ref(x: torch.Tensor, flat: list, eps: float) -> torch.Tensor:
     tall = x.shape[-2] > x.shape[-1]
     if tall:
         x = x.transpose(-2, -1)
-    x = x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps)
+    x = x.double()
+    x = (x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps)).float()
     for i in range(0, len(flat), 3):
         a, b, c = flat[i:i + 3]
         gram = x @ x.transpose(-2, -1)
@@ -428,12 +433,16 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS,
         raise ValueError("g must be a matrix or a batch of them")
     if g.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError("g must be bf16, fp16 or fp32")
+    if max(g.shape[-2:]) > NS_SIDE:
+        raise ValueError(f"a matrix's sides end at {NS_SIDE}")
     if out is None:
         out = torch.empty_like(g, memory_format=torch.contiguous_format)
     if out.shape != g.shape or out.dtype != g.dtype or out.device != g.device \
             or not out.is_contiguous():
         raise ValueError("out must be contiguous and of g's shape, type and "
                          "device")
+    if g.is_contiguous() and not _apart(out.view(1, -1), g.view(1, -1)):
+        raise ValueError("out may be g, but not overlap it in part")
     if _is_gpu(g):
         three = (-1 if g.numel() else 0, g.shape[-2], g.shape[-1])
         require_ext().orthogonalize(g.contiguous().view(three),
@@ -463,6 +472,8 @@ class MuonPlan:
             if off < end or off % 8 or m < 1 or n < 1:
                 raise ValueError("matrices must start on a multiple of 8 "
                                  "elements and not overlap")
+            if max(m, n) > NS_SIDE:
+                raise ValueError(f"a matrix's sides end at {NS_SIDE}")
             end = off + m * n
         if end > self.numel:
             raise ValueError("a matrix ends outside the arena")
@@ -696,13 +707,13 @@ def layernorm_fwd(x2d: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor,
     and, for training, mean and invstd (fp32 [M]). ``residual`` [M, C] is
     added first; the sum, rounded to x2d's type, is what gets normalised and
     goes to ``sum_out`` (the backward pass's x2d). ``out`` and ``sum_out`` may
-    be one of the inputs."""
+    each be one of the inputs, but not a part of one."""
     if _is_gpu(x2d):
         require_ext().layernorm_fwd(x2d, gamma, beta, eps, out, mean, invstd,
                                     residual, sum_out)
         return
     _check_layernorm(x2d, (out, residual, sum_out), (gamma, beta),
-                     (mean, invstd))
+                     (mean, invstd), (out, sum_out))
     if (mean is None) != (invstd is None):
         raise RuntimeError("mean and invstd come together")
     if sum_out is not None and residual is None:
@@ -730,13 +741,14 @@ def layernorm_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, mean: torch.Tensor,
     ``sum_out``) and its mean/invstd. Writes dgamma, dbeta (fp32 [C],
     overwritten; the same sums on every run) and dx. ``dskip`` [M, C], the
     gradient that reaches the sum past the norm, is added to dx, which then is
-    the gradient of x and of the residual alike."""
+    the gradient of x and of the residual alike. ``dx`` may be dy2d, x2d or
+    dskip, but not a part of one."""
     if _is_gpu(x2d):
         require_ext().layernorm_bwd(dy2d, x2d, mean, invstd, gamma, dgamma,
                                     dbeta, dx, dskip)
         return
     _check_layernorm(x2d, (dy2d, dx, dskip), (gamma, dgamma, dbeta),
-                     (mean, invstd))
+                     (mean, invstd), (dx,))
     g = dy2d.float()
     xhat = (x2d.float() - mean.view(-1, 1)) * invstd.view(-1, 1)
     h = g * gamma
@@ -749,7 +761,20 @@ def layernorm_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, mean: torch.Tensor,
     dx.copy_(d.to(dx.dtype))
 
 
-def _check_layernorm(x, rows, vecs, stats) -> None:
+def _apart(out: torch.Tensor, x: torch.Tensor) -> bool:
+    # out is x, or shares no element with it, or lies beside it in wider rows
+    if not out.numel() or out.device != x.device:
+        return True
+    (rows, cols), size = out.shape, out.element_size()
+    lo, li = (t.stride(0) if rows > 1 else cols for t in (out, x))
+    a, b = out.data_ptr(), x.data_ptr()
+    if (a, lo) == (b, li) or a + ((rows - 1) * lo + cols) * size <= b \
+            or b + ((rows - 1) * li + cols) * size <= a:
+        return True
+    return lo == li and cols * size <= (a - b) % (lo * size) <= (lo - cols) * size
+
+
+def _check_layernorm(x, rows, vecs, stats, outs) -> None:
     # the CPU path refuses what the kernels' bindings refuse
     if x.dim() != 2 or not 1 <= x.shape[1] <= 32768:
         raise RuntimeError("layer norm takes [rows, 1 to 32768 columns]")
@@ -766,6 +791,13 @@ def _check_layernorm(x, rows, vecs, stats) -> None:
                                   or t.device != x.device):
                 raise RuntimeError(f"statistics and parameters must be fp32 "
                                    f"with {n} values")
+    for o in outs:
+        if o is not None and o.shape[0] > 1 and o.stride(0) < o.shape[1]:
+            raise RuntimeError("an output must not overlap itself")
+        for t in (x, *rows):
+            if None not in (o, t) and o is not t and not _apart(o, t):
+                raise RuntimeError("an output may be an input, but not overlap "
+                                   "one in part")
 
 
 # ------------------------------------------------------------ residual add

@@ -230,6 +230,45 @@ def test_in_place(device, cols):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("cols", [5, 96, 516, 2051, 4099, 8195])
+@pytest.mark.parametrize("onto", ["x", "dskip"])
+def test_backward_onto_its_inputs(device, cols, onto):
+    """The last vector of a row shares elements with its neighbour, at 516 and
+    the wider ones across waves."""
+    d = _data(300, cols, torch.bfloat16, device)
+    s, o = _forward(d, False)
+    g = _backward(s, o, d, True)
+    e = {"x": s.clone(), "dskip": d["dskip"].clone()}
+    dg, db = torch.empty_like(d["gamma"]), torch.empty_like(d["beta"])
+    F.layernorm_bwd(d["dy"], e["x"], o["mean"], o["invstd"], d["gamma"], dg,
+                    db, e[onto], dskip=e["dskip"])
+    assert torch.equal(e[onto], g["dx"])
+    assert torch.equal(dg, g["dgamma"]) and torch.equal(db, g["dbeta"])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_outputs_that_overlap_an_input(device):
+    """Columns beside the input's in one buffer are taken, parts of it not."""
+    d = _data(8, 24, torch.float32, device)
+    s, o = _forward(d, False)
+    buf = torch.zeros(10, 50, device=device)
+    x, beside = buf[:8, :24], buf[1:9, 25:49]
+    x.copy_(d["x"])
+    F.layernorm_fwd(x, d["gamma"], d["beta"], EPS, beside)
+    assert torch.equal(beside, o["y"]) and torch.equal(x, d["x"])
+    flat = buf.view(-1)[:192].view(8, 24)
+    keep = buf.clone()
+    for x, bad in ((x, buf[1:9, :24]), (buf[1:9, :24], x), (x, buf[:8, 1:25]),
+                   (buf[1:9, 5:29], buf[:8, 26:50]), (x, flat), (flat, x)):
+        with pytest.raises(RuntimeError):
+            F.layernorm_fwd(x, d["gamma"], d["beta"], EPS, bad)
+        with pytest.raises(RuntimeError):
+            F.layernorm_bwd(d["dy"], x, o["mean"], o["invstd"], d["gamma"],
+                            d["gamma"].clone(), d["beta"].clone(), bad)
+        assert torch.equal(buf, keep)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("cols", [12, 130, 1030])
 def test_far_mean_and_constant_rows(device, cols):
     """A mean a thousand times the spread keeps its digits (the second sum is

@@ -122,6 +122,13 @@ def test_captured_steps():
     assert int(captured.t) == 4
 
 
+def test_ranges_do_not_overlap():
+    for bad in ([(0, 16), (8, 24)], [(8, 24), (0, 16)], [(0, 8), (0, 8)]):
+        with pytest.raises(ValueError):
+            F.AdamRanges(bad, 64, "cpu")
+    F.AdamRanges([(8, 24), (0, 8)], 64, "cpu")
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_ranges_refusals(device):
     for bad in ([(0, 12)], [(4, 16)], [(16, 8)], [(0, 72)], [(-8, 8)]):

@@ -145,6 +145,44 @@ def test_scales_beyond_fp32_squares(scale):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(50, 60), (130, 70)])
+@pytest.mark.parametrize("power", [-140, 123])
+def test_norms_out_of_range(device, shape, power):
+    """Whole numbers times a power of two, the norm (or what divides by it)
+    beyond fp32: the scale leaves no trace."""
+    gen = torch.Generator().manual_seed(9)
+    g = torch.randint(-15, 16, shape, generator=gen).float().to(device)
+    far = torch.ldexp(g.double(), torch.tensor(power)).float()
+    assert torch.equal(torch.ldexp(far.double(), torch.tensor(-power)).float(), g)
+    assert torch.equal(F.orthogonalize(far, eps=0.0),
+                       F.orthogonalize(g, eps=0.0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_outputs_that_overlap_the_input(device):
+    buf = _matrix((1, 5 * 6 * 8), device=device).view(-1)
+    g = buf[:4 * 48].view(4, 6, 8)
+    keep = buf.clone()
+    with pytest.raises(ValueError):
+        F.orthogonalize(g, out=buf[48:].view(4, 6, 8))
+    with pytest.raises(ValueError):
+        F.orthogonalize(g[1:], out=buf[8:8 + 3 * 48].view(3, 6, 8))
+    assert torch.equal(buf, keep)
+    want = F.orthogonalize(g[:2])
+    F.orthogonalize(g[:2], out=g[2:])
+    assert torch.equal(g[2:], want) and torch.equal(g[:2].reshape(-1), keep[:96])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sides_end(device):
+    for m, n in ((1, 2 ** 20 + 1), (2 ** 20 + 1, 1)):
+        with pytest.raises(ValueError):
+            F.orthogonalize(torch.zeros(m, n, device=device))
+        with pytest.raises(ValueError):
+            F.MuonPlan([(0, m, n)], 2 ** 20 + 8, device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_zero_and_bad_matrices_stay_alone(device):
     g = _matrix((4, 70, 40), device=device)
     want = F.orthogonalize(g)
