@@ -14,12 +14,17 @@
 // hi hi + hi lo + lo hi in fp32 accumulators: 1.9e-6 off where fp32 arithmetic
 // ends at 1.8e-6, at three fp16 matrix instructions instead of fp32's sixteen.
 //
-// Layout. A row holds 32 hi, then 32 lo values in turn, so that one 128-byte
-// line of a row feeds one 16x16x32 instruction of each kind. X is kept by rows
-// and, as Y, by columns: then every product is rows times rows,
-//   A = X X^T,  A A^T (A is symmetric),  X' = C Y^T,
-// and A and C, being symmetric, are computed on one triangle of tiles and
-// written to both. Sides are padded with zeros to whole tiles.
+// Layout. 32 columns of a row are a 128-byte line, 32 hi values, then 32 lo
+// ones, which feeds one 16x16x32 instruction of each kind; the lines of 32
+// columns lie together, row after row, so that all that a tile takes for a
+// step of its sum is one piece of memory (4096 x 4096 took 3 % longer with a
+// row's lines together). A = X X^T and A A^T (A is symmetric) are rows times
+// rows; X' = C X takes columns of X, which LDS turns as they are read
+// (ds_read_b64_tr_b16). With a second copy of X, by columns, to write and read
+// instead, 16 x 512 x 2048 took 742 us in place of 644, ResNet-50's matrices
+// 1290 in place of 1126. A and C, being symmetric, are computed on one
+// triangle of tiles and written to both. Sides are padded with zeros to whole
+// tiles.
 //
 // Sharing out. A call works on a group of matrices at once: a block finds its
 // matrix and tile in a table made with the plan, or by arithmetic for a batch
@@ -40,6 +45,7 @@ namespace {
 typedef _Float16 f16;
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef __fp16 h16x4 __attribute__((ext_vector_type(4)));  // the builtin's
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -50,10 +56,9 @@ struct Quad {
   typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
 };
 
-// element (row, k) of a split matrix with ld values a row; its lo half is 32
-// further
-LO_DEVICE long split_at(long row, int k, int ld) {
-  return row * 2 * ld + (k >> 5) * 64 + (k & 31);
+// element (row, k) of a split matrix of so many rows; its lo half is 32 further
+LO_DEVICE long split_at(int row, int k, int rows) {
+  return ((long)(k >> 5) * rows + row) * 64 + (k & 31);
 }
 
 LO_DEVICE void split(float v, f16& hi, f16& lo) {
@@ -94,15 +99,13 @@ LO_DEVICE NsMat find(const NsGroup& g, const NsBlock* __restrict__ table,
   return m;
 }
 
-// a matrix's workspace: X and Y, twice (a step reads one pair and writes the
-// other), A, C
+// a matrix's workspace: X twice (a step reads one and writes the other), A, C
 struct Planes {
   f16* w;
   long n, a_;
-  LO_DEVICE f16* x(int i) const { return w + 2 * i * n; }
-  LO_DEVICE f16* y(int i) const { return w + (2 * i + 1) * n; }
-  LO_DEVICE f16* a() const { return w + 4 * n; }
-  LO_DEVICE f16* c() const { return w + 4 * n + a_; }
+  LO_DEVICE f16* x(int i) const { return w + i * n; }
+  LO_DEVICE f16* a() const { return w + 2 * n; }
+  LO_DEVICE f16* c() const { return w + 2 * n + a_; }
 };
 
 template <typename M>  // NsMat or NsTask
@@ -202,7 +205,7 @@ __global__ __launch_bounds__(256) void ns_momentum_kernel(NsGroup g,
     g.slots[i] = 0;
 }
 
-// X and Y from the update: 64 x 64 elements a block
+// X from the update: 64 x 64 elements a block
 template <typename T>
 __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup g, NsInput in,
                                                        float scale, float eps) {
@@ -245,25 +248,19 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup g, NsInput in,
   }
   __syncthreads();
   const int r = threadIdx.x >> 2, k = (threadIdx.x & 3) * 16;
-  f16* ox = p.x(0) + split_at(r0 + r, c0 + k, m.np);
-  f16* oy = p.y(0) + split_at(c0 + r, r0 + k, m.mp);
+  f16* ox = p.x(0) + split_at(r0 + r, c0 + k, m.mp);
   #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    f16x8 xh, xl, yh, yl;
+    f16x8 xh, xl;
     #pragma unroll
     for (int j = 0; j < 8; ++j) {
       f16 hi, lo;
       split(tile[r][k + h * 8 + j], hi, lo);
       xh[j] = hi;
       xl[j] = lo;
-      split(tile[k + h * 8 + j][r], hi, lo);
-      yh[j] = hi;
-      yl[j] = lo;
     }
     *(f16x8*)(ox + h * 8) = xh;
     *(f16x8*)(ox + h * 8 + 32) = xl;
-    *(f16x8*)(oy + h * 8) = yh;
-    *(f16x8*)(oy + h * 8 + 32) = yl;
   }
 }
 
@@ -272,7 +269,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup g, NsInput in,
 struct NsProduct {
   const NsTask* tasks;  // or null: equal matrices
   void* ws;
-  int from;                 // the X and Y that the step reads
+  int from;                 // the X that the step reads
   int mp, np, tile;         // equal matrices: their shape,
   int blocks, whole, splits, count;  // blocks of one, and how shared out,
   long ws_step, part_step;  // and their spacing
@@ -345,42 +342,59 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
   const Planes pl = planes(t, pr.ws);
   const int ti = t.ti, tj = t.tj, splits = t.splits, slice = t.slice;
   const int k0 = t.k0, k1 = t.k1;
-  const int ld = KIND == NS_GRAM ? t.np : t.mp;  // values a row of operands
   const f16* P = KIND == NS_GRAM   ? pl.x(pr.from)
                  : KIND == NS_POLY ? pl.a()
                                    : pl.c();
-  const f16* Q = KIND == NS_GRAM   ? pl.x(pr.from)
-                 : KIND == NS_POLY ? pl.a()
-                                   : pl.y(pr.from);
+  const f16* Q = KIND == NS_POLY ? pl.a() : pl.x(pr.from);
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave >> 1, wc = wave & 1;
 
-  // 1 KiB (8 rows of 128 bytes) an instruction; the 16-byte piece that lands
-  // at place p of a row is piece p ^ (row & 7), which spreads a column of
-  // pieces over the banks. Addresses are a scalar base and a lane's offset, and
-  // the loop below is unrolled over the S buffers: with one wave a SIMD, what
-  // is computed between the loads would be waited for.
-  const unsigned lane_off =
-      (unsigned)(lane / 8) * 4 * ld + ((lane % 8) ^ (lane / 8)) * 16;
-  const char* Pb = (const char*)(P + (long)(ti * T + wave * LOADS * 8) * 2 * ld);
-  const char* Qb = (const char*)(Q + (long)(tj * T + wave * LOADS * 8) * 2 * ld);
+  // 1 KiB (8 lines) an instruction; the 16-byte piece that lands at place p of
+  // line l is piece p ^ (l & 7), which spreads a column of pieces over the
+  // banks. Addresses are a scalar base and a lane's offset, and the loop below
+  // is unrolled over the S buffers: with one wave a SIMD, what is computed
+  // between the loads would be waited for.
+  // APPLY's Q is 32 rows of X and T of its columns, an image of 32 lines for
+  // each 32 columns. There 4 lanes read 32 bytes of a line, 8 lines (0..3 and
+  // 8..11, say) at once: piece p lands at p ^ 2 ((l / 2 & 1) + 2 (l / 8 & 1)).
+  const unsigned lane_p = lane / 8 * 128 + ((lane % 8) ^ (lane / 8)) * 16;
+  const unsigned lane_q =
+      KIND != NS_APPLY
+          ? lane_p
+          : lane / 8 * 128 + ((lane % 8) ^ (lane / 8 & 2) ^ (wave & 1) * 4) * 16;
+  const long panel = (long)t.mp * 128;  // bytes of 32 columns
+  const char* Pb = (const char*)P + (ti * T + wave * LOADS * 8) * 128l;
+  const char* Qb = KIND != NS_APPLY
+                       ? (const char*)Q + (tj * T + wave * LOADS * 8) * 128l
+                       : (const char*)Q + tj * (T / 32) * panel + wave * 1024;
+  const unsigned lds_at =
+      (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
   auto stage = [&](int buf, int kt) {
-    char* to = lds + buf * (2 * KB * IMG) + wave * LOADS * 1024;
-    auto load = [&](const char* from, char* at) {
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) unsigned int*)(from +
-                                                                  lane_off),
-          (__attribute__((address_space(3))) unsigned int*)at, 16, 0, 0);
+    const unsigned to = lds_at + buf * (2 * KB * IMG);
+    // Written out, since before a ds_read_b64_tr_b16 the compiler waits for
+    // all loads to LDS that it knows of. These have no result in registers;
+    // `ready` waits for them.
+    auto load = [&](const char* from, unsigned lane_at, unsigned at) {
+      asm volatile(
+          "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at),
+          "v"(lane_at), "s"(from)
+          : "m0", "memory");
     };
     #pragma unroll
     for (int h = 0; h < KB; ++h)
       #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const long off = (long)i * 32 * ld + (long)(kt + h) * 128;
-        load(Pb + off, to + h * 2 * IMG + i * 1024);
-        load(Qb + off, to + h * 2 * IMG + IMG + i * 1024);
+        const unsigned p = to + h * 2 * IMG;
+        load(Pb + (kt + h) * panel + i * 1024, lane_p,
+             p + (wave * LOADS + i) * 1024);
+        if constexpr (KIND == NS_APPLY)
+          load(Qb + (kt + h) * 4096l + i * panel, lane_q,
+               p + IMG + (i * 4 + wave) * 1024);
+        else
+          load(Qb + (kt + h) * panel + i * 1024, lane_q,
+               p + IMG + (wave * LOADS + i) * 1024);
       }
   };
   struct Frags {
@@ -390,19 +404,41 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
     return *(const f16x8*)(img + row * 128 +
                            ((half * 64 + (lane >> 4) * 16) ^ ((row & 7) << 4)));
   };
+  // columns i*16.. of APPLY's Q: of 16 lanes, lane l names four columns of row
+  // l / 4, and gets column l of the four rows
+  const int q_row = (lane >> 4) * 8 + (lane >> 2 & 3);
+  const int q_at = q_row * 128 + (lane & 3) * 8 +
+                   ((lane >> 3 & 1) + (lane >> 4 & 1) * 2) * 32;
+  auto turned = [&](const char* img, int i, int half) {
+    const int col = wc * W + i * 16;
+    const char* at = img + (col >> 5) * 4096 +
+                     (q_at ^ ((half * 2 + (col >> 4 & 1)) * 32));
+    f16x8 v;
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f16x4 four = __builtin_bit_cast(
+          f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                     (__attribute__((address_space(3))) h16x4*)(at + h * 512)));
+      #pragma unroll
+      for (int j = 0; j < 4; ++j) v[h * 4 + j] = four[j];
+    }
+    return v;
+  };
+  auto frag_q = [&](const char* img, int i, int half) {
+    if constexpr (KIND == NS_APPLY) return turned(img, i, half);
+    else return frag(img, wc * W + i * 16 + (lane & 15), half);
+  };
   auto read = [&](int buf, int h, Frags& s) {
     const char* img = lds + (buf * KB + h) * 2 * IMG;
     #pragma unroll
     for (int i = 0; i < F; ++i) {
-      const int row = i * 16 + (lane & 15);
-      s.ph[i] = frag(img, wr * W + row, 0);
-      s.qh[i] = frag(img + IMG, wc * W + row, 0);
+      s.ph[i] = frag(img, wr * W + i * 16 + (lane & 15), 0);
+      s.qh[i] = frag_q(img + IMG, i, 0);
     }
     #pragma unroll
     for (int i = 0; i < F; ++i) {
-      const int row = i * 16 + (lane & 15);
-      s.ql[i] = frag(img + IMG, wc * W + row, 1);
-      s.pw[i] = frag(img, wr * W + row, 1);
+      s.ql[i] = frag_q(img + IMG, i, 1);
+      s.pw[i] = frag(img, wr * W + i * 16 + (lane & 15), 1);
     }
   };
   f32x4 acc[F][F] = {};
@@ -617,8 +653,6 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
     f16* rows = KIND == NS_GRAM   ? pl.a()
                 : KIND == NS_POLY ? pl.c()
                                   : pl.x(pr.from ^ 1);
-    f16* cols = KIND == NS_APPLY ? pl.y(pr.from ^ 1) : rows;
-    const int ldr = KIND == NS_APPLY ? t.np : t.mp;
     #pragma unroll 4
     for (int idx = lane; idx < W * W / 8; idx += 64) {
       int r, c;
@@ -626,13 +660,13 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
       f16x8 hi, lo;
       along_row(idx, r, c, a, b);
       unpack8(a, b, hi, lo);
-      f16* to = rows + split_at(rw + r, cw + c, ldr);
+      f16* to = rows + split_at(rw + r, cw + c, t.mp);
       *(f16x8*)to = hi;
       *(f16x8*)(to + 32) = lo;
-      if (KIND == NS_APPLY || ti != tj) {
+      if (KIND != NS_APPLY && ti != tj) {  // the other triangle
         along_col(idx, r, c, a, b);
         unpack8(a, b, hi, lo);
-        to = cols + split_at(cw + c, rw + r, t.mp);
+        to = rows + split_at(cw + c, rw + r, t.mp);
         *(f16x8*)to = hi;
         *(f16x8*)(to + 32) = lo;
       }

@@ -235,7 +235,7 @@ inline void ns_place(std::vector<NsMat>& mats, NsNeeds& sum) {
   for (NsMat& m : mats) {
     m.ws = sum.halfs;
     m.sum = (int)sum.chunks;
-    sum.halfs += 8l * m.mp * m.np + 4l * m.mp * m.mp;
+    sum.halfs += 4l * m.mp * m.np + 4l * m.mp * m.mp;
     sum.chunks += m.chunks;
     sum.splits += (int64_t)(m.mp / 64) * (m.np / 64);
     for (int k = 0; k < NS_KINDS; ++k) {

@@ -457,7 +457,7 @@ class MuonPlan:
     """What ``muon_step`` keeps between steps for the weight matrices of one
     flat arena of ``numel`` elements: ``views`` lists them as (offset, rows,
     cols), offsets being multiples of 8 as ParamArena's are. On a GPU it owns
-    the kernels' tables and their workspace (about 16 bytes an element for wide
+    the kernels' tables and their workspace (about 8 bytes an element for wide
     matrices), so steps that share a plan have to be ordered, like steps that
     share a momentum."""
 
