@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <cstdint>
 #include <stdexcept>
@@ -253,8 +254,14 @@ inline void ns_place(std::vector<NsMat>& mats, NsNeeds& sum) {
     throw std::invalid_argument("too many elements for one plan");
 }
 
-// the blocks of one product over placed matrices, longest sums first, so that
-// none of those starts last
+// Neighbouring blocks that share a die: ResNet-50's matrices take 1042 us with
+// 16, 1057 with 32, 1075 with 64, and 1114 with neighbours on all dies.
+constexpr size_t kNsPiece = 16;
+
+// The blocks of one product over placed matrices, longest sums first, so that
+// none of those starts last. Blocks go to the dies in turn, so a piece of a
+// matrix, some neighbouring tiles of one part of the sum, is listed eight
+// places apart and meets its operands in one die's cache.
 inline std::vector<NsTask> ns_tasks(const std::vector<NsMat>& mats, int kind) {
   std::vector<int> order(mats.size());
   for (size_t i = 0; i < mats.size(); ++i) order[i] = (int)i;
@@ -265,30 +272,55 @@ inline std::vector<NsTask> ns_tasks(const std::vector<NsMat>& mats, int kind) {
   };
   std::stable_sort(order.begin(), order.end(),
                    [&](int a, int b) { return work(a) > work(b); });
-  std::vector<NsTask> tasks;
-  int64_t part = 0, slot = 0;
+  std::array<std::vector<NsTask>, 8> dies;
+  std::array<int64_t, 8> load{};
+  int64_t part = 0, slot = 0, count = 0;
   for (int i : order) {
     const NsMat& m = mats[i];
     const auto [tile, whole, splits] = m.kind[kind];
     const int tiles = (int)ns_tiles(m, kind), depth = (int)ns_depth(m, kind);
-    for (int l = 0; l < tiles; ++l) {
-      NsTask t{};
-      t.ws = m.ws;
-      t.mat = i;
-      t.tile = tile;
-      t.mp = m.mp;
-      t.np = m.np;
-      ns_tile_at(kind, l, m.mp / tile, m.np / tile, t.ti, t.tj);
-      t.splits = l < whole ? 1 : splits;
-      t.part = part;
-      t.slot = (int)slot;
-      for (t.slice = 0; t.slice < t.splits; ++t.slice) {
-        t.k0 = depth / 2 * t.slice / t.splits * 2;
-        t.k1 = depth / 2 * (t.slice + 1) / t.splits * 2;
-        tasks.push_back(t);
+    std::vector<NsTask> mine;
+    for (int slice = 0; slice < splits; ++slice)
+      for (int l = slice ? whole : 0; l < tiles; ++l) {
+        NsTask t{};
+        t.ws = m.ws;
+        t.mat = i;
+        t.tile = tile;
+        t.mp = m.mp;
+        t.np = m.np;
+        ns_tile_at(kind, l, m.mp / tile, m.np / tile, t.ti, t.tj);
+        t.splits = l < whole ? 1 : splits;
+        t.slice = slice;
+        t.k1 = depth;
+        if (l >= whole) {
+          t.part = part + (int64_t)(l - whole) * splits * tile * tile;
+          t.slot = (int)(slot + l - whole);
+          t.k0 = depth / 2 * slice / splits * 2;
+          t.k1 = depth / 2 * (slice + 1) / splits * 2;
+        }
+        mine.push_back(t);
       }
-      if (l >= whole) part += (int64_t)splits * tile * tile, ++slot;
+    part += (int64_t)(tiles - whole) * splits * tile * tile;
+    slot += tiles - whole;
+    const size_t piece = std::max<size_t>(kNsPiece, (mine.size() + 7) / 8);
+    for (size_t at = 0; at < mine.size(); at += piece) {
+      const size_t end = std::min(mine.size(), at + piece);
+      const size_t die = std::min_element(load.begin(), load.end()) - load.begin();
+      for (size_t j = at; j < end; ++j) {
+        dies[die].push_back(mine[j]);
+        load[die] += (int64_t)(mine[j].k1 - mine[j].k0) * tile * tile;
+      }
     }
+    count += (int64_t)mine.size();
+  }
+  std::vector<NsTask> tasks;
+  std::array<size_t, 8> next{};
+  while ((int64_t)tasks.size() < count) {
+    size_t die = tasks.size() % 8;
+    if (next[die] == dies[die].size())  // the longest queue helps out
+      for (size_t d = 0; d < 8; ++d)
+        if (dies[d].size() - next[d] > dies[die].size() - next[die]) die = d;
+    tasks.push_back(dies[die][next[die]++]);
   }
   return tasks;
 }
