@@ -943,7 +943,10 @@ void orthogonalize(at::Tensor g, at::Tensor out, std::vector<double> coeffs,
   ng.slots = (unsigned*)slots.data_ptr();
   ng.slot_step = (int)n.slots;
   ng.part_step = n.parts;
-  for (int k = 0; k < lo::NS_KINDS; ++k) ng.kinds[k] = (int)n.kinds[k];
+  for (int k = 0; k < lo::NS_KINDS; ++k) {
+    ng.kinds[k] = (int)n.kinds[k];
+    ng.tile[k] = lo::ns_tile(mats, k);
+  }
   for (int64_t b0 = 0; b0 < g.size(0); b0 += group) {
     const int64_t count = std::min(group, g.size(0) - b0);
     ng.count = (int)count;
@@ -1028,7 +1031,10 @@ struct MuonPlan {
     g.all_chunks = n.chunks;
     g.all_splits = n.splits;
     g.all_slots = (int)n.slots;
-    for (int k = 0; k < lo::NS_KINDS; ++k) g.all_kinds[k] = n.kinds[k];
+    for (int k = 0; k < lo::NS_KINDS; ++k) {
+      g.all_kinds[k] = n.kinds[k];
+      g.tile[k] = lo::ns_tile(mats, k);
+    }
     g.ws = ws.data_ptr();
     g.sums = (double*)sums.data_ptr();
     g.parts = (float*)parts.data_ptr();

@@ -56,6 +56,7 @@ struct NsGroup {
   long src_step, ws_step, part_step;
   int sum_step, slot_step;
   int chunks, splits, kinds[NS_KINDS];               // blocks of one of them
+  int tile[NS_KINDS];  // the tiles' size, 0 where sizes differ
   long all_chunks, all_splits, all_kinds[NS_KINDS];  // of the group
   void* ws;
   double* sums;

@@ -494,10 +494,11 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
   read(0, 0, even);
   if (k0 + (S - 1) * KB < k1) stage(S - 1, k0 + (S - 1) * KB);
   [&] {
-    for (int k = k0;; k += S * KB) {
+    constexpr int ROUND = S * KB * (S * KB % 2 + 1);  // even
+    for (int k = k0;; k += ROUND) {
       #pragma unroll
-      for (int n = 0; n < S * KB; ++n) {
-        const int kt = k + n, s = n / KB, next = (n + 1) % (S * KB);
+      for (int n = 0; n < ROUND; ++n) {
+        const int kt = k + n, s = n / KB % S, next = (n + 1) % (S * KB);
         if (kt + 1 < k1) {
           const bool fresh = next % KB == 0;
           if (fresh) ready(kt + 1 + (S - 2) * KB);
@@ -674,12 +675,16 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
   }
 }
 
-template <int KIND, typename O, bool FINAL>
-__global__ __launch_bounds__(256, 2) void ns_product_kernel(NsProduct pr,
-                                                            NsFinal fin) {
+// MANY: only 64 x 64 tiles, more than fit the chip at two blocks a CU. With
+// three staged tiles there is room for three: 16 x 512 x 2048 (576 tiles) takes
+// 603 us in place of 629.
+template <int KIND, typename O, bool FINAL, bool MANY>
+__global__ __launch_bounds__(256, MANY ? 3 : 2) void ns_product_kernel(
+    NsProduct pr, NsFinal fin) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const NsTask t = task_of<KIND>(pr);
-  if (t.tile == 128) product_tile<128, KIND, 2, 1, O, FINAL>(t, pr, fin, lds);
+  if constexpr (MANY) product_tile<64, KIND, 3, 1, O, FINAL>(t, pr, fin, lds);
+  else if (t.tile == 128) product_tile<128, KIND, 2, 1, O, FINAL>(t, pr, fin, lds);
   else if (t.tile == 64) product_tile<64, KIND, 4, 1, O, FINAL>(t, pr, fin, lds);
   else product_tile<32, KIND, 4, 2, O, FINAL>(t, pr, fin, lds);
 }
@@ -1086,6 +1091,7 @@ void pick_small(const NsGroup& g, int shortest, int longest, const NsInput& in,
 
 // every tile size's staging buffers take 64 KiB; 128's squares need 4 KiB more
 constexpr int kNsLds = 4 * 64 * (64 + 4) * 4;
+constexpr int kNsLdsMany = 3 * 2 * 64 * 128;
 
 template <int KIND, typename O, bool FINAL>
 void product(const NsGroup& g, int from, float alpha, float beta, float diag,
@@ -1100,8 +1106,13 @@ void product(const NsGroup& g, int from, float alpha, float beta, float diag,
                      g.slot_step,       alpha,
                      beta,              diag,
                      g.parts,           g.slots};
-  hipLaunchKernelGGL((ns_product_kernel<KIND, O, FINAL>),
-                     dim3(g.all_kinds[KIND]), dim3(256), kNsLds, s, pr, fin);
+  const long blocks = g.all_kinds[KIND];
+  if (g.tile[KIND] == 64 && blocks > kNsSlots)
+    hipLaunchKernelGGL((ns_product_kernel<KIND, O, FINAL, true>), dim3(blocks),
+                       dim3(256), kNsLdsMany, s, pr, fin);
+  else
+    hipLaunchKernelGGL((ns_product_kernel<KIND, O, FINAL, false>), dim3(blocks),
+                       dim3(256), kNsLds, s, pr, fin);
 }
 
 template <typename T>

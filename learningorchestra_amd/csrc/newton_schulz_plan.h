@@ -229,6 +229,14 @@ inline std::vector<NsMat> ns_plan(
   return mats;
 }
 
+// the size of a product's tiles, 0 where matrices differ
+inline int ns_tile(const std::vector<NsMat>& mats, int kind) {
+  int tile = mats[0].kind[kind].tile;
+  for (const NsMat& m : mats)
+    if (m.kind[kind].tile != tile) tile = 0;
+  return tile;
+}
+
 // gives the matrices their places, one after the other, and adds them up (the
 // products of a step run one after the other and share parts and slots)
 inline void ns_place(std::vector<NsMat>& mats, NsNeeds& sum) {
