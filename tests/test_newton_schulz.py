@@ -96,6 +96,19 @@ def test_large_and_batched(shape):
     assert torch.equal(o, F.orthogonalize(g))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [
+    (100, 100, 130), (300, 130, 100), (40, 129, 260), (100, 129, 130),
+    (40, 129, 400), (60, 257, 260), (100, 129, 400)])
+def test_many_tiles_and_short_sums(shape):
+    """More 64 x 64 tiles than run at once, sums of 4 to 16 steps."""
+    g = _matrix(shape, torch.bfloat16, "cuda")
+    o = F.orthogonalize(g)
+    _check(o, g)
+    assert torch.equal(o, F.orthogonalize(g))
+    assert torch.equal(o[7], F.orthogonalize(g[7:8].expand(shape))[0])
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_converges_to_the_nearest_orthogonal_matrix(device):
     """Thirty cubic steps settle: O O^T = 1, and O G^T is positive."""
