@@ -41,7 +41,7 @@
 //   16 x 512 x 2048    603 us; C X 56 us, 0.92 PFLOP/s; X X^T 44 us, 0.66; A A^T
 //                      21 us. The ends of rounds and the traffic between the
 //                      dies (X is 67 MB) bound it.
-//   ResNet-50's matrices, a whole step: 1042 us, of which 118 move the
+//   ResNet-50's matrices, a whole step: 980 us, of which 118 move the
 //                      momentum, the update and X's first form at 5 TB/s
 //   256 x 3136 bf16    107 us for 17 launches of 4 to 9 us, of which some 3.5
 //                      are the launch, the first loads and the end

@@ -135,13 +135,15 @@ inline bool ns_fit_block(int shortest, int longest) {
 // a split sum, for each part that the last block adds and for each part on the
 // chip. So 256 x 3136 took 232 us with every sum split, 150 us with only deep
 // ones split on 64 x 64 tiles, and 115 us with A and C on 32 x 32; 512 x 512
-// 148 us on 64 x 64 tiles and 95 us on 32 x 32.
+// 148 us on 64 x 64 tiles and 95 us on 32 x 32. ResNet-50's group takes 979 us
+// with A and C on 64 x 64 tiles, 1033 us with A on 128 x 128; 2048 x 2048 653
+// us with A and C on 64 x 64, 748 us on 128 x 128.
 struct NsCost {
   int tile;
   double launch, alone, step, block, join, add, part;
 };
 constexpr NsCost kNsCosts[] = {{32, 3.4, 0.10, 0.10, 0.35, 1.0, 0.3, 0.004},
-                               {64, 4.1, 0.21, 0.22, 1.0, 1.0, 0.5, 0.006},
+                               {64, 4.1, 0.21, 0.19, 1.0, 1.0, 0.5, 0.006},
                                {128, 5.0, 1.0, 0.62, 2.0, 4.0, 1.2, 0.02}};
 constexpr int64_t kNsCus = 256;
 
@@ -149,10 +151,6 @@ constexpr int64_t kNsCus = 256;
 // into parts of at most `most` steps; fills in how
 inline double ns_share(std::vector<NsMat>& mats, int64_t copies, int kind,
                        const NsCost& want, int64_t most) {
-  // small tiles of different matrices share fewer panels in the caches:
-  // ResNet-50's group takes 1276 us with A's on 128 x 128 and C's on 64 x 64
-  // tiles, 1317 us with both on 128 x 128, 1420 us with both on 64 x 64
-  const double apart = mats.size() > 1 && want.tile < 128 ? 1.3 : 1;
   double longest = 0, sum = 0, join = 0, parts = 0;
   int64_t blocks = 0;
   for (NsMat& m : mats) {
@@ -167,7 +165,7 @@ inline double ns_share(std::vector<NsMat>& mats, int64_t copies, int kind,
     const double steps = (double)depth / s;
     longest = std::max(longest, steps * c.alone);
     blocks += tiles * copies * s;
-    sum += (double)(tiles * copies * s) * (steps * c.step * apart + c.block);
+    sum += (double)(tiles * copies * s) * (steps * c.step + c.block);
     if (s > 1) {
       join = std::max(join, c.join + c.add * s);
       parts += c.part * (double)(tiles * copies * s);
