@@ -640,26 +640,51 @@ LO_DEVICE void product_tile(const NsTask& t, const NsProduct& pr,
     const long src = m->src + (fin.mats ? 0 : t.mat * fin.src_step);
     const bool tall = nrows > ncols;
     const float step = out.lr * m->gain;
-    #pragma unroll 2
-    for (int idx = lane; idx < W * W / 8; idx += 64) {
-      int r, c;
-      u32x4 a, b;
-      if (tall) along_col(idx, r, c, a, b);
-      else along_row(idx, r, c, a, b);
+    // where a lane's eight values of piece idx go, and how many are left there
+    auto place = [&](int idx, long& at) {
+      const int r = tall ? (idx >> 4) % (W / 8) * 8 : idx / (W / 8);
+      const int c = tall ? (idx >> 4) / (W / 8) * 16 + (idx & 15)
+                         : idx % (W / 8) * 8;
       const int row = tall ? cw + c : rw + r, col = tall ? rw + r : cw + c;
-      if (row >= nrows) continue;
+      at = src + (long)row * ncols + col;
+      return row < nrows ? ncols - col : 0;
+    };
+    constexpr int N = W * W < 512 ? 1 : W * W / 512;  // pieces a lane
+    constexpr int CH = N < 4 ? N : 4;  // whose weights are read at a time
+    for (int i0 = 0; i0 < N; i0 += CH) {
+      f32x4 w[CH][2] = {};
+      if (out.master) {
+        #pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          long at;
+          const int idx = lane + (i0 + i) * 64;
+          const int n = idx < W * W / 8 ? place(idx, at) : 0;
+          #pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (n > h * 4) w[i][h] = load4(out.master, at + h * 4, n - h * 4);
+        }
+      }
       #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int n = ncols - col - h * 4;
-        if (n <= 0) continue;
-        const f32x4 o = __builtin_bit_cast(f32x4, h ? b : a);
-        const long i = src + (long)row * ncols + col + h * 4;
-        if (out.master) {
-          const f32x4 w = load4(out.master, i, n) * out.keep - step * o;
-          store4(out.master, i, n, w);
-          store4((bf16*)out.mirror, i, n, w);
-        } else {
-          store4((O*)out.out, i, n, o);
+      for (int i = 0; i < CH; ++i) {
+        const int idx = lane + (i0 + i) * 64;
+        if (idx >= W * W / 8) continue;
+        long at;
+        const int n = place(idx, at);
+        int r, c;
+        u32x4 a, b;
+        if (tall) along_col(idx, r, c, a, b);
+        else along_row(idx, r, c, a, b);
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (n <= h * 4) continue;
+          const f32x4 o = __builtin_bit_cast(f32x4, h ? b : a);
+          if (out.master) {
+            const f32x4 v = w[i][h] * out.keep - step * o;
+            store4(out.master, at + h * 4, n - h * 4, v);
+            store4((bf16*)out.mirror, at + h * 4, n - h * 4, v);
+          } else {
+            store4((O*)out.out, at + h * 4, n - h * 4, o);
+          }
         }
       }
     }
