@@ -35,13 +35,14 @@
 //
 // Measured on one MI355X, where 8192^3 library products reach 1.2 PFLOP/s in
 // fp16 and 0.154 in fp32 (five steps; rates count all three fp16 products):
-//   4096 x 4096        3.5 ms; C X 309 us, 1.33 PFLOP/s, matrix pipes busy 88 %
-//                      of a CU's cycles; X X^T 185 us, 1.15 PFLOP/s, 68 %. The
-//                      clock falls to 1.7 GHz: power bounds it.
-//   16 x 512 x 2048    603 us; C X 56 us, 0.92 PFLOP/s; X X^T 44 us, 0.66; A A^T
-//                      21 us. The ends of rounds and the traffic between the
-//                      dies (X is 67 MB) bound it.
-//   ResNet-50's matrices, a whole step: 980 us, of which 118 move the
+//   4096 x 4096        3.3 to 3.5 ms between cards; C X 309 us, 1.33 PFLOP/s,
+//                      matrix pipes busy 88 % of a CU's cycles; X X^T 185 us,
+//                      1.15 PFLOP/s, 68 %. The clock falls to 1.7 GHz: power
+//                      bounds it.
+//   16 x 512 x 2048    566 to 620 us; C X 56 us, 0.92 PFLOP/s; X X^T 44 us,
+//                      0.66; A A^T 21 us. The ends of rounds and the traffic
+//                      between the dies (X is 67 MB) bound it.
+//   ResNet-50's matrices, a whole step: 929 to 1006 us, of which 118 move the
 //                      momentum, the update and X's first form at 5 TB/s
 //   256 x 3136 bf16    107 us for 17 launches of 4 to 9 us, of which some 3.5
 //                      are the launch, the first loads and the end

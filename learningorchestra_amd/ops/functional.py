@@ -427,7 +427,8 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS,
     fp32; computed to fp32's accuracy and rounded once to ``out``, of g's shape
     and type (it may be g). ``coeffs``: (a, b, c), or a triple for each step;
     such that grow singular values past 2^20 are refused. A zero matrix stays
-    zero. A view that is not contiguous is copied first."""
+    zero. A view that is not contiguous is copied first. The same call gives
+    the same bits; batches of other sizes may sum in another order."""
     flat = _ns_coeffs(steps, coeffs, eps)
     if g.dim() < 2:
         raise ValueError("g must be a matrix or a batch of them")

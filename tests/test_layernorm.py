@@ -268,6 +268,30 @@ def test_outputs_that_overlap_an_input(device):
         assert torch.equal(buf, keep)
 
 
+@pytest.mark.gpu
+def test_rows_beyond_32_bits():
+    """The last row starts 2^31 elements on, in the inputs and the outputs."""
+    d = _data(3, 130, torch.bfloat16, "cuda")
+    s, o = _forward(d, True)
+    g = _backward(s, o, d, True)
+
+    def far(t=None):
+        v = torch.empty(2 ** 31 + 130, dtype=torch.bfloat16,
+                        device="cuda").as_strided((3, 130), (2 ** 30, 1))
+        return v if t is None else v.copy_(t)
+
+    x, y, total = far(d["x"]), far(), far()
+    F.layernorm_fwd(x, d["gamma"], d["beta"], EPS, y, residual=d["residual"],
+                    sum_out=total)
+    assert torch.equal(y, o["y"]) and torch.equal(total, o["sum"])
+    dy, dx = far(d["dy"]), far()
+    dg, db = torch.empty_like(d["gamma"]), torch.empty_like(d["beta"])
+    F.layernorm_bwd(dy, total, o["mean"], o["invstd"], d["gamma"], dg, db, dx,
+                    dskip=d["dskip"])
+    assert torch.equal(dx, g["dx"])
+    assert torch.equal(dg, g["dgamma"]) and torch.equal(db, g["dbeta"])
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("cols", [12, 130, 1030])
 def test_far_mean_and_constant_rows(device, cols):

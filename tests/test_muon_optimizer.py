@@ -122,6 +122,22 @@ def test_captured_steps():
     assert int(captured.t) == 4
 
 
+@pytest.mark.gpu
+def test_ranges_beyond_32_bits():
+    gen = torch.Generator().manual_seed(4)
+    near = [torch.rand(64, generator=gen).cuda() for _ in range(4)]
+    near.append(near[0].bfloat16())
+    far = [torch.empty(2 ** 31 + 64, dtype=t.dtype, device="cuda") for t in near]
+    for f, t in zip(far, near):
+        f[2 ** 31:] = t
+    step = torch.ones(1, dtype=torch.int32, device="cuda")
+    for at, arena in ((0, near), (2 ** 31, far)):
+        r = F.AdamRanges([(at + 8, at + 24), (at + 40, at + 64)], at + 64, "cuda")
+        F.adam_ranges(r, *arena, 0.1, 0.9, 0.99, 1e-8, 0.01, step)
+    for f, t in zip(far, near):
+        assert torch.equal(f[2 ** 31:], t)
+
+
 def test_ranges_do_not_overlap():
     for bad in ([(0, 16), (8, 24)], [(8, 24), (0, 16)], [(0, 8), (0, 8)]):
         with pytest.raises(ValueError):

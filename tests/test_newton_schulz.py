@@ -265,6 +265,36 @@ def test_workspace_in_groups():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(64, 512), (128, 640)])
+def test_batches_beyond_32_bits(m, n):
+    """Tiles, and with them the order of sums, go by the batch's size: equal
+    matrices of one batch are equal, those of two batches within tolerance."""
+    one = _matrix((2, m, n), torch.bfloat16, "cuda")
+    g = one[:1].repeat(2 ** 31 // (m * n) + 2, 1, 1)
+    g[-1] = one[1]
+    F.orthogonalize(g, out=g)
+    assert torch.equal(g[0], g[-2])
+    _check(g[0], one[0])
+    _check(g[-1], one[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(20, 30), (70, 90)])
+def test_arena_beyond_32_bits(m, n):
+    """The same step at the arena's start and 2^31 elements on."""
+    views, total, st = _arena([(m, n)], "cuda")
+    far = {k: torch.empty(2 ** 31 + total, dtype=v.dtype, device="cuda")
+           for k, v in st.items()}
+    for k in st:
+        far[k][2 ** 31:] = st[k]
+    F.muon_step(F.MuonPlan(views, total, "cuda"), *st.values(), **KW)
+    F.muon_step(F.MuonPlan([(o + 2 ** 31, *r) for o, *r in views],
+                           2 ** 31 + total, "cuda"), *far.values(), **KW)
+    for k in st:
+        assert torch.equal(far[k][2 ** 31:], st[k]), k
+
+
+@pytest.mark.gpu
 def test_more_small_matrices_than_one_launch_takes():
     """A row's direction does not change, and its length follows the
     polynomial: from 1, five steps end at p(p(p(p(p(1)))))."""
