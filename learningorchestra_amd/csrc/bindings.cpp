@@ -968,12 +968,14 @@ struct MuonPlan {
   int64_t numel;
   int shortest = 0, longest = 0;  // the largest short and long sides
 
-  MuonPlan(std::vector<std::array<int64_t, 3>> views, int64_t numel_,
-           at::Device device)
+  // views: (offset, rows, cols) in ascending order; gains: the factors on the
+  // learning rate
+  MuonPlan(std::vector<std::array<int64_t, 3>> views, std::vector<double> gains,
+           int64_t numel_, at::Device device)
       : numel(numel_) {
     TORCH_CHECK(device.is_cuda(), "the plan's device must be a GPU");
     TORCH_CHECK(!views.empty(), "a Muon plan needs a matrix");
-    std::sort(views.begin(), views.end());
+    TORCH_CHECK(gains.size() == views.size(), "a gain for each matrix");
     int64_t end = 0;
     std::vector<std::pair<int64_t, int64_t>> sides;
     for (const auto& v : views) {
@@ -990,7 +992,10 @@ struct MuonPlan {
     auto mats = lo::ns_plan(sides, 1);
     lo::NsNeeds n;
     lo::ns_place(mats, n);
-    for (size_t i = 0; i < mats.size(); ++i) mats[i].src = views[i][0];
+    for (size_t i = 0; i < mats.size(); ++i) {
+      mats[i].src = views[i][0];
+      mats[i].gain = (float)gains[i];
+    }
     for (const lo::NsMat& m : mats) {
       shortest = std::max(shortest, std::min(m.rows, m.cols));
       longest = std::max(longest, std::max(m.rows, m.cols));
@@ -1131,8 +1136,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("orthogonalize", &orthogonalize);
   py::class_<MuonPlan>(m, "MuonPlan")
       .def(py::init([](std::vector<std::array<int64_t, 3>> views,
-                       int64_t numel, const std::string& device) {
-        return new MuonPlan(std::move(views), numel, at::Device(device));
+                       std::vector<double> gains, int64_t numel,
+                       const std::string& device) {
+        return new MuonPlan(std::move(views), std::move(gains), numel,
+                            at::Device(device));
       }))
       .def("step", &MuonPlan::step);
   m.def("add_relu", &add_relu);

@@ -200,7 +200,6 @@ inline std::vector<NsMat> ns_plan(
     m.mp = (int)ns_up(std::min(rows, cols), pad);
     m.np = (int)ns_up(std::max(rows, cols), pad);
     m.chunks = (int)(ns_up(rows * cols, kNsChunk) / kNsChunk);
-    m.gain = (float)std::sqrt(std::max(1.0, (double)rows / (double)cols));
     mats.push_back(m);
   }
   for (int kind = 0; kind < NS_KINDS; ++kind) {

@@ -34,19 +34,24 @@ class ParamArena:
         self.device = torch.device(device)
         self._specs: List[Tuple[str, Tuple[int, ...], object]] = []
         self._offsets: Dict[str, Tuple[int, int]] = {}
+        self.sides: Dict[str, Tuple[int, int]] = {}   # of padded matrices
         self.master: Optional[torch.Tensor] = None
         self.mirror: Optional[torch.Tensor] = None
         self.grad: Optional[torch.Tensor] = None
         self.numel = 0
 
-    def add(self, name: str, shape: Tuple[int, ...], init) -> str:
+    def add(self, name: str, shape: Tuple[int, ...], init,
+            sides: Optional[Tuple[int, int]] = None) -> str:
         """Register a parameter before finalize(). ``init``: tensor, callable
-        (shape)->tensor, or float std for randn*std."""
+        (shape)->tensor, or float std for randn*std. ``sides``: a matrix's own
+        (rows, cols) where ``shape`` counts padding."""
         assert self.master is None, "arena already finalized"
         assert name not in self._offsets
         n = int(math.prod(shape))
         self._offsets[name] = (self.numel, n)
         self._specs.append((name, tuple(shape), init))
+        if sides is not None and tuple(sides) != tuple(shape):
+            self.sides[name] = tuple(sides)
         self.numel += _pad8(n)
         return name
 
@@ -166,8 +171,10 @@ class Muon:
     orthogonalised form, one grouped call for all of them (newton_schulz.hip);
     biases, norms and the matrices named in ``exclude`` - embeddings and the
     classifier's head, by custom - move by the fused Adam kernel, kept to their
-    ranges of the flat arena. ``weight_decay`` is decoupled on the
-    matrices (w <- (1 - lr wd) w) and Adam's own on the rest."""
+    ranges of the flat arena. A step's length goes by the matrix's own sides,
+    without the rows and columns that pad it (``ParamArena.add``'s ``sides``).
+    ``weight_decay`` is decoupled on the matrices (w <- (1 - lr wd) w) and
+    Adam's own on the rest."""
 
     def __init__(self, arena: ParamArena, lr: float = 0.02,
                  momentum: float = 0.95, nesterov: bool = True,
@@ -182,19 +189,20 @@ class Muon:
         unknown = set(exclude) - names
         if unknown:
             raise ValueError(f"exclude: no parameters {sorted(unknown)}")
-        self.matrices, views, rest = [], [], []
+        self.matrices, views, sides, rest = [], [], [], []
         for name, shape, _ in arena._specs:
             off, n = arena._offsets[name]
             if len(shape) == 2 and min(shape) > 1 and name not in exclude:
                 self.matrices.append(name)
                 views.append((off, *shape))
+                sides.append(arena.sides.get(name, shape))
             elif rest and rest[-1][1] == off:
                 rest[-1][1] = off + _pad8(n)
             else:
                 rest.append([off, off + _pad8(n)])
         if not views:
             raise ValueError("no weight matrix left for Muon")
-        self.plan = F.MuonPlan(views, arena.numel, arena.master.device)
+        self.plan = F.MuonPlan(views, arena.numel, arena.master.device, sides)
         self._rest = F.AdamRanges(rest, arena.numel, arena.master.device)
         self.mom = torch.zeros_like(arena.master)   # also Adam's m1
         self.m2 = torch.zeros_like(arena.master)

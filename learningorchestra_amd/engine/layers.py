@@ -54,8 +54,10 @@ class Conv2dNHWC(Layer):
     def __init__(self, name: str, in_c: int, out_c: int, kh: int, kw: int,
                  stride: int = 1, pad: int = 0, relu: bool = True,
                  first: bool = False, bias: bool = True,
-                 implicit: bool = False):
+                 implicit: bool = False, in_used: Optional[int] = None):
         self.name = name
+        # input channels that are no padding
+        self.in_used = in_c if in_used is None else in_used
         self.bias = bias
         # implicit=True: no col matrix — the fused conv kernels (or the
         # gather-GEMM) handle fwd/dW/dX directly. Measured per model:
@@ -91,7 +93,8 @@ class Conv2dNHWC(Layer):
             t[:, :kdim] = torch.randn((out_c, kdim), generator=g) * std
             return t
 
-        arena.add(self.name + ".w", (self.out_c, self.kpad), init_w)
+        arena.add(self.name + ".w", (self.out_c, self.kpad), init_w,
+                  sides=(out_c, self.kh * self.kw * self.in_used))
         if self.bias:
             arena.add(self.name + ".b", (self.out_c,), torch.zeros(self.out_c))
 
@@ -336,8 +339,11 @@ class Flatten(Layer):
 
 
 class Linear(Layer):
-    def __init__(self, name: str, in_f: int, out_f: int, relu: bool = False):
+    def __init__(self, name: str, in_f: int, out_f: int, relu: bool = False,
+                 in_used: Optional[int] = None, out_used: Optional[int] = None):
         self.name = name
+        # features and outputs that are no padding
+        self.in_used, self.out_used = in_used, out_used
         self.in_f, self.out_f = in_f, out_f
         self.relu = relu
         self.arena: Optional[ParamArena] = None
@@ -348,7 +354,8 @@ class Linear(Layer):
         std = math.sqrt(2.0 / self.in_f)
         g = torch.Generator(device="cpu").manual_seed(zlib.crc32(self.name.encode()) % (2 ** 31))
         arena.add(self.name + ".w", (self.out_f, self.in_f),
-                  torch.randn((self.out_f, self.in_f), generator=g) * std)
+                  torch.randn((self.out_f, self.in_f), generator=g) * std,
+                  sides=(self.out_used or self.out_f, self.in_used or self.in_f))
         arena.add(self.name + ".b", (self.out_f,), torch.zeros(self.out_f))
 
     def param_names(self) -> List[str]:
@@ -414,6 +421,9 @@ class SequentialClassifier:
                 nxt.fuse_relu = True
                 prev.relu_bwd_upstream = True
                 prev._fused_pool = nxt  # bias grad from the pool-level grad
+        head = layers[-1] if layers else None
+        if isinstance(head, Linear) and head.out_used is None:
+            head.out_used = min(num_classes, head.out_f)
         self.arena = ParamArena(device)
         for lay in layers:
             lay.build(self.arena)

@@ -113,7 +113,8 @@ class ResNet:
         # 3 ms/step, 3.6% — the padded channels are all-zero, their weights
         # receive zero gradient and stay at init)
         self.stem_conv = Conv2dNHWC("stem", 8, width, 7, 7, stride=2, pad=3,
-                                    relu=False, first=True, bias=False)
+                                    relu=False, first=True, bias=False,
+                                    in_used=3)
         self.stem_bn = BatchNormReLU("stem.bn", width)
         self.stem_pool = MaxPool2dNHWC(3, stride=2, pad=1)
         self.blocks: List[Bottleneck] = []
@@ -126,7 +127,7 @@ class ResNet:
                 self.blocks.append(blk)
                 in_c = mid * Bottleneck.expansion
         self.avgpool = AvgPoolGlobal()
-        self.fc = Linear("fc", in_c, self.cpad)
+        self.fc = Linear("fc", in_c, self.cpad, out_used=num_classes)
 
         self.stem_conv.build(self.arena)
         self.stem_bn.build(self.arena)

@@ -77,7 +77,8 @@ class LogisticRegressionClassifier:
         Xb = self._prep(X)
         fdim = Xb.shape[1]
         self.model = SequentialClassifier(
-            [Linear("lr.fc", fdim, cpad)], ncls, device=self.device,
+            [Linear("lr.fc", fdim, cpad, in_used=Xt.shape[1])], ncls,
+            device=self.device,
             seed=self.seed)
         trainer = Trainer(self.model, make_sgd(self.model, lr=self.lr,
                                                momentum=0.9), self.device)
@@ -208,9 +209,11 @@ class MLPClassifier:
         dims = [Xb.shape[1], *[_pad8(h) for h in self.hidden]]
         ncls = len(self.classes_)
         cpad = max(8, _pad8(ncls))
-        layers = [Linear(f"mlp.l{i}", dims[i], dims[i + 1], relu=True)
+        used = [Xt.shape[1], *dims[1:]]
+        layers = [Linear(f"mlp.l{i}", dims[i], dims[i + 1], relu=True,
+                         in_used=used[i])
                   for i in range(len(dims) - 1)]
-        layers.append(Linear("mlp.head", dims[-1], cpad))
+        layers.append(Linear("mlp.head", dims[-1], cpad, in_used=used[-1]))
         self.model = SequentialClassifier(layers, ncls, device=self.device,
                                           seed=self.seed)
         trainer = Trainer(self.model, make_sgd(self.model, lr=self.lr,

@@ -49,7 +49,8 @@ class TextCNN:
             # conv-ReLU backward folds into the pool's backward (relu_y mask)
             pool.fuse_relu = True
             conv.relu_bwd_upstream = True
-        self.fc = Linear("fc", filters * len(self.kernel_sizes), self.cpad)
+        self.fc = Linear("fc", filters * len(self.kernel_sizes), self.cpad,
+                         out_used=num_classes)
         self.ln_emb = self.ln_cat = None
         if layer_norm:
             self.ln_emb = LayerNorm("ln_emb", emb_dim)

@@ -460,9 +460,13 @@ class MuonPlan:
     cols), offsets being multiples of 8 as ParamArena's are. On a GPU it owns
     the kernels' tables and their workspace (about 8 bytes an element for wide
     matrices), so steps that share a plan have to be ordered, like steps that
-    share a momentum."""
+    share a momentum.
 
-    def __init__(self, views, numel: int, device) -> None:
+    ``sides`` lists the matrices' own (rows, cols) where the stored ones count
+    rows or columns of padding, which hold zeros: the factor on the learning
+    rate goes by the own sides, and zeros change nothing else."""
+
+    def __init__(self, views, numel: int, device, sides=None) -> None:
         self.views = [tuple(int(v) for v in t) for t in views]
         self.numel = int(numel)
         self.device = torch.device(device)
@@ -478,15 +482,25 @@ class MuonPlan:
             end = off + m * n
         if end > self.numel:
             raise ValueError("a matrix ends outside the arena")
+        self.sides = [t[1:] for t in self.views] if sides is None else \
+            [tuple(int(v) for v in t) for t in sides]
+        if len(self.sides) != len(self.views) or any(
+                len(s) != 2 or not (1 <= s[0] <= m and 1 <= s[1] <= n)
+                for s, (_, m, n) in zip(self.sides, self.views)):
+            raise ValueError("sides: each matrix's own (rows, cols), at most "
+                             "the stored ones")
+        self.gains = [math.sqrt(max(1.0, m / n)) for m, n in self.sides]
         self._native = None
         if self.device.type == "cuda":
             dev = self.device if self.device.index is not None else \
                 torch.device("cuda", torch.cuda.current_device())
+            order = sorted(range(len(self.views)), key=self.views.__getitem__)
             self._native = require_ext().MuonPlan(
-                [list(t) for t in self.views], self.numel, str(dev))
+                [list(self.views[i]) for i in order],
+                [self.gains[i] for i in order], self.numel, str(dev))
 
     def __reduce__(self):   # copies and pickles are plans of their own
-        return MuonPlan, (self.views, self.numel, str(self.device))
+        return MuonPlan, (self.views, self.numel, str(self.device), self.sides)
 
 
 def muon_step(plan: MuonPlan, master: torch.Tensor, grad: torch.Tensor,
@@ -500,7 +514,7 @@ def muon_step(plan: MuonPlan, master: torch.Tensor, grad: torch.Tensor,
         mom <- mu mom + gscale g;  U = gscale g + mu mom (nesterov) or mom
         w <- (1 - lr wd) w - lr sqrt(max(1, rows / cols)) orthogonalize(U)
 
-    Elements outside the matrices stay as they are. Every rank that starts
+    where rows and cols are the plan's ``sides``. Elements outside the matrices stay as they are. Every rank that starts
     from the same values ends with the same values."""
     flat = _ns_coeffs(steps, coeffs, eps)
     if plan._native is not None:
@@ -511,13 +525,12 @@ def muon_step(plan: MuonPlan, master: torch.Tensor, grad: torch.Tensor,
         if t.numel() != plan.numel or t.is_cuda:
             raise RuntimeError(f"the plan is for {plan.numel} elements on "
                                f"{plan.device}")
-    for off, m, n in plan.views:
+    for (off, m, n), gain in zip(plan.views, plan.gains):
         sl = slice(off, off + m * n)
         g = grad[sl] * gscale
         mom[sl].mul_(mu).add_(g)
         u = g + mu * mom[sl] if nesterov else mom[sl]
         o = _newton_schulz_ref(u.view(m, n), flat, eps).reshape(-1)
-        gain = max(1.0, m / n) ** 0.5
         master[sl].mul_(1.0 - lr * wd).add_(o, alpha=-lr * gain)
         mirror[sl] = master[sl].to(mirror.dtype)
 

@@ -1,6 +1,7 @@
 """The Muon optimizer and layer norm inside the engine: parameter split, steps
 against the operators they are made of, checkpoints, captured steps, and a
 small network's gradients."""
+import copy
 import io
 import os
 
@@ -10,9 +11,14 @@ import torch.multiprocessing as mp
 
 from learningorchestra_amd.data.synthetic import imdb_batch
 from learningorchestra_amd.engine.arena import Muon, ParamArena
-from learningorchestra_amd.engine.layers import (LayerNorm, Linear,
+from learningorchestra_amd.engine.layers import (Conv2dNHWC, Flatten,
+                                                 LayerNorm, Linear,
+                                                 MaxPool2dNHWC,
                                                  SequentialClassifier)
 from learningorchestra_amd.engine.trainer import Trainer, make_muon
+from learningorchestra_amd.models.mnist_cnn import build_mnist_cnn
+from learningorchestra_amd.models.resnet import ResNet
+from learningorchestra_amd.models.tabular import MLPClassifier
 from learningorchestra_amd.models.textcnn import build_textcnn
 from learningorchestra_amd.models.zoo import TextCNNClassifier
 from learningorchestra_amd.ops import functional as F
@@ -283,3 +289,83 @@ def test_two_ranks_stay_identical():
         p.join(timeout=30)
     assert not isinstance(results[0], str), results[0]
     assert results[0] == results[1]
+
+
+def _orthogonal64(u):
+    x = u / (u.norm() + 1e-7)
+    a, b, c = F.NS_COEFFS
+    for _ in range(5):
+        s = x @ x.T
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_padding_does_not_shorten_the_steps(device):
+    """Weights stored with rows or columns of padding (a convolution's taps,
+    the head's classes, the stem's channels) move as their own sides say. The
+    tolerance is that of fp32 steps, 1800 sqrt(K) 2^-24 of the step: three sums
+    of K products a step, grown by |p'| < 4 in each later one. The padded sides
+    would make it up to 28 % shorter."""
+    m = SequentialClassifier(
+        [Conv2dNHWC("wide", 1, 32, 5, 5, first=True), MaxPool2dNHWC(2),
+         Flatten(), Linear("narrow", 4 * 4 * 32, 8), Linear("fc", 8, 16)],
+        num_classes=10, device=device)
+    assert m.arena.p("wide.w").shape == (32, 32)
+    gen = torch.Generator().manual_seed(6)
+    x = torch.randn(40, 12, 12, 1, generator=gen).bfloat16().to(device)
+    y = torch.randint(0, 10, (40,), generator=gen).to(device)
+    m.train_step(x, y)
+    opt = make_muon(m, lr=0.1, momentum=0.5)
+    own = {"wide.w": (32, 25), "narrow.w": (8, 512), "fc.w": (10, 8)}
+    assert opt.matrices == list(own)
+    before = {n: m.arena.pf(n).double().cpu() for n in own}
+    opt.step()
+    for n, (rows, cols) in own.items():
+        g = m.arena.g(n).double().cpu()
+        assert bool((g[rows:] == 0).all()) and bool((g[:, cols:] == 0).all())
+        o = _orthogonal64(1.5 * g)
+        step = 0.1 * max(1.0, rows / cols) ** 0.5 * o
+        err = m.arena.pf(n).double().cpu() - (before[n] - step)
+        tol = 1800 * max(g.shape) ** 0.5 * 2 ** -24 * step.norm() \
+            + 4 * 2 ** -24 * (before[n].norm() + step.norm())
+        assert err.norm() <= tol, n
+
+
+def test_models_know_their_padding():
+    assert build_mnist_cnn().arena.sides == {"conv1.w": (32, 25),
+                                             "fc2.w": (10, 256)}
+    assert build_textcnn("cpu", vocab=50).arena.sides == {"fc.w": (2, 384)}
+    r = ResNet((1, 1, 1, 1), num_classes=10, width=16).arena.sides
+    assert r == {"stem.w": (16, 147), "fc.w": (10, 512)}
+    c = MLPClassifier(hidden=(16,), epochs=1, device="cpu")
+    c.fit(torch.randn(20, 5).numpy(), [0, 1] * 10)
+    assert c.model.arena.sides == {"mlp.l0.w": (16, 5), "mlp.head.w": (2, 16)}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sides_of_a_plan(device):
+    """In any order of the views, and refused where they are no part of them."""
+    views = [(64, 8, 4), (0, 6, 4)]
+    a = F.MuonPlan(views, 96, device, sides=[(8, 2), (6, 1)])
+    assert a.gains == [2.0, 6 ** 0.5]
+    b = F.MuonPlan(views[::-1], 96, device, sides=[(6, 1), (8, 2)])
+    none = F.MuonPlan(views, 96, device)
+    g = torch.zeros(96)
+    gen = torch.Generator().manual_seed(8)
+    g[0:24].view(6, 4)[:, :1] = torch.randn(6, 1, generator=gen)
+    g[64:96].view(8, 4)[:, :2] = torch.randn(8, 2, generator=gen)
+    got = []
+    for plan in (a, b, none, copy.deepcopy(a)):
+        w, m = (torch.zeros(96, device=device) for _ in range(2))
+        F.muon_step(plan, w, g.to(device), m, w.bfloat16(), lr=0.5)
+        got.append(w.cpu())
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[3])
+    for sl, ratio in ((slice(0, 24), 4 ** 0.5), (slice(64, 96), 2 ** 0.5)):
+        # two roundings apart: of the factors, and of the products
+        assert ((got[0] - ratio * got[2])[sl].abs()
+                <= 4 * 2 ** -24 * got[0][sl].abs()).all()
+        assert bool((got[0][sl] != 0).any())
+    for bad in ([(8, 4)], [(9, 4), (6, 4)], [(8, 0), (6, 4)], [(8,), (6, 4)]):
+        with pytest.raises(ValueError):
+            F.MuonPlan(views, 96, device, sides=bad)
