@@ -219,15 +219,43 @@ class Muon:
                       a.mirror, self.adam_lr, self.betas[0], self.betas[1],
                       self.eps, self.weight_decay, self.t, gscale)
 
+    def _stepped_otherwise(self, mom, m2):
+        # a state without a list of its matrices: Adam's second moment is zero
+        # on them, and on the rest only where no gradient came
+        other = []
+        for name, _, _ in self.arena._specs:
+            off, n = self.arena._offsets[name]
+            second = bool((m2[off:off + n] != 0).any())
+            if name in self.matrices:
+                wrong = second
+            else:
+                wrong = not second and bool((mom[off:off + n] != 0).any())
+            if wrong:
+                other.append(name)
+        return other
+
     def state_dict(self):
         return {"mom": self.mom.cpu().clone(), "m2": self.m2.cpu().clone(),
-                "t": int(self.t),
+                "t": int(self.t), "matrices": list(self.matrices),
                 "lr": self.lr, "momentum": self.momentum,
                 "nesterov": self.nesterov, "steps": self.steps,
                 "weight_decay": self.weight_decay, "adam_lr": self.adam_lr,
                 "betas": list(self.betas), "eps": self.eps}
 
     def load_state_dict(self, sd):
+        """Refuses, before anything changes, a state of other matrices: ``mom``
+        is a momentum on those and Adam's first moment on the rest."""
+        for k, own in (("mom", self.mom), ("m2", self.m2)):
+            if sd[k].shape != own.shape:
+                raise ValueError(f"{k}: {tuple(sd[k].shape)} in the state, "
+                                 f"{tuple(own.shape)} in this optimizer")
+        if "matrices" in sd:
+            other = set(sd["matrices"]) ^ set(self.matrices)
+        else:
+            other = self._stepped_otherwise(sd["mom"], sd["m2"])
+        if other:
+            raise ValueError("the state was saved with another choice of "
+                             f"matrices: {sorted(other)}")
         self.mom.copy_(sd["mom"].to(self.mom.device))
         self.m2.copy_(sd["m2"].to(self.m2.device))
         if torch.is_tensor(self.t):

@@ -369,3 +369,33 @@ def test_sides_of_a_plan(device):
     for bad in ([(8, 4)], [(9, 4), (6, 4)], [(8, 0), (6, 4)], [(8,), (6, 4)]):
         with pytest.raises(ValueError):
             F.MuonPlan(views, 96, device, sides=bad)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("listed", [True, False])
+def test_checkpoint_of_other_matrices(device, listed):
+    """Refused before anything changes, with the list of matrices and, in a
+    state that has none, by the moments; the same ones load either way."""
+    saved = Muon(_arena(device), lr=0.5, exclude=("emb.w",))
+    for seed in range(2):
+        _grads(saved.arena, seed)
+        saved.step()
+    sd = saved.state_dict()
+    assert sd["matrices"] == ["conv.w", "tall.w", "head.w"]
+    if not listed:
+        del sd["matrices"]
+    for exclude in ((), ("emb.w", "head.w"), ("head.w",)):
+        opt = Muon(_arena(device), lr=0.25, exclude=exclude)
+        _grads(opt.arena, 5)
+        opt.step()
+        mom, m2 = opt.mom.clone(), opt.m2.clone()
+        with pytest.raises(ValueError):
+            opt.load_state_dict(sd)
+        assert torch.equal(opt.mom, mom) and torch.equal(opt.m2, m2)
+        assert int(opt.t) == 1 and opt.lr == 0.25
+    opt = Muon(_arena(device), exclude=("emb.w",))
+    opt.load_state_dict(sd)
+    assert torch.equal(opt.mom, saved.mom) and int(opt.t) == 2 and opt.lr == 0.5
+    with pytest.raises(ValueError):
+        opt.load_state_dict({**sd, "m2": sd["m2"][:1]})
+    assert torch.equal(opt.m2, saved.m2)
