@@ -5,6 +5,7 @@
 #include <array>
 #include <cmath>
 #include <cstdint>
+#include <limits>
 #include <stdexcept>
 #include <vector>
 
@@ -21,24 +22,38 @@ inline int64_t ns_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 // stored value below 2^15: with singular values in [0, s] before a step, X's
 // entries stay below s, A's below s^2, C's below max |a + b q + c q^2| over
 // q in [0, s^2] and the next X's below max t |a + b t^2 + c t^4| over [0, s].
+// Singular values may go to 2^20 and, between steps, down to 2^-20, A's and C's
+// entries to the squares of that: with coefficients of fp32 all factors of the
+// products (at most sa^2 = 2^110) stay within fp32's range.
+// ops.functional._ns_bounds refuses the same ones.
 inline std::vector<NsStep> ns_steps(const std::vector<double>& coeffs) {
   if (coeffs.empty() || coeffs.size() % 3)
     throw std::invalid_argument(
         "coefficients come in threes, for one step at least");
-  auto scale = [](double bound) {
-    if (!(bound < 1048576.0))
+  // the power of two for values up to a bound, which is 0 or from 1 / most on
+  auto scale = [](double bound, double most) {
+    if (!(bound < most))
       throw std::invalid_argument(
-          "these coefficients let the singular values grow past 2^20");
+          "these coefficients let the singular values grow past 2^20, or a "
+          "step's polynomial past 2^40");
     int e;
-    std::frexp(std::max(bound * 1.001, 1e-3), &e);  // bound < 2^e
+    std::frexp(std::max(bound * 1.001, 1 / most), &e);  // bound < 2^e
     return (float)std::ldexp(1.0, 15 - e);
   };
+  constexpr double kX = 1l << 20, kA = 1l << 40;
   std::vector<NsStep> st(coeffs.size() / 3);
   double s = 1.001;
-  float sx = scale(s);
+  float sx = scale(s, kX);
   for (size_t i = 0; i < st.size(); ++i) {
     const double a = coeffs[3 * i], b = coeffs[3 * i + 1], c = coeffs[3 * i + 2];
     const double end = s * s;
+    if (s != 0 && s < 1 / kX)
+      throw std::invalid_argument(
+          "these coefficients let the singular values fall below 2^-20 before "
+          "a step");
+    for (double v : {a, b, c})
+      if (!(std::abs(v) <= (double)std::numeric_limits<float>::max()))
+        throw std::invalid_argument("coefficients must be finite in fp32");
     double most_c = 0, most_x = 0;
     auto try_at = [&](double q) {
       if (!(q >= 0 && q <= end)) return;
@@ -58,10 +73,11 @@ inline std::vector<NsStep> ns_steps(const std::vector<double>& coeffs) {
     } else if (b != 0) {
       try_at(-a / (3 * b));
     }
-    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c))
-      throw std::invalid_argument("coefficients must be finite");
-    st[i] = {(float)a, (float)b, (float)c, sx, scale(end), scale(most_c),
-             scale(most_x)};
+    if (most_c != 0 && most_c < 1 / kA)
+      throw std::invalid_argument(
+          "these coefficients make a step's polynomial fall below 2^-40");
+    st[i] = {(float)a, (float)b, (float)c, sx, scale(end, kA),
+             scale(most_c, kA), scale(most_x, kX)};
     sx = st[i].sn;
     s = most_x * 1.001;
   }

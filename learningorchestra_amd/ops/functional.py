@@ -386,23 +386,38 @@ def _ns_coeffs(steps: int, coeffs, eps: float) -> list:
         coeffs[0], "__len__") else list(coeffs)
     if len(rows) != steps or any(len(r) != 3 for r in rows):
         raise ValueError("coeffs: one (a, b, c), or one for each step")
-    flat = [float(v) for r in rows for v in r]
-    top = 1.0           # the largest singular value, before and after a step
+    return [float(v) for r in rows for v in r]
+
+
+def _ns_bounds(flat: list) -> None:
+    """Refuses for the CPU path the coefficients that the bindings refuse
+    (newton_schulz_plan.h), whose powers of two would leave fp32's range."""
+    top = 1.001         # the singular values' bound, before and after a step
     for a, b, c in zip(*[iter(flat)] * 3):
-        if not all(math.isfinite(v) for v in (a, b, c)):
-            raise ValueError("coeffs must be finite")
-        # |p| is largest at the end or where p' = a + 3 b q + 5 c q^2 = 0
-        q, disc = [top * top], 9 * b * b - 20 * a * c
+        if not all(abs(v) <= torch.finfo(torch.float32).max for v in (a, b, c)):
+            raise ValueError("coeffs must be finite in fp32")
+        if 0 < top < 2.0 ** -20:
+            raise ValueError("these coefficients let the singular values fall "
+                             "below 2^-20 before a step")
+        # |a + b q + c q^2| is largest at an end or where its slope is zero, and
+        # sqrt(q) times it at the end or where a + 3 b q + 5 c q^2 = 0
+        q, disc = [0.0, top * top], 9 * b * b - 20 * a * c
+        if c:
+            q.append(-b / (2 * c))
         if c and disc >= 0:
             q += [(-3 * b + r * math.sqrt(disc)) / (10 * c) for r in (1, -1)]
         elif not c and b:
             q.append(-a / (3 * b))
-        top = max(math.sqrt(v) * abs(a + b * v + c * v * v)
-                  for v in q if 0 <= v <= top * top)
-        if top >= 2 ** 20:
+        q = [v for v in q if 0 <= v <= top * top]
+        poly = [abs(a + b * v + c * v * v) for v in q]
+        most = max(math.sqrt(v) * p for v, p in zip(q, poly))
+        if most >= 2 ** 20 or max(poly) >= 2 ** 40:
             raise ValueError("these coefficients let the singular values "
-                             "grow past 2^20")
-    return flat
+                             "grow past 2^20, or a step's polynomial past 2^40")
+        if 0 < max(poly) < 2.0 ** -40:
+            raise ValueError("these coefficients make a step's polynomial "
+                             "fall below 2^-40")
+        top = most * 1.001
 
 
 def _newton_schulz_ref(x: torch.Tensor, flat: list, eps: float) -> torch.Tensor:
@@ -425,8 +440,10 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS,
     Newton-Schulz steps X <- a X + (b A + c A^2) X, A = X X^T, from
     X = G / (|G|_F + eps). g [m, n] or a batch [..., m, n] in bf16, fp16 or
     fp32; computed to fp32's accuracy and rounded once to ``out``, of g's shape
-    and type (it may be g). ``coeffs``: (a, b, c), or a triple for each step;
-    such that grow singular values past 2^20 are refused. A zero matrix stays
+    and type (it may be g). ``coeffs``: (a, b, c), or a triple for each step.
+    Refused are those that can bring a singular value past 2^20 or, before a
+    step, below 2^-20, and polynomials a + b q + c q^2 that stay below 2^-40.
+    A zero matrix stays
     zero. A view that is not contiguous is copied first. The same call gives
     the same bits; batches of other sizes may sum in another order."""
     flat = _ns_coeffs(steps, coeffs, eps)
@@ -449,6 +466,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS,
         require_ext().orthogonalize(g.contiguous().view(three),
                                     out.view(three), flat, eps)
         return out
+    _ns_bounds(flat)
     if g.numel():
         out.copy_(_newton_schulz_ref(g.contiguous().float(), flat, eps))
     return out
@@ -525,6 +543,7 @@ def muon_step(plan: MuonPlan, master: torch.Tensor, grad: torch.Tensor,
         if t.numel() != plan.numel or t.is_cuda:
             raise RuntimeError(f"the plan is for {plan.numel} elements on "
                                f"{plan.device}")
+    _ns_bounds(flat)
     for (off, m, n), gain in zip(plan.views, plan.gains):
         sl = slice(off, off + m * n)
         g = grad[sl] * gscale

@@ -520,3 +520,46 @@ def test_two_plans_on_two_streams():
     for st in states:
         for k in want:
             assert torch.equal(st[k], want[k]), k
+
+
+# coefficients of each step; those below the line pass 2^10 or fall below 2^-10
+# between steps, so that A's bound is beyond 2^20 or below 2^-20
+TAKEN = [[(8e5, 0.0, 0.0)], [(9e-7, 0.0, 0.0)], [(1e-12, 0.0, 0.0)],
+         [(0.0, 0.0, 0.0)], [(0.0, 0.0, 0.0), CUBIC],
+         [(0.0, 1.0, 0.0), (0.0, 0.0, 1.0)],
+         # ---
+         [(2000.0, 0.0, 0.0), (0.0005, 0.0, 0.0)],
+         [(1e6, 0.0, 0.0), (1e-6, 0.0, 0.0)],
+         [(1e-6, 0.0, 0.0), (1e6, 0.0, 0.0)],
+         [(1e-5, 0.0, 0.0), (1.5e5, -5e14, 0.0)],
+         [(4000.0, -6000.0, 2500.0), (2.5e-4, 0.0, 0.0)]]
+REFUSED = [[(1048576.0, 0.0, 0.0)], [(2000.0, 0.0, 0.0), (2000.0, 0.0, 0.0)],
+           [(0.0, 1e6, 1e6)], [(1e39, -1e39, 0.0)], [(1e300, 0.0, 0.0)],
+           [(float("inf"), 0.0, 0.0)], [(0.0, 0.0, float("nan"))],
+           [(9e-7, 0.0, 0.0), (1.0, 0.0, 0.0)], [(9e-13, 0.0, 0.0)],
+           [(1e-6, 0.0, 0.0), (2e12, 0.0, 0.0)],
+           [(1e-5, 0.0, 0.0), (1.0, 0.0, 1e60)]]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(20, 30), (70, 90)])
+@pytest.mark.parametrize("coeffs", TAKEN)
+def test_coefficients_within_the_limits(device, shape, coeffs):
+    g = _matrix(shape, device=device)
+    _check(F.orthogonalize(g, steps=len(coeffs), coeffs=coeffs), g, coeffs)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(20, 30), (70, 90), (0, 5)])
+@pytest.mark.parametrize("coeffs", REFUSED)
+def test_coefficients_beyond_the_limits(device, shape, coeffs):
+    """The same ones on the CPU and on GPUs."""
+    g = torch.zeros(shape, device=device)
+    with pytest.raises(ValueError):
+        F.orthogonalize(g, steps=len(coeffs), coeffs=coeffs)
+    plan = F.MuonPlan([(0, 4, 4)], 16, device)
+    st = [torch.ones(16, device=device) for _ in range(3)]
+    with pytest.raises(ValueError):
+        F.muon_step(plan, *st, st[0].bfloat16(), lr=0.1, steps=len(coeffs),
+                    coeffs=coeffs)
+    assert all(bool((t == 1).all()) for t in st)
