@@ -158,13 +158,14 @@ LO_DEVICE void store4(T* p, long i, int n, const f32x4& v) {
 }
 
 // X = U f 2^-e from the sum of U's squares: 1 / (norm + eps), so that neither
-// tiny nor huge updates leave fp32's range on the way
+// tiny nor huge updates leave fp32's range on the way; zeros stay zero without
+// an eps, too
 struct NsNorm {
   float f;
   int e;
   LO_DEVICE NsNorm(double squares, float eps) {
     const double m = frexp(sqrt(squares) + (double)eps, &e);
-    f = (float)(1.0 / m);
+    f = m == 0.0 ? 0.f : (float)(1.0 / m);
   }
   LO_DEVICE f32x4 operator()(f32x4 u) const {
     #pragma unroll

@@ -425,7 +425,8 @@ def _newton_schulz_ref(x: torch.Tensor, flat: list, eps: float) -> torch.Tensor:
     if tall:
         x = x.transpose(-2, -1)
     x = x.double()
-    x = (x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps)).float()
+    norm = x.square().sum((-2, -1), keepdim=True).sqrt() + eps
+    x = (x / norm.where(norm != 0, 1.0)).float()
     for i in range(0, len(flat), 3):
         a, b, c = flat[i:i + 3]
         gram = x @ x.transpose(-2, -1)

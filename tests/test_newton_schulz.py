@@ -563,3 +563,31 @@ def test_coefficients_beyond_the_limits(device, shape, coeffs):
         F.muon_step(plan, *st, st[0].bfloat16(), lr=0.1, steps=len(coeffs),
                     coeffs=coeffs)
     assert all(bool((t == 1).all()) for t in st)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("eps", [0.0, 1e-60])
+@pytest.mark.parametrize("shape", [(20, 30), (130, 70)])
+def test_zeros_without_an_eps(device, eps, shape):
+    """A zero matrix stays zero, and with no gradient a weight only decays,
+    also where eps is nothing in fp32. NaN and infinities are no zeros."""
+    g = _matrix((3, *shape), device=device)
+    want = F.orthogonalize(g, eps=eps)
+    g[1] = 0
+    o = F.orthogonalize(g, eps=eps)
+    assert bool((o[1] == 0).all())
+    assert torch.equal(o[0], want[0]) and torch.equal(o[2], want[2])
+    for bad in ("nan", "inf"):
+        g[1, 2, 3] = float(bad)
+        assert bool(F.orthogonalize(g, eps=eps)[1].isnan().all())
+    views, total, st = _arena([shape, (5, 9)], device)
+    for k in ("grad", "mom"):
+        st[k][views[0][0]:views[0][0] + shape[0] * shape[1]] = 0
+    old = st["master"].clone()
+    F.muon_step(F.MuonPlan(views, total, device), *st.values(),
+                **{**KW, "eps": eps})
+    sl = slice(views[0][0], views[0][0] + shape[0] * shape[1])
+    keep = 1.0 - KW["lr"] * KW["wd"]
+    assert (st["master"][sl].double() - keep * old[sl].double()).abs().max() \
+        <= 2 * U * old.abs().max()
+    assert bool(st["master"].isfinite().all())
