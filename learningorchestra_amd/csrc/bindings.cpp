@@ -793,6 +793,47 @@ void check_vec(const at::Tensor& t, const at::Tensor& like, int64_t n,
   TORCH_CHECK(t.numel() == n, name, " must hold ", n, " values");
 }
 
+// whether some row of t (cut to its columns) shares memory with vec
+bool touches(const at::Tensor& t, const at::Tensor& vec) {
+  if (t.numel() == 0 || vec.numel() == 0) return false;
+  const bool flat = t.dim() < 2;
+  const int64_t size = t.itemsize();
+  const int64_t row = flat || t.size(0) < 2 ? 0 : t.stride(0) * size;
+  const int64_t rows = row ? t.size(0) : 1;
+  const int64_t width = (flat ? t.numel() : t.size(1)) * size;
+  const auto at = (int64_t)t.data_ptr(), v = (int64_t)vec.data_ptr();
+  // the first row that ends behind vec's start
+  const int64_t r = row && v - at >= width ? (v - at - width) / row + 1 : 0;
+  return r < rows && at + r * row < v + (int64_t)vec.nbytes() &&
+         at + r * row + width > v;
+}
+
+struct Named {
+  const char* name;
+  const at::Tensor* t;  // or null
+};
+
+// statistics and parameters' gradients share no memory with anything else, nor
+// do the activations' outputs with statistics and parameters
+void check_own(const Named& vec_out0, const Named& vec_out1,
+               std::initializer_list<Named> vecs,
+               std::initializer_list<Named> outs,
+               std::initializer_list<Named> ins) {
+  auto apart = [](const Named& a, const Named& b) {
+    TORCH_CHECK(!a.t || !b.t || !touches(*a.t, *b.t), a.name, " and ", b.name,
+                " must not share memory");
+  };
+  apart(vec_out0, vec_out1);
+  for (const auto* others : {&vecs, &outs, &ins})
+    for (const Named& o : *others) apart(o, vec_out0), apart(o, vec_out1);
+  for (const Named& o : outs)
+    for (const Named& v : vecs) apart(o, v);
+}
+
+const at::Tensor* given(const c10::optional<at::Tensor>& t) {
+  return t ? &*t : nullptr;
+}
+
 constexpr int64_t kLayerNormCols = 32768;  // a row fits one block's registers
 
 void check_layernorm(const at::Tensor& x) {
@@ -831,6 +872,10 @@ void layernorm_fwd(at::Tensor x, at::Tensor gamma, at::Tensor beta, double eps,
     check_apart(*sum_out, *residual, "sum_out");
     check_apart(*sum_out, out, "sum_out");
   }
+  check_own({"mean", given(mean)}, {"invstd", given(invstd)},
+            {{"gamma", &gamma}, {"beta", &beta}},
+            {{"out", &out}, {"sum_out", given(sum_out)}},
+            {{"x", &x}, {"residual", given(residual)}});
   if (rows == 0) return;
   const c10::DeviceGuard guard(x.device());
   lo::launch_layernorm_fwd(
@@ -863,6 +908,9 @@ void layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor mean,
   check_vec(gamma, x, cols, "gamma");
   check_vec(dgamma, x, cols, "dgamma");
   check_vec(dbeta, x, cols, "dbeta");
+  check_own({"dgamma", &dgamma}, {"dbeta", &dbeta},
+            {{"gamma", &gamma}, {"mean", &mean}, {"invstd", &invstd}},
+            {{"dx", &dx}}, {{"dy", &dy}, {"x", &x}, {"dskip", given(dskip)}});
   const c10::DeviceGuard guard(x.device());
   if (rows == 0) {
     dgamma.zero_();

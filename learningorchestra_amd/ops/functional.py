@@ -741,13 +741,15 @@ def layernorm_fwd(x2d: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor,
     and, for training, mean and invstd (fp32 [M]). ``residual`` [M, C] is
     added first; the sum, rounded to x2d's type, is what gets normalised and
     goes to ``sum_out`` (the backward pass's x2d). ``out`` and ``sum_out`` may
-    each be one of the inputs, but not a part of one."""
+    each be one of x2d and the residual, but not a part of one; outputs share
+    no memory otherwise."""
     if _is_gpu(x2d):
         require_ext().layernorm_fwd(x2d, gamma, beta, eps, out, mean, invstd,
                                     residual, sum_out)
         return
     _check_layernorm(x2d, (out, residual, sum_out), (gamma, beta),
-                     (mean, invstd), (out, sum_out))
+                     (mean, invstd), (out, sum_out), (gamma, beta),
+                     (mean, invstd))
     if (mean is None) != (invstd is None):
         raise RuntimeError("mean and invstd come together")
     if sum_out is not None and residual is None:
@@ -776,13 +778,14 @@ def layernorm_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, mean: torch.Tensor,
     overwritten; the same sums on every run) and dx. ``dskip`` [M, C], the
     gradient that reaches the sum past the norm, is added to dx, which then is
     the gradient of x and of the residual alike. ``dx`` may be dy2d, x2d or
-    dskip, but not a part of one."""
+    dskip, but not a part of one; outputs share no memory otherwise."""
     if _is_gpu(x2d):
         require_ext().layernorm_bwd(dy2d, x2d, mean, invstd, gamma, dgamma,
                                     dbeta, dx, dskip)
         return
     _check_layernorm(x2d, (dy2d, dx, dskip), (gamma, dgamma, dbeta),
-                     (mean, invstd), (dx,))
+                     (mean, invstd), (dx,), (gamma, mean, invstd),
+                     (dgamma, dbeta))
     g = dy2d.float()
     xhat = (x2d.float() - mean.view(-1, 1)) * invstd.view(-1, 1)
     h = g * gamma
@@ -808,7 +811,21 @@ def _apart(out: torch.Tensor, x: torch.Tensor) -> bool:
     return lo == li and cols * size <= (a - b) % (lo * size) <= (lo - cols) * size
 
 
-def _check_layernorm(x, rows, vecs, stats, outs) -> None:
+def _touches(t: torch.Tensor, vec: torch.Tensor) -> bool:
+    # whether some row of t (cut to its columns) shares memory with vec
+    if not t.numel() or not vec.numel() or t.device != vec.device:
+        return False
+    size = t.element_size()
+    row = t.stride(0) * size if t.dim() > 1 and t.shape[0] > 1 else 0
+    rows = t.shape[0] if row else 1
+    width = (t.shape[1] if t.dim() > 1 else t.numel()) * size
+    at, v = t.data_ptr(), vec.data_ptr()
+    r = (v - at - width) // row + 1 if row and v - at >= width else 0
+    return r < rows and at + r * row < v + vec.numel() * vec.element_size() \
+        and at + r * row + width > v
+
+
+def _check_layernorm(x, rows, vecs, stats, outs, vec_ins, vec_outs) -> None:
     # the CPU path refuses what the kernels' bindings refuse
     if x.dim() != 2 or not 1 <= x.shape[1] <= 32768:
         raise RuntimeError("layer norm takes [rows, 1 to 32768 columns]")
@@ -832,6 +849,14 @@ def _check_layernorm(x, rows, vecs, stats, outs) -> None:
             if None not in (o, t) and o is not t and not _apart(o, t):
                 raise RuntimeError("an output may be an input, but not overlap "
                                    "one in part")
+    # pairs of which one is written and one is a vector
+    pairs = [(o, v) for o in outs for v in vec_ins]
+    for i, v in enumerate(vec_outs):
+        pairs += [(t, v) for t in (x, *rows, *vec_ins, *vec_outs[:i])]
+    if any(t is not None and v is not None and _touches(t, v)
+           for t, v in pairs):
+        raise RuntimeError("statistics, parameters and their gradients must "
+                           "not share memory with an output")
 
 
 # ------------------------------------------------------------ residual add

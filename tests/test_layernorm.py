@@ -476,3 +476,70 @@ def test_layer(device):
     # another batch without the skip path
     y = layer.forward(x3[:2].contiguous())
     assert layer.sum is None and y.shape == (2, 6, 48)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_vectors_share_no_memory_with_outputs(device):
+    """Statistics, parameters and their gradients are refused in one another's
+    place and where they share an element with an activation's rows, before
+    anything is written; between the rows of a wider buffer they are taken."""
+    n = 12
+    d = _data(n, n, torch.float32, device)
+    wide = {k: torch.zeros(n, 64, device=device)
+            for k in ("x", "residual", "y", "sum", "dy", "dskip", "dx")}
+    t = {k: w[:, 26:38] for k, w in wide.items()}
+    for k in ("x", "residual", "dy", "dskip"):
+        t[k].copy_(d[k])
+    v = [torch.ones(n, device=device) for _ in range(5)]
+    long = torch.ones(n + 1, device=device)
+    part = (long[:n], long[1:])
+
+    def fwd(ga=v[0], be=v[1], mean=v[2], invstd=v[3]):
+        F.layernorm_fwd(t["x"], ga, be, EPS, t["y"], mean=mean, invstd=invstd,
+                        residual=t["residual"], sum_out=t["sum"])
+
+    def bwd(ga=v[0], mean=v[1], invstd=v[2], dg=v[3], db=v[4]):
+        F.layernorm_bwd(t["dy"], t["x"], mean, invstd, ga, dg, db, t["dx"],
+                        dskip=t["dskip"])
+
+    calls = [(fwd, dict(mean=v[3])), (fwd, dict(mean=v[0])),
+             (fwd, dict(invstd=v[1])),
+             (fwd, dict(mean=part[0], invstd=part[1])),
+             (fwd, dict(ga=part[0], mean=part[1])),
+             (bwd, dict(dg=v[4])), (bwd, dict(dg=v[0])), (bwd, dict(db=v[1])),
+             (bwd, dict(dg=v[2])), (bwd, dict(dg=part[1], db=part[0]))]
+    taken = []
+
+    def inside(call, name, arg):
+        for row in (0, 5, n - 1):
+            for col, shared in ((14, False), (15, True), (26, True),
+                                (37, True), (38, False)):
+                at = dict([(arg, wide[name][row, col:col + n])])
+                (calls if shared else taken).append((call, at))
+
+    for arg in ("mean", "invstd"):
+        for name in ("x", "residual", "y", "sum"):
+            inside(fwd, name, arg)
+    for arg in ("ga", "be"):
+        for name in ("y", "sum"):
+            inside(fwd, name, arg)
+    for arg in ("dg", "db"):
+        for name in ("dy", "x", "dskip", "dx"):
+            inside(bwd, name, arg)
+    for arg in ("ga", "mean", "invstd"):
+        inside(bwd, "dx", arg)
+    keep = {k: w.clone() for k, w in wide.items()}
+    for i, (call, at) in enumerate(calls):
+        with pytest.raises(RuntimeError):
+            call(**at)
+            pytest.fail(f"call {i} was taken")
+    assert all(torch.equal(wide[k], keep[k]) for k in keep)
+    assert all(bool((w == 1).all()) for w in (*v, long))
+    for call, at in taken:
+        call(**at)
+    for k in ("x", "residual", "dy", "dskip"):
+        assert torch.equal(t[k], d[k])
+    near = wide["x"][3, 38:50]
+    fwd(mean=near)
+    want = t["sum"].double().mean(1)
+    assert (near.double() - want).abs().max() <= 64 * U * t["sum"].abs().max()
