@@ -596,6 +596,29 @@ void adam_step(at::Tensor master, at::Tensor grad, at::Tensor m1, at::Tensor m2,
                   (float)wd, (float)gscale, stream());
 }
 
+// whether some row of t (cut to its columns) shares memory with vec
+bool touches(const at::Tensor& t, const at::Tensor& vec) {
+  if (t.numel() == 0 || vec.numel() == 0) return false;
+  const bool flat = t.dim() < 2;
+  const int64_t size = t.itemsize();
+  const int64_t row = flat || t.size(0) < 2 ? 0 : t.stride(0) * size;
+  const int64_t rows = row ? t.size(0) : 1;
+  const int64_t width = (flat ? t.numel() : t.size(1)) * size;
+  const auto at = (int64_t)t.data_ptr(), v = (int64_t)vec.data_ptr();
+  // the first row that ends behind vec's start
+  const int64_t r = row && v - at >= width ? (v - at - width) / row + 1 : 0;
+  return r < rows && at + r * row < v + (int64_t)vec.nbytes() &&
+         at + r * row + width > v;
+}
+
+// an arena's tensors, all contiguous
+void check_arena(std::initializer_list<const at::Tensor*> ts) {
+  for (auto a = ts.begin(); a != ts.end(); ++a)
+    for (auto b = ts.begin(); b != a; ++b)
+      TORCH_CHECK(!touches(**a, **b),
+                  "the arena's tensors must not share memory");
+}
+
 // what an object keeps may be used on another stream than it was made on: its
 // memory is not given to others before this stream is done with it
 void used_here(std::initializer_list<at::Tensor> kept) {
@@ -628,6 +651,8 @@ void adam_ranges(at::Tensor master, at::Tensor grad, at::Tensor m1,
                   ranges.device() == master.device() &&
                   ranges.size(0) <= 65535,
               "ranges must be int64 [k, 2] on the arena's GPU");
+  TORCH_CHECK(step_dev.numel() == 1, "step_dev must hold one value");
+  check_arena({&master, &grad, &m1, &m2, &mirror});
   if (ranges.size(0) == 0 || longest <= 0) return;
   const c10::DeviceGuard guard(master.device());
   used_here({ranges});
@@ -791,21 +816,6 @@ void check_vec(const at::Tensor& t, const at::Tensor& like, int64_t n,
   TORCH_CHECK(t.device() == like.device(), name,
               " must be on the input's device");
   TORCH_CHECK(t.numel() == n, name, " must hold ", n, " values");
-}
-
-// whether some row of t (cut to its columns) shares memory with vec
-bool touches(const at::Tensor& t, const at::Tensor& vec) {
-  if (t.numel() == 0 || vec.numel() == 0) return false;
-  const bool flat = t.dim() < 2;
-  const int64_t size = t.itemsize();
-  const int64_t row = flat || t.size(0) < 2 ? 0 : t.stride(0) * size;
-  const int64_t rows = row ? t.size(0) : 1;
-  const int64_t width = (flat ? t.numel() : t.size(1)) * size;
-  const auto at = (int64_t)t.data_ptr(), v = (int64_t)vec.data_ptr();
-  // the first row that ends behind vec's start
-  const int64_t r = row && v - at >= width ? (v - at - width) / row + 1 : 0;
-  return r < rows && at + r * row < v + (int64_t)vec.nbytes() &&
-         at + r * row + width > v;
 }
 
 struct Named {
@@ -1106,6 +1116,7 @@ struct MuonPlan {
       TORCH_CHECK(t.device() == table.device(), "the plan is on ",
                   table.device());
     }
+    check_arena({&master, &grad, &mom, &mirror});
     TORCH_CHECK(eps >= 0, "eps must not be negative");
     const auto st = lo::ns_steps(coeffs);
     const c10::DeviceGuard guard(table.device());

@@ -356,6 +356,8 @@ def adam_ranges(ranges: AdamRanges, master: torch.Tensor, grad: torch.Tensor,
     """``adam_step`` on some ranges of the arena, in one launch."""
     if ranges.numel != master.numel():
         raise RuntimeError(f"the ranges are for {ranges.numel} elements")
+    if not _is_gpu(master):
+        _check_arena(master, grad, m1, m2, mirror)
     if _is_gpu(master):
         if not torch.is_tensor(step):
             step = torch.tensor([int(step)], dtype=torch.int32,
@@ -367,6 +369,15 @@ def adam_ranges(ranges: AdamRanges, master: torch.Tensor, grad: torch.Tensor,
     for a, b in ranges.ranges:
         adam_step(master[a:b], grad[a:b], m1[a:b], m2[a:b], mirror[a:b], lr,
                   b1, b2, eps, wd, step, gscale)
+
+
+def _check_arena(*tensors) -> None:
+    # the CPU path refuses what the kernels' bindings refuse
+    if any(t.numel() != tensors[0].numel() for t in tensors):
+        raise RuntimeError("the arena's tensors must match")
+    for i, a in enumerate(tensors):
+        if any(_touches(a, b) for b in tensors[:i]):
+            raise RuntimeError("the arena's tensors must not share memory")
 
 
 # ------------------------------------------------- Newton-Schulz and Muon
@@ -544,6 +555,7 @@ def muon_step(plan: MuonPlan, master: torch.Tensor, grad: torch.Tensor,
         if t.numel() != plan.numel or t.is_cuda:
             raise RuntimeError(f"the plan is for {plan.numel} elements on "
                                f"{plan.device}")
+    _check_arena(master, grad, mom, mirror)
     _ns_bounds(flat)
     for (off, m, n), gain in zip(plan.views, plan.gains):
         sl = slice(off, off + m * n)

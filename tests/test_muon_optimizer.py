@@ -399,3 +399,44 @@ def test_checkpoint_of_other_matrices(device, listed):
     with pytest.raises(ValueError):
         opt.load_state_dict({**sd, "m2": sd["m2"][:1]})
     assert torch.equal(opt.m2, saved.m2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_arenas_that_share_memory(device):
+    """One tensor in two places, or two that overlap, are refused before
+    anything is written."""
+    flat = torch.ones(5 * 64, device=device)
+    own = [flat[i * 64:(i + 1) * 64] for i in range(4)]
+    half = flat[256:].view(torch.bfloat16)[:64]
+    plan = F.MuonPlan([(0, 4, 8)], 64, device)
+    ranges = F.AdamRanges([(32, 64)], 64, device)
+    step = torch.ones(1, dtype=torch.int32, device=device)
+
+    def muon(t, mirror):
+        F.muon_step(plan, *t, mirror, lr=0.1)
+
+    def adam(t, mirror):
+        F.adam_ranges(ranges, *t, mirror, 0.1, 0.9, 0.99, 1e-8, 0.0, step)
+
+    for call, n in ((muon, 3), (adam, 4)):
+        for i in range(n):
+            for j in range(n):
+                for bad in (own[j], flat[j * 64 + 8:j * 64 + 72]):
+                    t = own[:n]
+                    t[i] = bad
+                    if i == j and bad is own[j] or i == n - 1 and j == n - 1:
+                        continue
+                    with pytest.raises(RuntimeError):
+                        call(t, half)
+            with pytest.raises(RuntimeError):
+                call(own[:n], own[i].view(torch.bfloat16)[30:94])
+        with pytest.raises(RuntimeError):
+            call([*own[:n - 1], own[n - 1][:56]], half)
+    assert bool((flat == 1).all())
+    muon(own[:3], half)
+    adam(own, half)
+    assert bool((own[0][:32] != 1).any()) and bool((own[0][32:] != 1).all())
+    if device == "cuda":
+        with pytest.raises(RuntimeError):
+            F.adam_ranges(ranges, *own, half, 0.1, 0.9, 0.99, 1e-8, 0.0,
+                          step[:0])
