@@ -679,19 +679,24 @@ class LayerNorm(Layer):
             }
         return self._bufs
 
+    def _rows(self, t: torch.Tensor) -> torch.Tensor:
+        # any view: the kernels take any row stride, but whole rows
+        t = t.reshape(self._bufs["M"], self.c)
+        return t if t.stride(1) == 1 or self.c == 1 else t.contiguous()
+
     def forward(self, x: torch.Tensor,
                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``residual``: normalise x + residual; the sum stays in
         ``self.sum`` (x's shape) for the skip path."""
         assert x.shape[-1] == self.c
         bufs = self._alloc(x)
-        x2 = x.reshape(bufs["M"], self.c)
+        x2 = self._rows(x)
         self._x2 = x2
         if residual is not None:
             if "sum" not in bufs:
                 bufs["sum"] = torch.empty_like(bufs["y"])
             self._x2 = bufs["sum"]
-            residual = residual.reshape(bufs["M"], self.c)
+            residual = self._rows(residual)
         F.layernorm_fwd(x2, self.arena.pf(self.name + ".g"),
                         self.arena.pf(self.name + ".b"), self.eps, bufs["y"],
                         mean=bufs["mean"], invstd=bufs["invstd"],
@@ -706,8 +711,8 @@ class LayerNorm(Layer):
         result is the gradient of x and of the residual alike."""
         bufs = self._bufs
         if dskip is not None:
-            dskip = dskip.reshape(bufs["M"], self.c)
-        F.layernorm_bwd(dy.reshape(bufs["M"], self.c), self._x2, bufs["mean"],
+            dskip = self._rows(dskip)
+        F.layernorm_bwd(self._rows(dy), self._x2, bufs["mean"],
                         bufs["invstd"], self.arena.pf(self.name + ".g"),
                         self.arena.g(self.name + ".g"),
                         self.arena.g(self.name + ".b"), bufs["dx"],

@@ -848,6 +848,9 @@ def _check_layernorm(x, rows, vecs, stats, outs, vec_ins, vec_outs) -> None:
                               or t.device != x.device):
             raise RuntimeError("activations must have the input's shape, "
                                "type and device")
+    if x.shape[1] > 1 and any(t is not None and t.stride(1) != 1
+                              for t in (x, *rows)):
+        raise RuntimeError("activations must be contiguous along their columns")
     for group, n in ((vecs, x.shape[1]), (stats, x.shape[0])):
         for t in group:
             if t is not None and (t.numel() != n or t.dtype != torch.float32

@@ -543,3 +543,36 @@ def test_vectors_share_no_memory_with_outputs(device):
     fwd(mean=near)
     want = t["sum"].double().mean(1)
     assert (near.double() - want).abs().max() <= 64 * U * t["sum"].abs().max()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layer_takes_any_view(device):
+    """Transposed and broadcast activations and gradients; the operators
+    themselves refuse columns that do not lie together."""
+    arena = ParamArena(device)
+    layer = LayerNorm("ln", 24)
+    layer.build(arena)
+    arena.finalize()
+    d = _data(30, 24, torch.bfloat16, device)
+    arena.pf("ln.g").copy_(d["gamma"])
+    want = layer.forward(d["x"], residual=d["residual"]).clone()
+    dx = layer.backward(d["dy"], dskip=d["dskip"]).clone()
+    turned = {k: d[k].t().contiguous().t()
+              for k in ("x", "residual", "dy", "dskip")}
+    y = layer.forward(turned["x"], residual=turned["residual"])
+    assert torch.equal(y, want)
+    assert torch.equal(layer.backward(turned["dy"], dskip=turned["dskip"]), dx)
+    once = d["dy"][:1, :1].expand(30, 24)
+    dx = layer.backward(once.contiguous()).clone()
+    assert torch.equal(layer.backward(once), dx)
+    five = turned["x"].view(5, 6, 24)
+    y = layer.forward(five).clone()
+    assert torch.equal(y, layer.forward(d["x"].view(5, 6, 24)))
+    x, g = turned["x"], d["gamma"]
+    st = torch.empty(30, device=device)
+    for call in (lambda: F.layernorm_fwd(x, g, g, EPS, torch.empty_like(d["x"])),
+                 lambda: F.layernorm_fwd(d["x"], g, g, EPS, x.clone()),
+                 lambda: F.layernorm_bwd(x, d["x"], st, st, g, g.clone(),
+                                         g.clone(), torch.empty_like(d["x"]))):
+        with pytest.raises(RuntimeError):
+            call()
