@@ -177,3 +177,33 @@ def test_muon_step(device, mats):
         tol = step * (8 * yard + 512 * U * norm(o)) + 4 * U * (norm(w)
                                                               + step * norm(o))
         assert norm(err) <= tol
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(64, 640), (24, 1000), (128, 640),
+                                   (640, 128), (300, 300)])
+@pytest.mark.parametrize("small", [1.0, 1e-2, 1e-4, 1e-6, 1e-8])
+def test_rows_far_below_the_norm(device, shape, small):
+    """Half of the short side's rows are scaled down. What fp32 keeps relative
+    to a row, two fp16 halves keep down to half a step of the lower half's
+    scale: 2^-25 / 2^14 = 2^-39 for X and A, whose scale is 2^14, and 2^-38 for
+    C. On n columns and m rows, a step takes from a row sqrt(n) 2^-39 through X,
+    and sqrt(m) |X| <= 1.21 sqrt(m) times what an element of C is off by: its
+    own 2^-38, |b| 2^-39 and 2 |c| 1.21^2 2^-39 through A. That is below
+    (sqrt(n) + 16 sqrt(m)) 2^-39, and what a row loses in one step grows by
+    a in each later one, 1 + a + ... + a^4 = 200."""
+    gen = torch.Generator().manual_seed(4)
+    m, n = shape
+    g = torch.randn(m, n, generator=gen)
+    tall = m > n
+    (g.T if tall else g)[::2] *= small
+    got = F.orthogonalize(g.to(device)).double().cpu()
+    ref = _steps(g, torch.float64)
+    yard = (_steps(g, torch.float32).double() - ref)
+    got, ref, yard = (t.T if tall else t for t in (got, ref, yard))
+    m, n = ref.shape
+    size = ref.norm(dim=1)
+    tol = 8 * yard.norm(dim=1) + 512 * U * size \
+        + 200 * (math.sqrt(n) + 16 * math.sqrt(m)) * 2.0 ** -39
+    err = (got - ref).norm(dim=1)
+    assert bool((err <= tol).all()), f"off by {(err / tol).max():.2f} tolerances"
