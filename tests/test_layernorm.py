@@ -576,3 +576,61 @@ def test_layer_takes_any_view(device):
                                          g.clone(), torch.empty_like(d["x"]))):
         with pytest.raises(RuntimeError):
             call()
+
+
+# Both ways to the sums of wide rows' gradients, a row above and at the limit
+# between them: taken along by the kernel that writes dx, one owner a column, or
+# down the columns before it. All threads a row (256, 1024) and vectors a thread
+# of each type. A thread adds at most rows/256 + 1 rows in turn (256 blocks of a
+# row each, or 64 of four), and 100 covers the joins: 24 + 32 of 768 blocks' sums.
+B, H, S = torch.bfloat16, torch.float16, torch.float32
+WIDE = [(B, 3072, 1030), (B, 3072, 4095), (B, 2048, 4100), (B, 2048, 8200),
+        (H, 3072, 2050), (H, 2048, 8191), (H, 2048, 9001),
+        (S, 1536, 1001), (S, 1536, 1030), (S, 512, 2050), (S, 512, 4100),
+        (S, 512, 8195)]
+
+
+def _wide_check(d, s, o, g, dtype, dskip):
+    ref, tol = _reference(s, d, dtype, dskip)
+    depth = (s.shape[0] / 256 + 101) * U
+    x, dy = s.double().cpu(), d["dy"].double().cpu()
+    invstd = ref["invstd"].view(-1, 1)
+    xhat = (x - ref["mean"].view(-1, 1)) * invstd
+    ex = U * (64 * invstd * x.abs().mean(1, keepdim=True) + 40 * xhat.abs())
+    tol["dgamma"] = depth * (dy * xhat).abs().sum(0) + (dy.abs() * ex).sum(0)
+    tol["dbeta"] = depth * dy.abs().sum(0)
+    _close(o["y"], ref["y"], tol["y"], "y")
+    for k in ("dx", "dgamma", "dbeta"):
+        _close(g[k], ref[k], tol[k], k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("skip", [False, True])
+@pytest.mark.parametrize("more", [0, 1])
+@pytest.mark.parametrize("dtype,rows,cols", WIDE)
+def test_sums_of_wide_rows(dtype, rows, cols, more, skip):
+    d = _data(rows + more, cols, dtype, "cuda")
+    s, o = _forward(d, skip)
+    g = _backward(s, o, d, skip)
+    _wide_check(d, s, o, g, dtype, d["dskip"] if skip else None)
+    for onto in ("dy", "x", "dskip")[:2 + skip]:
+        e = {"dy": d["dy"].clone(), "x": s.clone(), "dskip": d["dskip"].clone()}
+        dg, db = (torch.full_like(d["gamma"], 7.0) for _ in range(2))
+        F.layernorm_bwd(e["dy"], e["x"], o["mean"], o["invstd"], d["gamma"], dg,
+                        db, e[onto], dskip=e["dskip"] if skip else None)
+        assert torch.equal(e[onto], g["dx"]), onto
+        assert torch.equal(dg, g["dgamma"]) and torch.equal(db, g["dbeta"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 1001), (1, 2050), (1, 4100),
+                                       (1, 9000), (1, 16384), (1, 32768),
+                                       (300, 20000), (515, 32768)])
+def test_one_wide_row_and_the_widest(dtype, rows, cols):
+    """One block writes its sums itself; rows of more than 16 elements a thread
+    leave them to the pass down the columns."""
+    d = _data(rows, cols, dtype, "cuda")
+    s, o = _forward(d, True)
+    g = _backward(s, o, d, True)
+    _wide_check(d, s, o, g, dtype, d["dskip"])
