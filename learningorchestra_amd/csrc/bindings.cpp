@@ -596,27 +596,42 @@ void adam_step(at::Tensor master, at::Tensor grad, at::Tensor m1, at::Tensor m2,
                   (float)wd, (float)gscale, stream());
 }
 
-// whether some row of t (cut to its columns) shares memory with vec
-bool touches(const at::Tensor& t, const at::Tensor& vec) {
-  if (t.numel() == 0 || vec.numel() == 0) return false;
-  const bool flat = t.dim() < 2;
-  const int64_t size = t.itemsize();
-  const int64_t row = flat || t.size(0) < 2 ? 0 : t.stride(0) * size;
-  const int64_t rows = row ? t.size(0) : 1;
-  const int64_t width = (flat ? t.numel() : t.size(1)) * size;
-  const auto at = (int64_t)t.data_ptr(), v = (int64_t)vec.data_ptr();
-  // the first row that ends behind vec's start
-  const int64_t r = row && v - at >= width ? (v - at - width) / row + 1 : 0;
-  return r < rows && at + r * row < v + (int64_t)vec.nbytes() &&
-         at + r * row + width > v;
+// where a tensor's rows (one, if it is flat) lie, in bytes; none: no rows
+struct Span {
+  int64_t at = 0, width = 0, row = 0, rows = 0, end = 0;
+  const char* name = "";
+  Span() = default;
+  Span(const at::Tensor& t, const char* name_) : name(name_) {
+    if (t.numel() == 0) return;
+    const auto sizes = t.sizes();
+    const int64_t size = t.itemsize();
+    const bool flat = sizes.size() != 2;  // and contiguous
+    at = (int64_t)t.const_data_ptr();
+    width = (flat ? t.numel() : sizes[1]) * size;
+    row = flat || sizes[0] < 2 ? 0 : t.strides()[0] * size;
+    rows = row ? sizes[0] : 1;
+    end = at + (rows - 1) * row + width;
+  }
+  Span(const c10::optional<at::Tensor>& t, const char* name_) {
+    if (t) *this = Span(*t, name_);
+  }
+};
+
+// whether some row of a shares memory with v, which has one row
+bool touches(const Span& a, const Span& v) {
+  if (a.rows == 0 || v.rows == 0 || a.end <= v.at || v.end <= a.at) return false;
+  // the first row that ends behind v's start
+  const int64_t gap = v.at - a.at - a.width;
+  const int64_t r = a.row && gap >= 0 ? gap / a.row + 1 : 0;
+  return a.at + r * a.row < v.end;
 }
 
 // an arena's tensors, all contiguous
-void check_arena(std::initializer_list<const at::Tensor*> ts) {
+void check_arena(std::initializer_list<Span> ts) {
   for (auto a = ts.begin(); a != ts.end(); ++a)
     for (auto b = ts.begin(); b != a; ++b)
-      TORCH_CHECK(!touches(**a, **b),
-                  "the arena's tensors must not share memory");
+      TORCH_CHECK(!touches(*a, *b), "the arena's ", b->name, " and ", a->name,
+                  " must not share memory");
 }
 
 // what an object keeps may be used on another stream than it was made on: its
@@ -652,7 +667,8 @@ void adam_ranges(at::Tensor master, at::Tensor grad, at::Tensor m1,
                   ranges.size(0) <= 65535,
               "ranges must be int64 [k, 2] on the arena's GPU");
   TORCH_CHECK(step_dev.numel() == 1, "step_dev must hold one value");
-  check_arena({&master, &grad, &m1, &m2, &mirror});
+  check_arena({{master, "master"}, {grad, "grad"}, {m1, "m1"}, {m2, "m2"},
+               {mirror, "mirror"}});
   if (ranges.size(0) == 0 || longest <= 0) return;
   const c10::DeviceGuard guard(master.device());
   used_here({ranges});
@@ -818,30 +834,21 @@ void check_vec(const at::Tensor& t, const at::Tensor& like, int64_t n,
   TORCH_CHECK(t.numel() == n, name, " must hold ", n, " values");
 }
 
-struct Named {
-  const char* name;
-  const at::Tensor* t;  // or null
-};
-
 // statistics and parameters' gradients share no memory with anything else, nor
 // do the activations' outputs with statistics and parameters
-void check_own(const Named& vec_out0, const Named& vec_out1,
-               std::initializer_list<Named> vecs,
-               std::initializer_list<Named> outs,
-               std::initializer_list<Named> ins) {
-  auto apart = [](const Named& a, const Named& b) {
-    TORCH_CHECK(!a.t || !b.t || !touches(*a.t, *b.t), a.name, " and ", b.name,
+void check_own(const Span& vec_out0, const Span& vec_out1,
+               std::initializer_list<Span> vecs,
+               std::initializer_list<Span> outs,
+               std::initializer_list<Span> ins) {
+  auto apart = [](const Span& a, const Span& b) {
+    TORCH_CHECK(!touches(a, b), a.name, " and ", b.name,
                 " must not share memory");
   };
   apart(vec_out0, vec_out1);
   for (const auto* others : {&vecs, &outs, &ins})
-    for (const Named& o : *others) apart(o, vec_out0), apart(o, vec_out1);
-  for (const Named& o : outs)
-    for (const Named& v : vecs) apart(o, v);
-}
-
-const at::Tensor* given(const c10::optional<at::Tensor>& t) {
-  return t ? &*t : nullptr;
+    for (const Span& o : *others) apart(o, vec_out0), apart(o, vec_out1);
+  for (const Span& o : outs)
+    for (const Span& v : vecs) apart(o, v);
 }
 
 constexpr int64_t kLayerNormCols = 32768;  // a row fits one block's registers
@@ -882,10 +889,10 @@ void layernorm_fwd(at::Tensor x, at::Tensor gamma, at::Tensor beta, double eps,
     check_apart(*sum_out, *residual, "sum_out");
     check_apart(*sum_out, out, "sum_out");
   }
-  check_own({"mean", given(mean)}, {"invstd", given(invstd)},
-            {{"gamma", &gamma}, {"beta", &beta}},
-            {{"out", &out}, {"sum_out", given(sum_out)}},
-            {{"x", &x}, {"residual", given(residual)}});
+  check_own({mean, "mean"}, {invstd, "invstd"},
+            {{gamma, "gamma"}, {beta, "beta"}},
+            {{out, "out"}, {sum_out, "sum_out"}},
+            {{x, "x"}, {residual, "residual"}});
   if (rows == 0) return;
   const c10::DeviceGuard guard(x.device());
   lo::launch_layernorm_fwd(
@@ -918,9 +925,9 @@ void layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor mean,
   check_vec(gamma, x, cols, "gamma");
   check_vec(dgamma, x, cols, "dgamma");
   check_vec(dbeta, x, cols, "dbeta");
-  check_own({"dgamma", &dgamma}, {"dbeta", &dbeta},
-            {{"gamma", &gamma}, {"mean", &mean}, {"invstd", &invstd}},
-            {{"dx", &dx}}, {{"dy", &dy}, {"x", &x}, {"dskip", given(dskip)}});
+  check_own({dgamma, "dgamma"}, {dbeta, "dbeta"},
+            {{gamma, "gamma"}, {mean, "mean"}, {invstd, "invstd"}},
+            {{dx, "dx"}}, {{dy, "dy"}, {x, "x"}, {dskip, "dskip"}});
   const c10::DeviceGuard guard(x.device());
   if (rows == 0) {
     dgamma.zero_();
@@ -1116,7 +1123,8 @@ struct MuonPlan {
       TORCH_CHECK(t.device() == table.device(), "the plan is on ",
                   table.device());
     }
-    check_arena({&master, &grad, &mom, &mirror});
+    check_arena({{master, "master"}, {grad, "grad"}, {mom, "mom"},
+                 {mirror, "mirror"}});
     TORCH_CHECK(eps >= 0, "eps must not be negative");
     const auto st = lo::ns_steps(coeffs);
     const c10::DeviceGuard guard(table.device());
