@@ -52,7 +52,7 @@
 //                      between the dies (X is 67 MB) bound it.
 //   ResNet-50's matrices, a whole step: 929 to 1006 us, of which 118 move the
 //                      momentum, the update and X's first form at 5 TB/s
-//   256 x 3136 bf16    107 us for 17 launches of 4 to 9 us, of which some 3.5
+//   256 x 3136 bf16    108 us for 17 launches of 4 to 9 us, of which some 3.5
 //                      are the launch, the first loads and the end
 
 #include <type_traits>

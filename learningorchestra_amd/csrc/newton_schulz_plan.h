@@ -14,7 +14,10 @@
 namespace lo {
 
 constexpr int64_t kNsSide = 1 << 20;
-constexpr int64_t kNsSlots = 512;  // blocks that run at once: two on each CU
+// Blocks that run at once at two on each CU, as 128 x 128 tiles run. 64 x 64
+// tiles beyond them run three a CU (ns_product_kernel's MANY); what a single
+// matrix leaves over is counted in these rounds all the same.
+constexpr int64_t kNsSlots = 512;
 
 inline int64_t ns_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
@@ -143,17 +146,21 @@ inline bool ns_fit_block(int shortest, int longest) {
   return shortest <= 32 ? longest <= 2048 : shortest <= 64 && longest <= 1024;
 }
 
-// What a tile size costs, in microseconds, fitted to launches of single
-// products with 3 to 1300 tiles and 8 to 128 steps, to rank the choices by: a
+// What a tile size costs, in microseconds, to rank the choices by, fitted to
+// launches of single products with 3 to 1300 tiles and 8 to 128 steps (but for
+// 64's shared step, see below): a
 // launch with its first loads and its end; a step of 32 values of the sum (8,
 // 16 or 32 KiB of operands) in a block alone on its CU; a step and a block's
 // own start and end where several blocks share one; handing over the parts of
 // a split sum, for each part that the last block adds and for each part on the
 // chip. So 256 x 3136 took 232 us with every sum split, 150 us with only deep
 // ones split on 64 x 64 tiles, and 115 us with A and C on 32 x 32; 512 x 512
-// 148 us on 64 x 64 tiles and 95 us on 32 x 32. ResNet-50's group takes 979 us
-// with A and C on 64 x 64 tiles, 1033 us with A on 128 x 128; 2048 x 2048 653
-// us with A and C on 64 x 64, 748 us on 128 x 128.
+// 148 us on 64 x 64 tiles and 95 us on 32 x 32.
+// A step of 64 x 64 tiles that share a CU is 0.22 us at two blocks a CU; three
+// take the 0.19 here, set by whole calls and used for all such launches:
+// ResNet-50's group takes 979 us with A and C on 64 x 64 tiles, 1033 us with A
+// on 128 x 128; 2048 x 2048 653 us with A and C on 64 x 64, 748 us on
+// 128 x 128; with 0.16, 12 x 768 x 768 went from 477 to 512 us.
 struct NsCost {
   int tile;
   double launch, alone, step, block, join, add, part;

@@ -499,7 +499,7 @@ class MuonPlan:
     cols), offsets being multiples of 8 as ParamArena's are. On a GPU it owns
     the kernels' tables and their workspace (about 8 bytes an element for wide
     matrices), so steps that share a plan have to be ordered, like steps that
-    share a momentum.
+    share a momentum, and the plan has to outlive graphs that captured them.
 
     ``sides`` lists the matrices' own (rows, cols) where the stored ones count
     rows or columns of padding, which hold zeros: the factor on the learning
