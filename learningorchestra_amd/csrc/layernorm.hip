@@ -123,6 +123,13 @@ LO_DEVICE void row_sum(float (&v)[K], float* red, int& turn) {
   }
 }
 
+// a * b, rounded: fused into the sum that follows, dy * gamma would not be the
+// value that its mean was taken of, and what is left of it, times invstd, would
+// stand where dx is zero (rows of one column)
+LO_DEVICE float rounded_product(float a, float b) {
+  return __builtin_fmaf(a, b, 0.f);
+}
+
 constexpr int ln_block(int tpr) { return tpr > 256 ? tpr : 256; }
 
 // gamma and beta stay in registers for all of a block's rows, but where a row
@@ -295,7 +302,7 @@ __global__ __launch_bounds__(ln_block(TPR)) void layernorm_bwd_kernel(
       for (int j = 0; j < VE; ++j) {
         const float g = j >= skip[i] ? elem<VE>(gv[i], j) : 0.f;
         const float xh = (elem<VE>(xv[i], j) - mu) * is;
-        const float h = g * ga[j];
+        const float h = rounded_product(g, ga[j]);
         s[0] += h;
         s[1] += j >= skip[i] ? h * xh : 0.f;
         if constexpr (SUMS) {
@@ -315,7 +322,7 @@ __global__ __launch_bounds__(ln_block(TPR)) void layernorm_bwd_kernel(
       #pragma unroll
       for (int j = 0; j < VE; ++j) {
         const float xh = (elem<VE>(xv[i], j) - mu) * is;
-        const float h = elem<VE>(gv[i], j) * ga[j];
+        const float h = rounded_product(elem<VE>(gv[i], j), ga[j]);
         float d = is * (h - c1 - xh * c2);
         if (skipg) d += elem<VE>(kv[i], j);
         if constexpr (VE == 1) o = (T)d;

@@ -634,3 +634,21 @@ def test_one_wide_row_and_the_widest(dtype, rows, cols):
     s, o = _forward(d, True)
     g = _backward(s, o, d, True)
     _wide_check(d, s, o, g, dtype, d["dskip"])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 70, 5000])
+def test_one_column(device, dtype, rows):
+    """A single value is its own mean: y is beta, dx nothing or dskip, and
+    dgamma nothing, all of them to the bit."""
+    d = _data(rows, 1, dtype, device)
+    s, o = _forward(d, True)
+    assert torch.equal(o["y"], d["beta"].to(dtype).expand(rows, 1))
+    assert torch.equal(o["mean"], s[:, 0].float())
+    g = _backward(s, o, d, True)
+    assert torch.equal(g["dx"], d["dskip"])
+    assert bool((_backward(s, o, d, False)["dx"] == 0).all())
+    assert float(g["dgamma"]) == 0
+    ref, tol = _reference(s, d, dtype)
+    _close(g["dbeta"], ref["dbeta"], tol["dbeta"], "dbeta")
