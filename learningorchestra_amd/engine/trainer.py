@@ -25,6 +25,26 @@ def _fn_params(fn):
         return {}
 
 
+def _held_tensors(obj, seen=None) -> list:
+    """Every tensor that a model's objects hold, layers' buffers included."""
+    seen = {} if seen is None else seen
+    if id(obj) in seen:
+        return []
+    if isinstance(obj, torch.Tensor):
+        seen[id(obj)] = obj
+        return [obj]
+    if isinstance(obj, dict):
+        inner = list(obj.values())
+    elif isinstance(obj, (list, tuple, set)):
+        inner = list(obj)
+    elif type(obj).__module__.startswith(__name__.split(".")[0]):
+        inner = list(getattr(obj, "__dict__", {}).values())
+    else:
+        return []
+    seen[id(obj)] = obj
+    return [t for v in inner for t in _held_tensors(v, seen)]
+
+
 class Trainer:
     def __init__(self, model: SequentialClassifier, optimizer, device="cpu",
                  use_graph: bool = False):
@@ -41,6 +61,10 @@ class Trainer:
         self._graph = None          # world==1: whole step; world>1: fwd+bwd
         self._graph_opt = None      # world>1: optimizer + mirror refresh
         self._split = False         # world>1 split-graph mode
+        # what the graphs write to: layers replace their buffers when another
+        # batch size comes by (a prediction, say), and memory that they let go
+        # would be other tensors' by the next replay
+        self._graph_held = []
         self._static_x = None
         self._static_y = None
         # oversubscribed runs (more ranks than GPUs) serialize device work
@@ -194,6 +218,7 @@ class Trainer:
                                   capture_error_mode="thread_local"):
                 self._opt_body()
             torch.cuda.synchronize()
+            self._graph_held = _held_tensors(self.model)
             return
         for _ in range(3):
             self._step_body(self._static_x, self._static_y)
@@ -202,6 +227,7 @@ class Trainer:
         with torch.cuda.graph(self._graph):
             self._step_body(self._static_x, self._static_y)
         torch.cuda.synchronize()
+        self._graph_held = _held_tensors(self.model)
 
     # -- in-training checkpoint/resume (the reference had no
     # epoch-level resume; fit was atomic) --------------------------------

@@ -15,7 +15,8 @@ from learningorchestra_amd.engine.layers import (Conv2dNHWC, Flatten,
                                                  LayerNorm, Linear,
                                                  MaxPool2dNHWC,
                                                  SequentialClassifier)
-from learningorchestra_amd.engine.trainer import Trainer, make_muon
+from learningorchestra_amd.engine.trainer import (Trainer, _held_tensors,
+                                                  make_muon)
 from learningorchestra_amd.models.mnist_cnn import build_mnist_cnn
 from learningorchestra_amd.models.resnet import ResNet
 from learningorchestra_amd.models.tabular import MLPClassifier
@@ -440,3 +441,42 @@ def test_arenas_that_share_memory(device):
         with pytest.raises(RuntimeError):
             F.adam_ranges(ranges, *own, half, 0.1, 0.9, 0.99, 1e-8, 0.0,
                           step[:0])
+
+
+def test_held_tensors():
+    """All that a model's layers keep, whatever holds it."""
+    m = build_textcnn("cpu", vocab=50, emb_dim=32, filters=64, layer_norm=True)
+    ids, y = imdb_batch(4, seq_len=12, vocab=50, seed=0)
+    m.train_step(ids, y)
+    held = {id(t) for t in _held_tensors(m)}
+    for lay in (m.ln_emb, m.ln_cat, *m.convs, m.fc):
+        bufs = [t for t in lay._bufs.values() if isinstance(t, torch.Tensor)]
+        assert bufs and all(id(t) in held for t in bufs)
+    assert all(id(t) in held for t in (m.arena.master, m.arena.mirror,
+                                       m.arena.grad, m.emb._out, m.loss_sum))
+
+
+@pytest.mark.gpu
+def test_predictions_between_captured_steps():
+    """Another batch size between replays: the layers' buffers are replaced, and
+    the captured step neither loses its own nor writes to new tensors."""
+    gen = torch.Generator().manual_seed(9)
+    x = torch.randn(96, 48, generator=gen).bfloat16().cuda()
+    y = torch.randint(0, 10, (96,), generator=gen).cuda()
+    twin, m = _network("cuda"), _network("cuda")
+    eager = Trainer(twin, make_muon(twin, exclude=("fc2.w",)), "cuda")
+    graph = Trainer(m, make_muon(m, exclude=("fc2.w",)), "cuda", use_graph=True)
+    graph.step_async(x, y)          # warms up with three steps and captures
+    for _ in range(3):
+        eager.step_async(x, y)
+    assert graph._graph is not None
+    own = {t.data_ptr() for t in graph._graph_held}
+    m.predict(x[:40])
+    new = [torch.full_like(t, 3) for t in graph._graph_held for _ in range(3)]
+    assert not own & {t.data_ptr() for t in new}
+    for n in (40, 17, 96):
+        graph.step_async(x, y)
+        eager.step_async(x, y)
+        assert torch.equal(m.predict(x[:n]), twin.predict(x[:n]))
+        assert torch.equal(m.arena.master, twin.arena.master)
+    assert all(bool((t == 3).all()) for t in new)
