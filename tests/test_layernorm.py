@@ -578,16 +578,16 @@ def test_layer_takes_any_view(device):
             call()
 
 
-# Both ways to the sums of wide rows' gradients, a row above and at the limit
-# between them: taken along by the kernel that writes dx, one owner a column, or
-# down the columns before it. All threads a row (256, 1024) and vectors a thread
+# Both ways to the sums of wide rows' gradients, a row below and above the limit
+# between them: down the columns before dx is written, or taken along by the
+# kernel that writes it, one owner a column. All threads a row (256, 1024) and vectors a thread
 # of each type. A thread adds at most rows/256 + 1 rows in turn (256 blocks of a
 # row each, or 64 of four), and 100 covers the joins: 24 + 32 of 768 blocks' sums.
 B, H, S = torch.bfloat16, torch.float16, torch.float32
-WIDE = [(B, 3072, 1030), (B, 3072, 4095), (B, 2048, 4100), (B, 2048, 8200),
-        (H, 3072, 2050), (H, 2048, 8191), (H, 2048, 9001),
-        (S, 1536, 1001), (S, 1536, 1030), (S, 512, 2050), (S, 512, 4100),
-        (S, 512, 8195)]
+WIDE = [(B, 3071, 1030), (B, 3071, 4095), (B, 2047, 4100), (B, 2047, 8200),
+        (H, 3071, 2050), (H, 2047, 8191), (H, 2047, 9001),
+        (S, 1535, 1001), (S, 1535, 1030), (S, 511, 2050), (S, 511, 4100),
+        (S, 511, 8195)]
 
 
 def _wide_check(d, s, o, g, dtype, dskip):
@@ -606,7 +606,7 @@ def _wide_check(d, s, o, g, dtype, dskip):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("skip", [False, True])
-@pytest.mark.parametrize("more", [0, 1])
+@pytest.mark.parametrize("more", [0, 2])
 @pytest.mark.parametrize("dtype,rows,cols", WIDE)
 def test_sums_of_wide_rows(dtype, rows, cols, more, skip):
     d = _data(rows + more, cols, dtype, "cuda")
