@@ -463,10 +463,9 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS,
 
     ``coeffs``: (a, b, c), or a triple for each step. Refused are those that
     can bring a singular value past 2^20 or, before a step, below 2^-20, and
-    polynomials a + b q + c q^2 that stay below 2^-40.
-    A zero matrix stays zero. A view that is not contiguous is copied first.
-    The same call gives the same bits; batches of other sizes may sum in
-    another order."""
+    polynomials a + b q + c q^2 that stay below 2^-40. A zero matrix stays zero.
+    A view that is not contiguous is copied first. The same call gives the same
+    bits; batches of other sizes may sum in another order."""
     flat = _ns_coeffs(steps, coeffs, eps)
     if g.dim() < 2:
         raise ValueError("g must be a matrix or a batch of them")
@@ -553,8 +552,9 @@ def muon_step(plan: MuonPlan, master: torch.Tensor, grad: torch.Tensor,
         mom <- mu mom + gscale g;  U = gscale g + mu mom (nesterov) or mom
         w <- (1 - lr wd) w - lr sqrt(max(1, rows / cols)) orthogonalize(U)
 
-    where rows and cols are the plan's ``sides``. Elements outside the matrices stay as they are. Every rank that starts
-    from the same values ends with the same values."""
+    where rows and cols are the plan's ``sides``. Elements outside the matrices
+    stay as they are. Every rank that starts from the same values ends with the
+    same values."""
     flat = _ns_coeffs(steps, coeffs, eps)
     if plan._native is not None:
         plan._native.step(master, grad, mom, mirror, lr, mu, wd, gscale,
